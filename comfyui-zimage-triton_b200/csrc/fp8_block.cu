@@ -1,0 +1,294 @@
+// Matrix products in 8-bit floating point (e4m3) with one scale for each block of 128.
+//
+// Quantiser: a block of values (1 x 128 of an activation row, 128 x 128 of a weight) with largest
+// magnitude a is held as e4m3 values q = x / s, s = 2^e with the least e >= -120 such that
+// a <= 448 s.  A power of two makes the division exact, so q is the one rounding of x to e4m3's
+// 4-bit mantissa (ties to even) and any implementation gives the same bits; as the format floats,
+// scales between the powers would gain no precision but at the bottom of its range.  A block with
+// an infinity or a NaN gets NaN for its scale and its values.
+//
+// Product: y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} q[m, k] w[n, k] (+ bias[n]),
+// the scales being any fp32 values; sums in fp32, rounded once to the output type.
+#include "zib_async.cuh"
+#include "zib_types.cuh"
+
+#include <cuda_fp8.h>
+
+namespace zib {
+namespace fp8 {
+
+constexpr int kBlock = 128;
+
+// e with s = 2^e for a block's largest magnitude (given as its fp32 bits: NaN > infinity > finite)
+__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
+  if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+  // a = m 2^k with m in [1, 2); 448 = 1.75 * 2^8
+  int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  if (e < -120) e = -120;
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+// 1 / s, exact for a power of two
+__device__ __forceinline__ float inverse_scale(float s) {
+  const uint32_t b = __float_as_uint(s);
+  return b >= 0x7F800000u ? s : __uint_as_float((254u << 23) - b);
+}
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
+  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float from_e4m3(uint8_t v) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+}
+
+// one warp per (row, block)
+template <typename T>
+__global__ void __launch_bounds__(256) quant_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
+                                                         int64_t ldq, float* __restrict__ s, int64_t s_m, int64_t s_k,
+                                                         int64_t M, int64_t K) {
+  const int lane = threadIdx.x & 31;
+  const int64_t kb = (K + kBlock - 1) / kBlock;
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (id >= M * kb) return;
+  const int64_t m = id / kb, b = id - m * kb;
+  float v[4];
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = b * kBlock + lane + 32 * i;
+    v[i] = k < K ? to_f32(x[m * ldx + k]) : 0.0f;
+    const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+    a = bits > a ? bits : a;
+  }
+  a = __reduce_max_sync(0xFFFFFFFFu, a);
+  const float sc = block_scale(a), inv = inverse_scale(sc);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = b * kBlock + lane + 32 * i;
+    if (k < K) q[m * ldq + k] = to_e4m3(v[i] * inv);
+  }
+  if (lane == 0) s[m * s_m + b * s_k] = sc;
+}
+
+// one CTA per 128 x 128 block
+template <typename T>
+__global__ void __launch_bounds__(256) quant_blocks_kernel(const T* __restrict__ w, int64_t ldw,
+                                                           uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s,
+                                                           int64_t s_n, int64_t s_k, int64_t N, int64_t K) {
+  __shared__ uint32_t red[8];
+  const int64_t n0 = (int64_t)blockIdx.y * kBlock, k = (int64_t)blockIdx.x * kBlock + (threadIdx.x & 127);
+  uint32_t a = 0;
+  for (int r = threadIdx.x >> 7; r < kBlock; r += 2) {
+    if (n0 + r < N && k < K) {
+      const uint32_t bits = __float_as_uint(to_f32(w[(n0 + r) * ldw + k])) & 0x7FFFFFFFu;
+      a = bits > a ? bits : a;
+    }
+  }
+  a = __reduce_max_sync(0xFFFFFFFFu, a);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = red[i] > a ? red[i] : a;
+  const float sc = block_scale(a), inv = inverse_scale(sc);
+  for (int r = threadIdx.x >> 7; r < kBlock; r += 2)
+    if (n0 + r < N && k < K) q[(n0 + r) * ldq + k] = to_e4m3(to_f32(w[(n0 + r) * ldw + k]) * inv);
+  if (threadIdx.x == 0) s[blockIdx.y * s_n + blockIdx.x * s_k] = sc;
+}
+
+// 64 x 64 output tile per CTA, 4 x 4 per thread
+template <typename T>
+__global__ void __launch_bounds__(256) gemm_simple_kernel(const uint8_t* __restrict__ q, int64_t ldq,
+                                                          const float* __restrict__ sx, int64_t sx_m, int64_t sx_k,
+                                                          const uint8_t* __restrict__ w, int64_t ldw,
+                                                          const float* __restrict__ sw, int64_t sw_n, int64_t sw_k,
+                                                          const T* __restrict__ bias, T* __restrict__ y, int64_t ldy,
+                                                          int64_t M, int64_t N, int64_t K) {
+  __shared__ float a[16][65], b[16][65];
+  const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float acc[4][4] = {}, part[4][4] = {};
+  for (int64_t k0 = 0; k0 < K; k0 += 16) {
+    for (int i = threadIdx.x; i < 1024; i += 256) {
+      const int r = i >> 4, c = i & 15;
+      a[c][r] = m0 + r < M && k0 + c < K ? from_e4m3(q[(m0 + r) * ldq + k0 + c]) : 0.0f;
+      b[c][r] = n0 + r < N && k0 + c < K ? from_e4m3(w[(n0 + r) * ldw + k0 + c]) : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(a[k][ty * 4 + i], b[k][tx * 4 + j], part[i][j]);
+    __syncthreads();
+    if ((k0 + 16) % kBlock == 0 || k0 + 16 >= K) {  // a block of 128 is complete
+      const int64_t kb = k0 / kBlock;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
+          if (m < M && n < N)
+            acc[i][j] = fmaf(part[i][j], sx[m * sx_m + kb * sx_k] * sw[n / kBlock * sw_n + kb * sw_k], acc[i][j]);
+          part[i][j] = 0.0f;
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
+      if (m < M && n < N) y[m * ldy + n] = from_f32<T>(acc[i][j] + (bias ? to_f32(bias[n]) : 0.0f));
+    }
+}
+
+// wt[k, n] = w[n, k], 64 x 64 bytes per CTA
+__global__ void __launch_bounds__(256) transpose_kernel(const uint8_t* __restrict__ w, int64_t ldw,
+                                                        uint8_t* __restrict__ wt, int64_t ldt, int64_t N, int64_t K) {
+  __shared__ uint8_t t[64][68];
+  const int64_t n0 = (int64_t)blockIdx.y * 64, k0 = (int64_t)blockIdx.x * 64;
+  for (int i = threadIdx.x; i < 4096; i += 256) {
+    const int r = i >> 6, c = i & 63;
+    if (n0 + r < N && k0 + c < K) t[r][c] = w[(n0 + r) * ldw + k0 + c];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 4096; i += 256) {
+    const int r = i >> 6, c = i & 63;
+    if (k0 + r < K && n0 + c < N) wt[(k0 + r) * ldt + n0 + c] = t[c][r];
+  }
+}
+
+// column sums of x [M, N] in fp32 (a bias gradient): partial sums of row slabs, then their sums
+template <typename T>
+__global__ void __launch_bounds__(256) col_sum_part_kernel(const T* __restrict__ x, int64_t ldx,
+                                                           float* __restrict__ part, int64_t M, int64_t N,
+                                                           int64_t slab) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  const int64_t m1 = ((int64_t)blockIdx.y + 1) * slab < M ? ((int64_t)blockIdx.y + 1) * slab : M;
+  float s = 0.0f;
+  for (int64_t m = (int64_t)blockIdx.y * slab; m < m1; ++m) s += to_f32(x[m * ldx + n]);
+  part[blockIdx.y * N + n] = s;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) col_sum_kernel(const float* __restrict__ part, T* __restrict__ y, int64_t N,
+                                                      int slabs) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  double s = 0.0;
+  for (int i = 0; i < slabs; ++i) s += part[i * N + n];
+  y[n] = from_f32<T>((float)s);
+}
+
+constexpr int kMaxSlabs = 64;
+
+}  // namespace fp8
+}  // namespace zib
+
+using namespace zib;
+
+extern "C" int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m,
+                                  int64_t s_k, int64_t M, int64_t K, void* stream) {
+  const char* what = "zib_fp8_quant_rows";
+  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
+  ZIB_HOST_CHECK(M >= 0 && K >= 1 && ldx >= K && ldq >= K, ZIB_ERR_INVALID_ARG, "%s: bad shape M=%lld K=%lld", what,
+                 (long long)M, (long long)K);
+  if (M == 0) return ZIB_OK;
+  ZIB_HOST_CHECK(x && q && s, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+  const int64_t grid = ceil_div(M * ceil_div(K, fp8::kBlock), 8);
+  ZIB_HOST_CHECK(grid <= 0x7FFFFFFF, ZIB_ERR_TOO_LARGE, "%s: M=%lld K=%lld", what, (long long)M, (long long)K);
+  cudaStream_t st = (cudaStream_t)stream;
+  const unsigned g = (unsigned)grid;
+  if (dtype == ZIB_BF16)
+    fp8::quant_rows_kernel<<<g, 256, 0, st>>>((const __nv_bfloat16*)x, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
+  else if (dtype == ZIB_F16)
+    fp8::quant_rows_kernel<<<g, 256, 0, st>>>((const __half*)x, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
+  else
+    fp8::quant_rows_kernel<<<g, 256, 0, st>>>((const float*)x, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
+  return zib_check_launch(what);
+}
+
+extern "C" int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void* q, int64_t ldq, float* s, int64_t s_n,
+                                    int64_t s_k, int64_t N, int64_t K, void* stream) {
+  const char* what = "zib_fp8_quant_blocks";
+  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
+  ZIB_HOST_CHECK(N >= 1 && K >= 1 && ldw >= K && ldq >= K, ZIB_ERR_INVALID_ARG, "%s: bad shape N=%lld K=%lld", what,
+                 (long long)N, (long long)K);
+  ZIB_HOST_CHECK(w && q && s, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+  const int64_t nb = ceil_div(N, fp8::kBlock), kb = ceil_div(K, fp8::kBlock);
+  ZIB_HOST_CHECK(nb <= 65535, ZIB_ERR_TOO_LARGE, "%s: N=%lld", what, (long long)N);
+  cudaStream_t st = (cudaStream_t)stream;
+  const dim3 g((unsigned)kb, (unsigned)nb);
+  if (dtype == ZIB_BF16)
+    fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const __nv_bfloat16*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
+  else if (dtype == ZIB_F16)
+    fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const __half*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
+  else
+    fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const float*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
+  return zib_check_launch(what);
+}
+
+extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
+                                  const void* w, int64_t ldw, const float* sw, int64_t sw_n, int64_t sw_k,
+                                  const void* bias, void* y, int64_t ldy, int dtype, int64_t M, int64_t N, int64_t K,
+                                  void* stream) {
+  const char* what = "zib_fp8_block_gemm";
+  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
+  ZIB_HOST_CHECK(M >= 0 && N >= 1 && K >= 1 && ldq >= K && ldw >= K && ldy >= N, ZIB_ERR_INVALID_ARG,
+                 "%s: bad shape M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
+  ZIB_HOST_CHECK(M < (1ll << 31) - 512 && N < (1ll << 31) - 512 && K < (1ll << 31) - 512, ZIB_ERR_TOO_LARGE,
+                 "%s: M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
+  ZIB_HOST_CHECK(ldq % 16 == 0 && ldw % 16 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)w % 16 == 0,
+                 ZIB_ERR_ALIGNMENT, "%s: q and w need 16-byte aligned rows", what);
+  if (M == 0) return ZIB_OK;
+  ZIB_HOST_CHECK(q && sx && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+  cudaStream_t st = (cudaStream_t)stream;
+  const dim3 g((unsigned)ceil_div(N, 64), (unsigned)ceil_div(M, 64));
+  if (dtype == ZIB_BF16)
+    fp8::gemm_simple_kernel<<<g, 256, 0, st>>>((const uint8_t*)q, ldq, sx, sx_m, sx_k, (const uint8_t*)w, ldw, sw,
+                                               sw_n, sw_k, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y, ldy, M, N, K);
+  else if (dtype == ZIB_F16)
+    fp8::gemm_simple_kernel<<<g, 256, 0, st>>>((const uint8_t*)q, ldq, sx, sx_m, sx_k, (const uint8_t*)w, ldw, sw,
+                                               sw_n, sw_k, (const __half*)bias, (__half*)y, ldy, M, N, K);
+  else
+    fp8::gemm_simple_kernel<<<g, 256, 0, st>>>((const uint8_t*)q, ldq, sx, sx_m, sx_k, (const uint8_t*)w, ldw, sw,
+                                               sw_n, sw_k, (const float*)bias, (float*)y, ldy, M, N, K);
+  return zib_check_launch(what);
+}
+
+extern "C" int zib_fp8_transpose(const void* w, int64_t ldw, void* wt, int64_t ldt, int64_t N, int64_t K,
+                                 void* stream) {
+  const char* what = "zib_fp8_transpose";
+  ZIB_HOST_CHECK(N >= 1 && K >= 1 && ldw >= K && ldt >= N, ZIB_ERR_INVALID_ARG, "%s: bad shape N=%lld K=%lld", what,
+                 (long long)N, (long long)K);
+  ZIB_HOST_CHECK(w && wt, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+  ZIB_HOST_CHECK(ceil_div(N, 64) <= 65535, ZIB_ERR_TOO_LARGE, "%s: N=%lld", what, (long long)N);
+  fp8::transpose_kernel<<<dim3((unsigned)ceil_div(K, 64), (unsigned)ceil_div(N, 64)), 256, 0, (cudaStream_t)stream>>>(
+      (const uint8_t*)w, ldw, (uint8_t*)wt, ldt, N, K);
+  return zib_check_launch(what);
+}
+
+extern "C" int zib_col_sum(const void* x, int64_t ldx, int dtype, void* y, float* workspace, int64_t workspace_bytes,
+                           int64_t M, int64_t N, void* stream) {
+  const char* what = "zib_col_sum";
+  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
+  ZIB_HOST_CHECK(M >= 0 && N >= 1 && ldx >= N, ZIB_ERR_INVALID_ARG, "%s: bad shape M=%lld N=%lld", what, (long long)M,
+                 (long long)N);
+  ZIB_HOST_CHECK((x || M == 0) && y && workspace, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+  ZIB_HOST_CHECK(workspace_bytes >= fp8::kMaxSlabs * N * (int64_t)sizeof(float), ZIB_ERR_INVALID_ARG,
+                 "%s: workspace of %lld bytes needed", what, (long long)(fp8::kMaxSlabs * N * sizeof(float)));
+  const int64_t slab = ceil_div(M > 0 ? M : 1, fp8::kMaxSlabs);
+  const int slabs = (int)ceil_div(M, slab);
+  const dim3 g((unsigned)ceil_div(N, 256), (unsigned)(slabs > 0 ? slabs : 1));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == ZIB_BF16) {
+    if (slabs) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const __nv_bfloat16*)x, ldx, workspace, M, N, slab);
+    fp8::col_sum_kernel<<<g.x, 256, 0, st>>>(workspace, (__nv_bfloat16*)y, N, slabs);
+  } else if (dtype == ZIB_F16) {
+    if (slabs) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const __half*)x, ldx, workspace, M, N, slab);
+    fp8::col_sum_kernel<<<g.x, 256, 0, st>>>(workspace, (__half*)y, N, slabs);
+  } else {
+    if (slabs) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const float*)x, ldx, workspace, M, N, slab);
+    fp8::col_sum_kernel<<<g.x, 256, 0, st>>>(workspace, (float*)y, N, slabs);
+  }
+  return zib_check_launch(what);
+}

@@ -44,6 +44,7 @@ extern "C" const char* zib_last_error(void) { return g_last_error; }
 int zib_err_read_clear_gemm();
 void zib_gemm_split_reset();
 int zib_err_read_clear_rows();
+int zib_err_read_clear_rotary();
 
 extern "C" int zib_device_error_read_clear(void) {
   // every stream of the device, non-blocking ones included, has finished before the
@@ -52,8 +53,9 @@ extern "C" int zib_device_error_read_clear(void) {
   cudaGetLastError();
   int a = zib_err_read_clear_gemm();
   int b = zib_err_read_clear_rows();
+  int c = zib_err_read_clear_rotary();
   if (a) zib_gemm_split_reset();  // a stopped GEMM may have left split-K counters mid-count
-  return a ? a : b;
+  return a ? a : b ? b : c;
 }
 
 extern "C" int zib_device_check(int dev) {

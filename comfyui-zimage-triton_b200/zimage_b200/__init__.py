@@ -10,9 +10,13 @@ entry points and the same NextDiT patching function, backed by
 __version__ = "0.1.0"
 
 from .kernels import (  # noqa: E402
+    GroupNormAct,
     TritonAdaLNModulation,
     TritonRMSNorm,
     TritonSwiGLU,
+    group_norm_act,
+    rotary_embed,
+    rotary_table,
     triton_adaln_modulation,
     triton_fused_norm_gate_residual,
     triton_fused_qknorm_rope,
@@ -21,7 +25,15 @@ from .kernels import (  # noqa: E402
     triton_swiglu_forward,
 )
 from .patching import apply_triton_kernels_comfyui  # noqa: E402
-from .quantization import apply_int8_quantization, restore_int8_quantization  # noqa: E402
+from .quantization import (  # noqa: E402
+    apply_int8_quantization,
+    fp8_block_linear,
+    fp8_block_matmul,
+    fp8_block_quantize,
+    fp8_block_quantize_weight,
+    fp8_block_transpose,
+    restore_int8_quantization,
+)
 
 __all__ = [
     "triton_rms_norm",
@@ -36,4 +48,13 @@ __all__ = [
     "apply_triton_kernels_comfyui",
     "apply_int8_quantization",
     "restore_int8_quantization",
+    "fp8_block_quantize",
+    "fp8_block_quantize_weight",
+    "fp8_block_transpose",
+    "fp8_block_matmul",
+    "fp8_block_linear",
+    "rotary_embed",
+    "rotary_table",
+    "group_norm_act",
+    "GroupNormAct",
 ]

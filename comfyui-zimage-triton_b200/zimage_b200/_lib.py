@@ -26,6 +26,7 @@ ZIB_ERR_TOO_LARGE = 5
 ZIB_ERR_TIMEOUT = 6
 
 _VP, _I64, _I32, _F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_F64 = ctypes.c_double
 _FP = ctypes.POINTER(ctypes.c_float)
 
 # name -> argtypes (all return int status unless listed in _RESTYPES)
@@ -66,8 +67,27 @@ SIGNATURES: dict[str, list] = {
                         _I64, _I64, _F32, _VP],
     "zib_adaln_modulation": [_VP, _I64, _VP, _VP, _VP, _VP, _I64, _I64, _VP],
     "zib_adaln_gates": [_VP, _I64, _VP, _I64, _I64, _VP],
+    "zib_fp8_quant_rows": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP],
+    "zib_fp8_quant_blocks": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP],
+    "zib_fp8_block_gemm": [_VP, _I64, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _I32, _I64,
+                           _I64, _I64, _VP],
+    "zib_fp8_transpose": [_VP, _I64, _VP, _I64, _I64, _I64, _VP],
+    "zib_col_sum": [_VP, _I64, _I32, _VP, _VP, _I64, _I64, _I64, _VP],
+    "zib_rotary": [_VP, _I64, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _VP, _I64, _I32, _VP, _VP, _I64,
+                   _I64, _I64, _VP, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _VP],
+    "zib_rotary_table": [_VP, _I32, _I64, _I64, _I64, _I64, _F64, _I32, _F64, _F64, _F64, _F64, _F64, _VP, _VP,
+                         _VP],
+    "zib_group_norm_workspace": [_I64, _I64, _I64, _I64, _I32],
+    "zib_group_norm": [_VP, _I64, _I64, _VP, _VP, _VP, _I32, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, _I32,
+                       _F32, _I32, _VP],
+    "zib_group_norm_backward": [_VP, _I64, _I64, _VP, _I64, _I64, _VP, _VP, _VP, _I32, _VP, _VP, _VP, _VP, _VP,
+                                _I64, _I64, _I64, _I64, _I64, _I32, _I32, _VP],
 }
-_RESTYPES = {"zib_status_string": ctypes.c_char_p, "zib_last_error": ctypes.c_char_p}
+_RESTYPES = {"zib_status_string": ctypes.c_char_p, "zib_last_error": ctypes.c_char_p,
+             "zib_group_norm_workspace": ctypes.c_int64}
+
+# zib_dtype codes of the entry points that take several element types
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 _lib = None
 _lock = threading.Lock()
@@ -157,6 +177,31 @@ def call(name: str, *args) -> None:
         ensure_split_workspace()
     LAUNCHES += 1
     check(getattr(load(), name)(*args), name)
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` on the device of ``t``, whichever device is current; the stream is appended."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+        return
+    with torch.cuda.device(dev):
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def dtype_code(t: torch.Tensor, what: str) -> int:
+    """The zib_dtype of ``t``; ValueError for a type the entry points do not take."""
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be bfloat16, float16 or float32; got {t.dtype}")
+    return code
+
+
+def same_device(t: torch.Tensor, **others: torch.Tensor | None) -> None:
+    """ValueError unless every given tensor lies on the device of ``t``."""
+    for name, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f"{name} is on {o.device}, expected {t.device}")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

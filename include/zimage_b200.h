@@ -42,6 +42,18 @@ typedef enum zib_status {
   ZIB_ERR_TIMEOUT = 6      /* a bounded device wait expired  -> RuntimeError */
 } zib_status;
 
+/* Element types of the entry points that take several. */
+typedef enum zib_dtype { ZIB_BF16 = 0, ZIB_F16 = 1, ZIB_F32 = 2 } zib_dtype;
+/* Activation of zib_group_norm. */
+typedef enum zib_activation { ZIB_ACT_NONE = 0, ZIB_ACT_SILU = 1 } zib_activation;
+/* Frequency scaling of zib_rotary_table. */
+typedef enum zib_rotary_scaling {
+  ZIB_ROTARY_NONE = 0,
+  ZIB_ROTARY_LINEAR = 1,
+  ZIB_ROTARY_NTK = 2,
+  ZIB_ROTARY_YARN = 3
+} zib_rotary_scaling;
+
 /* Library version (major*10000 + minor*100 + patch). */
 ZIB_API int zib_version(void);
 /* Human-readable text of a zib_status. */
@@ -54,7 +66,8 @@ ZIB_API int zib_device_check(int dev);
  * kernel whose bounded wait expired: ZIB_ERR_TIMEOUT).  Synchronises the current
  * device first (every stream, non-blocking ones included) and, after a GEMM
  * error, each device whose split-K counters it re-zeroes; not for the hot path
- * nor inside a stream capture.  Returns 0 when no kernel reported an error. */
+ * nor inside a stream capture.  Returns 0 when no kernel reported an error;
+ * ZIB_ERR_INVALID_ARG after zib_rotary met a position outside its table. */
 ZIB_API int zib_device_error_read_clear(void);
 /* Launches one thread that waits on a barrier nothing arrives at: the bounded
  * wait of the GEMM and row kernels expires (2 s), the device error word reads
@@ -299,6 +312,94 @@ ZIB_API int zib_adaln_modulation(const void* raw, int64_t ldr, void* scale_msa, 
  * bf16 [rows, 2, dim] contiguous. */
 ZIB_API int zib_adaln_gates(const void* raw, int64_t ldr, void* gates, int64_t rows, int64_t dim,
                     void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Operators without a counterpart in the reference: matrix products in 8-bit
+ * floating point, rotary positions, group normalisation.  `dtype` is a
+ * zib_dtype; strides count elements.
+ * ------------------------------------------------------------------------- */
+
+/* Activation rows as e4m3 with one scale per block of 1 x 128 values.
+ * x: [M,K] row stride ldx; q: e4m3 [M,K] row stride ldq; s: fp32, element (m, b)
+ * of [M, ceil(K/128)] at m*s_m + b*s_k.  A block with largest magnitude a has
+ * s = 2^e, e >= -120 the least with a <= 448 s, and q = x / s rounded to nearest
+ * (ties to even); a block with an infinity or NaN has NaN scale and values. */
+ZIB_API int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s,
+                       int64_t s_m, int64_t s_k, int64_t M, int64_t K, void* stream);
+
+/* The same for a weight [N,K] with one scale per block of 128 x 128, element
+ * (i, j) of [ceil(N/128), ceil(K/128)] at i*s_n + j*s_k. */
+ZIB_API int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void* q, int64_t ldq, float* s,
+                         int64_t s_n, int64_t s_k, int64_t N, int64_t K, void* stream);
+
+/* y[m,n] = sum_b sx[m,b] * sw[n/128,b] * sum_{k in block b} q[m,k] w[n,k] (+ bias[n]),
+ * fp32 sums, rounded once to `dtype` (of y and bias).  q: e4m3 [M,K] row stride
+ * ldq; w: e4m3 [N,K] row stride ldw; both with 16-byte aligned rows.  sx, sw: any
+ * fp32 scales, strided as above. */
+ZIB_API int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
+                       const void* w, int64_t ldw, const float* sw, int64_t sw_n, int64_t sw_k,
+                       const void* bias, void* y, int64_t ldy, int dtype, int64_t M, int64_t N,
+                       int64_t K, void* stream);
+
+/* wt[k,n] = w[n,k] of 8-bit values: the weight of the gradient towards the
+ * activations (its scales are the same blocks, transposed). */
+ZIB_API int zib_fp8_transpose(const void* w, int64_t ldw, void* wt, int64_t ldt, int64_t N, int64_t K,
+                      void* stream);
+
+/* y[n] = sum_m x[m,n] (a bias gradient), fp32 partial sums in a fixed order,
+ * rounded once to dtype.  workspace: 64 * N floats. */
+ZIB_API int zib_col_sum(const void* x, int64_t ldx, int dtype, void* y, float* workspace,
+                int64_t workspace_bytes, int64_t M, int64_t N, void* stream);
+
+/* Rotary positions of q and k (Hk = 0: q alone) in one launch.  q: [B,S,Hq,D],
+ * k: [B,S,Hk,D] with strides (sb, ss, sh), last dimension contiguous; outputs
+ * contiguous [B,S,H,D].  The first R features turn, the rest pass through:
+ * pairs (2j, 2j+1), or (j, j + R/2) with half_layout.  cos, sin: fp32, row l of
+ * batch entry b at b*cs_b + l*cs_l, R/2 values, L rows; l = positions[b,s]
+ * (int64 if pos64, else int32; strides ps_b, ps_s), or s where positions is
+ * NULL.  inverse turns the other way (the gradient).  A position outside
+ * [0, L) reads no table row: its turned features are NaN and the device error
+ * word becomes ZIB_ERR_INVALID_ARG. */
+ZIB_API int zib_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void* q_out, int64_t Hq,
+               const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh, void* k_out, int64_t Hk,
+               int dtype, const float* cos, const float* sin, int64_t cs_b, int64_t cs_l, int64_t L,
+               const void* positions, int pos64, int64_t ps_b, int64_t ps_s, int64_t B, int64_t S,
+               int64_t D, int64_t R, int half_layout, int inverse, void* stream);
+
+/* cos and sin [T, dim/2] of positions[t] (stride ps; NULL: start + t) times
+ * theta^(-2j/dim), scaled for long contexts (zib_rotary_scaling):
+ *   linear  the frequencies divided by factor;
+ *   ntk     the base multiplied by factor^(dim/(dim-2));
+ *   yarn    frequencies with fewer than beta_slow turns over `original`
+ *           positions divided by factor, those with more than beta_fast kept, a
+ *           linear ramp between; cos and sin times attention_factor.
+ * Angles are formed in fp64. */
+ZIB_API int zib_rotary_table(const void* positions, int pos64, int64_t ps, int64_t start, int64_t T,
+                     int64_t dim, double theta, int scaling, double factor, double original,
+                     double beta_fast, double beta_slow, double attention_factor, float* cos,
+                     float* sin, void* stream);
+
+/* Bytes of workspace for zib_group_norm (backward = 0) or its backward pass on
+ * the current device. */
+ZIB_API int64_t zib_group_norm_workspace(int64_t B, int64_t P, int64_t C, int64_t G, int backward);
+
+/* Group normalisation with an activation, channels last.  x: [B,P,C] with batch
+ * stride xsb and pixel stride xsp, channels contiguous; y: contiguous [B,P,C];
+ * w, b: [C] of wdtype, each may be NULL; mean, rstd: fp32 [B,G] outputs.
+ * y = act((x - mean) * rstd * w + b), statistics per batch entry over the
+ * P * C/G values of a group. */
+ZIB_API int zib_group_norm(const void* x, int64_t xsb, int64_t xsp, void* y, const void* w, const void* b,
+                   int wdtype, float* mean, float* rstd, void* workspace, int64_t workspace_bytes,
+                   int64_t B, int64_t P, int64_t C, int64_t G, int dtype, float eps, int act,
+                   void* stream);
+
+/* Its gradients: dx (contiguous [B,P,C]) and dw, db ([C] of wdtype), each NULL
+ * where not wanted; mean, rstd as the forward pass wrote them. */
+ZIB_API int zib_group_norm_backward(const void* x, int64_t xsb, int64_t xsp, const void* dy, int64_t dsb,
+                            int64_t dsp, void* dx, const void* w, const void* b, int wdtype, void* dw,
+                            void* db, const float* mean, const float* rstd, void* workspace,
+                            int64_t workspace_bytes, int64_t B, int64_t P, int64_t C, int64_t G,
+                            int dtype, int act, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,145 @@
+"""What the block-scaled 8-bit products, rotary positions and group normalisation refuse, before any launch."""
+
+import math
+
+import pytest
+import torch
+
+from zimage_b200 import (GroupNormAct, _lib, fp8_block_linear, fp8_block_matmul, fp8_block_quantize,
+                         fp8_block_quantize_weight, fp8_block_transpose, group_norm_act, rotary_embed, rotary_table)
+
+E4M3 = torch.float8_e4m3fn
+INV = _lib.ZIB_ERR_INVALID_ARG
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 128)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8_block_quantize(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8_block_quantize_weight(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8_block_transpose(x.to(E4M3))
+    with pytest.raises(ValueError, match="CUDA"):
+        fp8_block_linear(x, torch.zeros(64, 128).to(E4M3), torch.ones(1, 1))
+    with pytest.raises(ValueError, match="CUDA"):
+        group_norm_act(x, 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        rotary_embed(torch.zeros(1, 2, 1, 8), None, torch.ones(2, 4), torch.ones(2, 4))
+    with pytest.raises(ValueError, match="CUDA"):
+        rotary_table(torch.arange(4), 8)
+
+
+def test_fp8_shapes_and_types():
+    x, w, s = torch.zeros(3, 200), torch.zeros(130, 200).to(E4M3), torch.ones(2, 2)
+    for bad in (dict(w_q=w.float()), dict(w_q=w[:, :128]), dict(w_scale=s[:1]), dict(w_scale=s.double()),
+                dict(bias=torch.zeros(129)), dict(bias=torch.zeros(130).half()), dict(w_q_t=w),
+                dict(w_q_t=torch.zeros(200, 130))):
+        kw = {"w_q": w, "w_scale": s, **bad}
+        with pytest.raises(ValueError):
+            fp8_block_linear(x, **kw)
+    with pytest.raises(ValueError, match="bfloat16, float16 or float32"):
+        fp8_block_linear(x.double(), w, s)
+    with pytest.raises(ValueError):
+        fp8_block_quantize(torch.zeros(4, 0))
+    with pytest.raises(ValueError):
+        fp8_block_quantize(torch.zeros(()))
+    with pytest.raises(ValueError):
+        fp8_block_quantize_weight(torch.zeros(2, 3, 4))
+    with pytest.raises(ValueError):
+        fp8_block_transpose(torch.zeros(4, 4))
+    xq, xs = x.to(E4M3), torch.ones(3, 2)
+    for args in ((x, xs, w, s), (xq, xs[:2], w, s), (xq, xs.half(), w, s), (xq, xs, w, s[:1])):
+        with pytest.raises(ValueError):
+            fp8_block_matmul(*args)
+    with pytest.raises(ValueError, match="out_dtype"):
+        fp8_block_matmul(xq, xs, w, s, out_dtype=torch.float64)
+
+
+def test_rotary_shapes_and_types():
+    q, c = torch.zeros(2, 3, 4, 16), torch.ones(5, 8)
+    bad = [
+        (q[0], None, c, c, {}), (q, q[:1], c, c, {}), (q, q.half(), c, c, {}), (q, q[..., :8], c, c, {}),
+        (q, None, c, c[:4], {}), (q, None, c.double(), c.double(), {}), (q, None, c[:2], c[:2], {}),
+        (q, None, torch.ones(5, 9), torch.ones(5, 9), {}), (q, None, torch.ones(5, 0), torch.ones(5, 0), {}),
+        (q, None, torch.ones(3, 5, 8), torch.ones(3, 5, 8), {}), (q, None, c, c, {"layout": "other"}),
+        (q, None, c, c, {"positions": torch.zeros(2, 3)}),
+        (q, None, c, c, {"positions": torch.zeros(2, 4, dtype=torch.long)}),
+        (q, None, c[:0], c[:0], {"positions": torch.zeros(2, 3, dtype=torch.long)}),
+        (q.double(), None, c, c, {}), (torch.zeros(1, 1, 1, 15), None, c[:, :7], c[:, :7], {}),
+        (torch.zeros(1, 1, 1, 2048), None, c, c, {}),
+    ]
+    for a, b, cos, sin, kw in bad:
+        with pytest.raises(ValueError):
+            rotary_embed(a, b, cos, sin, **kw)
+
+
+def test_rotary_table_arguments():
+    for dim in (0, 3, -2, 8.0):
+        with pytest.raises(ValueError):
+            rotary_table(4, dim)
+    for sc in ({"type": "other"}, {"factor": 2.0}, {"type": "linear", "factor": 0.5}, {"type": "ntk", "factor": math.nan},
+               {"type": "yarn", "factor": 2.0}, {"type": "linear", "factor": 2.0, "extra": 1},
+               {"type": "yarn", "factor": 2.0, "original_length": 10, "beta_fast": 1.0, "beta_slow": 2.0},
+               {"type": "yarn", "factor": 2.0, "original_length": 10, "attention_factor": 0.0}):
+        with pytest.raises(ValueError):
+            rotary_table(torch.arange(4), 8, scaling=sc)
+    with pytest.raises(ValueError):
+        rotary_table(torch.zeros(4), 8)
+    with pytest.raises(ValueError):
+        rotary_table(torch.zeros(2, 2, dtype=torch.long), 8)
+
+
+def test_group_norm_arguments():
+    x = torch.zeros(2, 5, 12)
+    for args, kw in (((x, 5), {}), ((x, 0), {}), ((x[0, 0], 4), {}), ((x.double(), 4), {}),
+                     ((x, 4, torch.ones(11)), {}), ((x, 4, torch.ones(12).double()), {}),
+                     ((x, 4, torch.ones(12), torch.ones(12).half()), {}), ((x, 4), {"activation": "other"}),
+                     ((x, 4), {"eps": -1.0}), ((x, 4), {"eps": math.nan})):
+        with pytest.raises(ValueError):
+            group_norm_act(*args, **kw)
+    with pytest.raises(RuntimeError, match="at most"):
+        group_norm_act(torch.zeros(1, 1, 8200), 8)
+    with pytest.raises(ValueError):
+        GroupNormAct(5, 12)
+    with pytest.raises(ValueError):
+        GroupNormAct(4, 12, activation="other")
+
+
+def test_c_entries_validate_on_the_host():
+    lib = _lib.load()
+    # null operands, unknown types, impossible shapes: an error code, no launch
+    assert lib.zib_fp8_quant_rows(None, 128, 0, None, 128, None, 1, 1, 4, 128, None) == INV
+    assert lib.zib_fp8_quant_rows(16, 128, 7, 16, 128, 16, 1, 1, 4, 128, None) == INV
+    assert lib.zib_fp8_quant_rows(16, 64, 0, 16, 128, 16, 1, 1, 4, 128, None) == INV
+    assert lib.zib_fp8_quant_blocks(16, 128, 0, 16, 128, 16, 1, 1, 0, 128, None) == INV
+    assert lib.zib_fp8_block_gemm(16, 128, 16, 1, 1, 16, 128, 16, 1, 1, None, 16, 8, 9, 4, 8, 128, None) == INV
+    assert lib.zib_fp8_block_gemm(16, 120, 16, 1, 1, 16, 128, 16, 1, 1, None, 16, 8, 0, 4, 8, 120, None) == \
+        _lib.ZIB_ERR_ALIGNMENT
+    assert lib.zib_fp8_block_gemm(24, 128, 16, 1, 1, 16, 128, 16, 1, 1, None, 16, 8, 0, 4, 8, 128, None) == \
+        _lib.ZIB_ERR_ALIGNMENT
+    assert lib.zib_fp8_block_gemm(16, 1 << 31, 16, 1, 1, 16, 1 << 31, 16, 1, 1, None, 16, 8, 0, 4, 8, 1 << 31, None) \
+        == _lib.ZIB_ERR_TOO_LARGE
+    assert lib.zib_fp8_block_gemm(None, 128, None, 1, 1, None, 128, None, 1, 1, None, None, 8, 0, 0, 8, 128, None) == 0
+    assert lib.zib_fp8_transpose(None, 8, None, 8, 8, 8, None) == INV
+    assert lib.zib_col_sum(16, 8, 0, 16, 16, 4, 4, 8, None) == INV
+    rot = [16, 0, 0, 0, 16, 1, None, 0, 0, 0, None, 0]
+    tab = [16, 16, 0, 4, 8, None, 0, 0, 0]
+    assert lib.zib_rotary(*rot, 5, *tab, 1, 1, 8, 8, 0, 0, None) == INV
+    assert lib.zib_rotary(*rot, 0, *tab, 1, 1, 8, 6 + 1, 0, 0, None) == INV
+    assert lib.zib_rotary(*rot, 0, *tab, 1, 1, 8, 10, 0, 0, None) == INV
+    assert lib.zib_rotary(*rot, 0, *tab, 1, 9, 8, 8, 0, 0, None) == INV  # 9 tokens, 8 rows
+    assert lib.zib_rotary(*rot, 0, *tab, 0, 9, 8, 8, 0, 0, None) == 0
+    assert lib.zib_rotary(17, *rot[1:], 0, *tab, 1, 1, 8, 8, 0, 0, None) == _lib.ZIB_ERR_ALIGNMENT
+    assert lib.zib_rotary_table(None, 0, 0, 0, 4, 7, 1e4, 0, 1.0, 0.0, 32.0, 1.0, 1.0, 16, 16, None) == INV
+    assert lib.zib_rotary_table(None, 0, 0, 0, 4, 8, -1.0, 0, 1.0, 0.0, 32.0, 1.0, 1.0, 16, 16, None) == INV
+    assert lib.zib_rotary_table(None, 0, 0, 0, 4, 2, 1e4, 2, 2.0, 0.0, 32.0, 1.0, 1.0, 16, 16, None) == INV
+    assert lib.zib_rotary_table(None, 0, 0, 0, 4, 8, 1e4, 3, 2.0, 0.0, 32.0, 1.0, 1.0, 16, 16, None) == INV
+    gn = [16, 0, 0, 16, None, None, 0, 16, 16, 16]
+    assert lib.zib_group_norm(*gn, 1 << 20, 1, 4, 12, 5, 0, 1e-6, 1, None) == INV
+    assert lib.zib_group_norm(*gn, 1 << 20, 1, 4, 12, 4, 0, 1e-6, 9, None) == INV
+    assert lib.zib_group_norm(*gn, 0, 1, 4, 12, 4, 0, 1e-6, 1, None) == INV  # workspace
+    assert lib.zib_group_norm(*gn, 1 << 40, 1, 4, 1 << 14, 4, 0, 1e-6, 1, None) == _lib.ZIB_ERR_TOO_LARGE
+    assert lib.zib_group_norm(*gn, 0, 0, 4, 12, 4, 0, 1e-6, 1, None) == 0
+    assert lib.zib_group_norm_workspace(0, 4, 12, 4, 0) == 0
+    assert lib.zib_group_norm_workspace(2, 400, 12, 4, 1) > 0
