@@ -19,7 +19,8 @@ CSRC = Path(__file__).resolve().parent
 PKG = CSRC.parent / "zimage_b200"
 INCLUDE = CSRC.parent.parent / "include"
 OUT = PKG / "libzimage_b200.so"
-SOURCES = ["zib_api.cu", "rowops.cu", "gemm_w8a8.cu", "rotary.cu", "group_norm.cu", "fp8_block.cu"]
+SOURCES = ["zib_api.cu", "rowops.cu", "gemm_w8a8.cu", "rotary.cu", "group_norm.cu", "fp8_block.cu",
+           "fp8_gemm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden",
          "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills"]

@@ -1,4 +1,4 @@
-// Matrix products in 8-bit floating point (e4m3) with one scale for each block of 128.
+// Operands of matrix products in 8-bit floating point (e4m3) with one scale for each block of 128.
 //
 // Quantiser: a block of values (1 x 128 of an activation row, 128 x 128 of a weight) with largest
 // magnitude a is held as e4m3 values q = x / s, s = 2^e with the least e >= -120 such that
@@ -6,9 +6,6 @@
 // 4-bit mantissa (ties to even) and any implementation gives the same bits; as the format floats,
 // scales between the powers would gain no precision but at the bottom of its range.  A block with
 // an infinity or a NaN gets NaN for its scale and its values.
-//
-// Product: y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} q[m, k] w[n, k] (+ bias[n]),
-// the scales being any fp32 values; sums in fp32, rounded once to the output type.
 #include "zib_async.cuh"
 #include "zib_types.cuh"
 
@@ -35,10 +32,6 @@ __device__ __forceinline__ float inverse_scale(float s) {
 __device__ __forceinline__ uint8_t to_e4m3(float v) {
   return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ float from_e4m3(uint8_t v) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
-}
-
 // one warp per (row, block)
 template <typename T>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
@@ -91,54 +84,6 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const T* __restrict__
   for (int r = threadIdx.x >> 7; r < kBlock; r += 2)
     if (n0 + r < N && k < K) q[(n0 + r) * ldq + k] = to_e4m3(to_f32(w[(n0 + r) * ldw + k]) * inv);
   if (threadIdx.x == 0) s[blockIdx.y * s_n + blockIdx.x * s_k] = sc;
-}
-
-// 64 x 64 output tile per CTA, 4 x 4 per thread
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_simple_kernel(const uint8_t* __restrict__ q, int64_t ldq,
-                                                          const float* __restrict__ sx, int64_t sx_m, int64_t sx_k,
-                                                          const uint8_t* __restrict__ w, int64_t ldw,
-                                                          const float* __restrict__ sw, int64_t sw_n, int64_t sw_k,
-                                                          const T* __restrict__ bias, T* __restrict__ y, int64_t ldy,
-                                                          int64_t M, int64_t N, int64_t K) {
-  __shared__ float a[16][65], b[16][65];
-  const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {}, part[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += 16) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {
-      const int r = i >> 4, c = i & 15;
-      a[c][r] = m0 + r < M && k0 + c < K ? from_e4m3(q[(m0 + r) * ldq + k0 + c]) : 0.0f;
-      b[c][r] = n0 + r < N && k0 + c < K ? from_e4m3(w[(n0 + r) * ldw + k0 + c]) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(a[k][ty * 4 + i], b[k][tx * 4 + j], part[i][j]);
-    __syncthreads();
-    if ((k0 + 16) % kBlock == 0 || k0 + 16 >= K) {  // a block of 128 is complete
-      const int64_t kb = k0 / kBlock;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-          if (m < M && n < N)
-            acc[i][j] = fmaf(part[i][j], sx[m * sx_m + kb * sx_k] * sw[n / kBlock * sw_n + kb * sw_k], acc[i][j]);
-          part[i][j] = 0.0f;
-        }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m < M && n < N) y[m * ldy + n] = from_f32<T>(acc[i][j] + (bias ? to_f32(bias[n]) : 0.0f));
-    }
 }
 
 // wt[k, n] = w[n, k], 64 x 64 bytes per CTA
@@ -224,34 +169,6 @@ extern "C" int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void*
     fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const __half*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
   else
     fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const float*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
-  return zib_check_launch(what);
-}
-
-extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
-                                  const void* w, int64_t ldw, const float* sw, int64_t sw_n, int64_t sw_k,
-                                  const void* bias, void* y, int64_t ldy, int dtype, int64_t M, int64_t N, int64_t K,
-                                  void* stream) {
-  const char* what = "zib_fp8_block_gemm";
-  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
-  ZIB_HOST_CHECK(M >= 0 && N >= 1 && K >= 1 && ldq >= K && ldw >= K && ldy >= N, ZIB_ERR_INVALID_ARG,
-                 "%s: bad shape M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
-  ZIB_HOST_CHECK(M < (1ll << 31) - 512 && N < (1ll << 31) - 512 && K < (1ll << 31) - 512, ZIB_ERR_TOO_LARGE,
-                 "%s: M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
-  ZIB_HOST_CHECK(ldq % 16 == 0 && ldw % 16 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)w % 16 == 0,
-                 ZIB_ERR_ALIGNMENT, "%s: q and w need 16-byte aligned rows", what);
-  if (M == 0) return ZIB_OK;
-  ZIB_HOST_CHECK(q && sx && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
-  cudaStream_t st = (cudaStream_t)stream;
-  const dim3 g((unsigned)ceil_div(N, 64), (unsigned)ceil_div(M, 64));
-  if (dtype == ZIB_BF16)
-    fp8::gemm_simple_kernel<<<g, 256, 0, st>>>((const uint8_t*)q, ldq, sx, sx_m, sx_k, (const uint8_t*)w, ldw, sw,
-                                               sw_n, sw_k, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y, ldy, M, N, K);
-  else if (dtype == ZIB_F16)
-    fp8::gemm_simple_kernel<<<g, 256, 0, st>>>((const uint8_t*)q, ldq, sx, sx_m, sx_k, (const uint8_t*)w, ldw, sw,
-                                               sw_n, sw_k, (const __half*)bias, (__half*)y, ldy, M, N, K);
-  else
-    fp8::gemm_simple_kernel<<<g, 256, 0, st>>>((const uint8_t*)q, ldq, sx, sx_m, sx_k, (const uint8_t*)w, ldw, sw,
-                                               sw_n, sw_k, (const float*)bias, (float*)y, ldy, M, N, K);
   return zib_check_launch(what);
 }
 

@@ -1,0 +1,482 @@
+// Block-scaled 8-bit product on 5th-generation tensor cores (tcgen05, kind::f8f6f4) for sm_100a.
+//
+//   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} q[m, k] w[n, k]  (+ bias[n])
+//
+// The tensor cores sum one block of 128 products per accumulator; the scales differ from block to
+// block, so the sum over blocks is formed outside of them, in fp32 registers.
+//
+// Design (persistent, warp-specialised, clusters of two CTAs, tiles of 256 rows x BN columns):
+//   warp 0     TMA producer: 128-byte swizzled K-major boxes, one K-block of 128 per stage (each CTA
+//              stages its 128 rows of q and half of the BN rows of w).
+//   warp 1     issues tcgen05.mma (cta_group::2, M = 256) from one thread of the leading CTA.  Every
+//              K-block starts a fresh accumulator; the 512 TMEM columns hold 512 / BN of them, so
+//              the MMAs run ahead of the warps that empty them.
+//   warps 2-9  add s * accumulator to their registers: the warps w and w + 4 share a TMEM lane
+//              quarter (32 rows) and take half of the BN columns each.  A thread owns one row, so the
+//              row's scale is one value; its BN / 2 columns lie in one block of 128 weight rows, so
+//              that scale is one value too: one packed multiply-add per two elements and K-block.
+//              The output tile leaves through shared memory and TMA stores that drain while the
+//              next tile is summed.
+// Every mbarrier wait is bounded; on expiry the CTA records ZIB_ERR_TIMEOUT in a device error word,
+// drains its loads and MMAs, frees TMEM and exits.
+#include "rot_pack.cuh"
+#include "zib_tcgen05.cuh"
+#include "zib_types.cuh"
+
+ZIB_DEFINE_ERROR_READER(zib_err_read_clear_fp8)
+
+namespace zib {
+namespace fp8 {
+
+using namespace tc;
+
+constexpr int kBlock = 128;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (2 + kEpiWarps) * 32;
+constexpr int kTmemCols = 512;
+constexpr int kABytes = 128 * kBlock;
+
+template <int BN>
+struct Cfg {
+  static constexpr int BUFS = kTmemCols / BN;  // accumulators in flight
+  static constexpr int STAGE = kABytes + BN / 2 * kBlock;
+  static constexpr int STAGES = BN == 256 ? 5 : 6;
+  static constexpr int XWARP = 8192;  // output staging per warp: two boxes of 32 rows x 128 bytes
+  static constexpr int SMEM = STAGES * STAGE + kEpiWarps * XWARP + 256 + 1024;
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+};
+
+// D = f32, A = B = e4m3, both K-major
+__host__ __device__ constexpr uint32_t idesc_f8(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+struct GemmParams {
+  int M, N;
+  int num_mb, num_nb, num_kb, num_tiles;
+  int n_fast, group;
+  const float* sx;
+  int64_t sx_m, sx_k;
+  const float* sw;
+  int64_t sw_n, sw_k;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int tma_store;  // y's rows are 16-byte aligned
+};
+
+__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// waits for this thread's TMEM loads; r is tied in so that no use of it moves above the wait
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+// Tile t -> (M-block, N-block): the fast index runs in groups whose rows stay in L2 while the
+// tiles sweep the slow index (the same order as the int8 GEMM's).
+__device__ __forceinline__ void tile_at(const GemmParams& p, int tile, int& mb, int& nb) {
+  const int nfast = p.n_fast ? p.num_nb : p.num_mb, nslow = p.n_fast ? p.num_mb : p.num_nb;
+  const int per_group = p.group * nslow;
+  const int g = tile / per_group, r = tile - g * per_group;
+  const int gsize = min(p.group, nfast - g * p.group);
+  const int f = g * p.group + r % gsize, sl = r / gsize;
+  nb = p.n_fast ? f : sl;
+  mb = p.n_fast ? sl : f;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// acc[c * 8 .. c * 8 + 7] (pairs of columns) += s * r
+template <int N2>
+__device__ __forceinline__ void add_scaled(px::f2 (&acc)[N2], int c, const uint32_t (&r)[16], px::f2 s2) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    acc[c * 8 + j] = px::fma(px::mk(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[c * 8 + j]);
+}
+
+// This thread's CW columns of row `row` to y, through the warp's staging boxes (32 rows x 128 bytes,
+// 16-byte chunk c of row r at c ^ (r & 7): the TMA's 128-byte swizzle).
+template <typename T, int CW>
+__device__ __forceinline__ void store_tile(const GemmParams& p, const CUtensorMap* map_y, px::f2 (&acc)[CW / 2],
+                                           uint8_t* xw, int row0, int n0, int lane) {
+  constexpr int BOXC = 128 / sizeof(T);            // columns per box
+  constexpr int BOXES = CW / BOXC;                 // boxes of this warp's part
+  constexpr int PER = BOXES < 2 ? BOXES : 2;       // staged at a time
+#pragma unroll
+  for (int b0 = 0; b0 < BOXES; b0 += PER) {
+    if (p.tma_store) {  // the boxes' previous contents have been read
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (int b = 0; b < PER; ++b) {
+      const int col = (b0 + b) * BOXC;  // first of the box's columns
+      uint8_t* line = xw + b * 4096 + lane * 128;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        constexpr int EC = 16 / sizeof(T);  // columns per 16-byte chunk
+        float v[EC];
+#pragma unroll
+        for (int j = 0; j < EC; j += 2) px::split(acc[(col + c * EC + j) / 2], v[j], v[j + 1]);
+        if (p.bias) {
+#pragma unroll
+          for (int j = 0; j < EC; ++j) {
+            const int n = n0 + col + c * EC + j;
+            if (n < p.N) v[j] += to_f32(reinterpret_cast<const T*>(p.bias)[n]);
+          }
+        }
+        uint4 o;
+        if constexpr (sizeof(T) == 2) {
+          o = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        } else {
+          o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        }
+        *reinterpret_cast<uint4*>(line + ((c ^ (lane & 7)) << 4)) = o;
+      }
+    }
+    if (p.tma_store) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && row0 < p.M) {
+#pragma unroll
+        for (int b = 0; b < PER; ++b)
+          if (n0 + (b0 + b) * BOXC < p.N) tma_store_2d(map_y, xw + b * 4096, n0 + (b0 + b) * BOXC, row0);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    } else {
+      __syncwarp();
+      for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+        T* dst = reinterpret_cast<T*>(p.y) + (int64_t)(row0 + r) * p.ldy;
+#pragma unroll
+        for (int b = 0; b < PER; ++b) {
+          const int col = n0 + (b0 + b) * BOXC;
+          for (int e = lane; e < BOXC && col + e < p.N; e += 32) {
+            const int at = e * (int)sizeof(T);
+            dst[col + e] = *reinterpret_cast<const T*>(xw + b * 4096 + r * 128 + (((at >> 4) ^ (r & 7)) << 4) +
+                                                       (at & 15));
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <typename T, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                     const __grid_constant__ CUtensorMap map_y, const GemmParams p) {
+  using C = Cfg<BN>;
+  constexpr int STAGES = C::STAGES, BUFS = C::BUFS, CW = BN / 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* xbuf = smem + STAGES * C::STAGE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xbuf + kEpiWarps * C::XWARP);
+  uint64_t* full_bar = bars;                       // leader's is used
+  uint64_t* empty_bar = bars + STAGES;             // both
+  uint64_t* tfull_bar = bars + 2 * STAGES;         // both
+  uint64_t* tempty_bar = tfull_bar + BUFS;         // leader's is used
+  uint64_t* mma_done_bar = tempty_bar + BUFS;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(mma_done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  static_assert((2 * STAGES + 2 * BUFS + 1) * 8 + 8 <= 256, "barrier area");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int cluster_id = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < BUFS; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 2 * kEpiWarps);  // epilogue warps of both CTAs
+    }
+    mbar_init(mma_done_bar, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before any cross-CTA signal
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  bool aborted = false;
+
+  if (warp == 0) {
+    if (lane == 0) {  // ---- TMA producer (both CTAs)
+      int stage = 0;
+      uint32_t phase = 0, pend_mask = 0, pend_parity = 0;
+      bool ok = true;
+      for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
+        int mb, nb;
+        tile_at(p, t, mb, nb);
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+          const uint32_t fb = smem_u32(&full_bar[stage]);
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * C::STAGE);
+          const uint32_t fb_leader = leader ? fb : mapa_rank(fb, 0);
+          uint8_t* st = smem + stage * C::STAGE;
+          tma_load_2d_pair(st, &map_a, fb_leader, kb * kBlock, mb * 256 + (int)rank * 128);
+          tma_load_2d_pair(st + kABytes, &map_b, fb_leader, kb * kBlock, nb * BN + (int)rank * (BN / 2));
+          pend_mask |= 1u << stage;
+          pend_parity = (pend_parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {
+        aborted = true;
+        if (leader)
+          for (int s = 0; s < STAGES; ++s)
+            if (pend_mask & (1u << s)) mbar_drain_wait(&full_bar[s], (pend_parity >> s) & 1u);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {  // ---- MMA issuer
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      bool ok = true;
+      const uint32_t base = smem_u32(smem);
+      constexpr uint32_t idesc = idesc_f8(256, BN);
+      for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!mbar_wait_bounded(&tempty_bar[buf], buf_phase ^ 1u, abort_flag) ||
+              !mbar_wait_bounded(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem_base + (uint32_t)(buf * BN);
+          const uint64_t adesc = sdesc_sw128(base + stage * C::STAGE);
+          const uint64_t bdesc = sdesc_sw128(base + stage * C::STAGE + kABytes);
+#pragma unroll
+          for (int k = 0; k < kBlock / 32; ++k)
+            umma_f8_pair(d, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k != 0 ? 1u : 0u);
+          umma_commit_pair(&empty_bar[stage], (uint16_t)3);  // frees the stage in both CTAs
+          umma_commit_pair(&tfull_bar[buf], (uint16_t)3);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          if (++buf == BUFS) { buf = 0; buf_phase ^= 1u; }
+        }
+      }
+      if (!ok) aborted = true;
+      umma_commit_pair(mma_done_bar, (uint16_t)1);
+      mbar_drain_wait(mma_done_bar, 0);
+    }
+    __syncwarp();
+  } else {
+    // ---- sums over K-blocks and output (both CTAs)
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* xw = xbuf + (warp - 2) * C::XWARP;
+    const uint32_t t_warp = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * CW);
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    bool ok = true;
+    // scales of the coming K-block, loaded one ahead
+    const float *px_ = nullptr, *pw_ = nullptr;
+    int mb = 0, nb = 0;
+    float sx = 0.0f, sw = 0.0f;
+    auto locate = [&](int t) {
+      tile_at(p, t, mb, nb);
+      const int row = mb * 256 + (int)rank * 128 + quarter * 32 + lane, n0 = nb * BN + half * CW;
+      px_ = row < p.M ? p.sx + row * p.sx_m : nullptr;
+      pw_ = n0 < p.N ? p.sw + (n0 / kBlock) * p.sw_n : nullptr;
+      sx = px_ ? __ldg(px_) : 0.0f;
+      sw = pw_ ? __ldg(pw_) : 0.0f;
+    };
+    if (cluster_id < p.num_tiles) locate(cluster_id);
+    for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
+      const int row0 = mb * 256 + (int)rank * 128 + quarter * 32, n0 = nb * BN + half * CW;
+      px::f2 acc[CW / 2];
+#pragma unroll
+      for (int j = 0; j < CW / 2; ++j) acc[j] = 0ull;
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        const float s = sx * sw;
+        const px::f2 s2 = px::mk(s, s);
+        if (kb + 1 < p.num_kb) {
+          sx = px_ ? __ldg(px_ + (kb + 1) * p.sx_k) : 0.0f;
+          sw = pw_ ? __ldg(pw_ + (kb + 1) * p.sw_k) : 0.0f;
+        }
+        int got = 1;
+        if (lane == 0) got = mbar_wait_bounded(&tfull_bar[buf], buf_phase, abort_flag) ? 1 : 0;
+        got = __shfl_sync(0xFFFFFFFFu, got, 0);
+        if (!got) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t ta = t_warp + (uint32_t)(buf * BN);
+        uint32_t r0[16], r1[16];
+        tmem_ld16(ta, r0);
+        wait_ld(r0);
+#pragma unroll
+        for (int c = 0; c < CW / 16; c += 2) {
+          tmem_ld16(ta + (uint32_t)((c + 1) * 16), r1);
+          add_scaled(acc, c, r0, s2);
+          wait_ld(r1);
+          if (c + 2 < CW / 16) {
+            tmem_ld16(ta + (uint32_t)((c + 2) * 16), r0);
+          } else {  // read: the accumulator may be filled again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_rank(smem_u32(&tempty_bar[buf]), 0));
+          }
+          add_scaled(acc, c + 1, r1, s2);
+          if (c + 2 < CW / 16) wait_ld(r0);
+        }
+        if (++buf == BUFS) { buf = 0; buf_phase ^= 1u; }
+      }
+      if (!ok) break;
+      if (t + nclusters < p.num_tiles) locate(t + nclusters);
+      store_tile<T, CW>(p, &map_y, acc, xw, row0, n0, lane);
+    }
+    if (!ok) aborted = true;
+    if (p.tma_store && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+
+  // An aborted CTA gives copies still in flight (the peer's loads complete on the leader's
+  // barrier) a bounded grace period before the CTAs leave.
+  if (__syncthreads_or(aborted ? 1 : 0)) {
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 2000000ull) {
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs are done with TMEM and with each other's barriers
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols)
+                 : "memory");
+}
+
+// --- host ------------------------------------------------------------------------
+
+// [rows, cols] row-major with row stride ld_bytes, boxes of 128 bytes x box_rows, 128-byte swizzle
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, int size, const void* base, int64_t cols,
+                    int64_t rows, int64_t ld_bytes, uint32_t box_rows, const char* what) {
+  EncodeTiledFn enc = get_encode_fn();
+  ZIB_HOST_CHECK(enc, ZIB_ERR_UNSUPPORTED, "%s: cuTensorMapEncodeTiled unavailable", what);
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld_bytes};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / size), box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  ZIB_HOST_CHECK(r == CUDA_SUCCESS, ZIB_ERR_INVALID_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+  return ZIB_OK;
+}
+
+constexpr int64_t kGroupBudget = 48ll << 20;  // L2 bytes for the operand that every wave re-reads
+
+template <typename T, int BN>
+static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K,
+                       cudaStream_t st, const char* what) {
+  CUtensorMap ta, tb, ty;
+  int rc = make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, K, p.M, ldq, 128u, what);
+  if (!rc) rc = make_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, K, p.N, ldw, BN / 2, what);
+  p.tma_store = ((uintptr_t)p.y % 16 == 0 && p.ldy * sizeof(T) % 16 == 0) ? 1 : 0;
+  ty = ta;
+  if (!rc && p.tma_store)
+    rc = make_map(&ty, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T),
+                  p.y, p.N, p.M, p.ldy * (int64_t)sizeof(T), 32u, what);
+  if (rc) return rc;
+  static bool set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(gemm_pair_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               Cfg<BN>::SMEM);
+    ZIB_HOST_CHECK(e == cudaSuccess, ZIB_ERR_LAUNCH, "%s: cudaFuncSetAttribute failed: %s", what,
+                   cudaGetErrorString(e));
+    set[dev] = true;
+  }
+  p.num_mb = (int)ceil_div(p.M, 256);
+  p.num_nb = (int)ceil_div(p.N, BN);
+  p.num_kb = (int)ceil_div(K, kBlock);
+  ZIB_HOST_CHECK((int64_t)p.num_mb * p.num_nb < (1ll << 30), ZIB_ERR_TOO_LARGE, "%s: M=%d N=%d", what, p.M, p.N);
+  p.num_tiles = p.num_mb * p.num_nb;
+  p.n_fast = (int64_t)p.M * K > (int64_t)p.N * K ? 1 : 0;  // the smaller operand is re-read from L2
+  const int64_t nfast = p.n_fast ? p.num_nb : p.num_mb;
+  const int64_t per = kGroupBudget / ((p.n_fast ? BN : 256) * K);
+  const int64_t groups = ceil_div(nfast, per < 1 ? 1 : per);
+  p.group = (int)ceil_div(nfast, groups);
+  int clusters = sm_count() / 2;
+  if (clusters > p.num_tiles) clusters = p.num_tiles;
+  gemm_pair_kernel<T, BN><<<2 * clusters, kThreads, Cfg<BN>::SMEM, st>>>(ta, tb, ty, p);
+  return zib_check_launch(what);
+}
+
+template <typename T>
+static int gemm(const GemmParams& p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K,
+                cudaStream_t st, const char* what) {
+  // whole waves of 256 x 256 tiles, or twice as many 256 x 128 ones where those end sooner
+  const int64_t pairs = sm_count() / 2, mb = ceil_div(p.M, 256);
+  const int64_t wide = ceil_div(mb * ceil_div(p.N, 256), pairs) * 2, slim = ceil_div(mb * ceil_div(p.N, 128), pairs);
+  if (slim < wide) return launch_pair<T, 128>(p, q, ldq, w, ldw, K, st, what);
+  return launch_pair<T, 256>(p, q, ldq, w, ldw, K, st, what);
+}
+
+}  // namespace fp8
+}  // namespace zib
+
+using namespace zib;
+
+extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
+                                  const void* w, int64_t ldw, const float* sw, int64_t sw_n, int64_t sw_k,
+                                  const void* bias, void* y, int64_t ldy, int dtype, int64_t M, int64_t N, int64_t K,
+                                  void* stream) {
+  const char* what = "zib_fp8_block_gemm";
+  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
+  ZIB_HOST_CHECK(M >= 0 && N >= 1 && K >= 1 && ldq >= K && ldw >= K && ldy >= N, ZIB_ERR_INVALID_ARG,
+                 "%s: bad shape M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
+  ZIB_HOST_CHECK(M < (1ll << 31) - 512 && N < (1ll << 31) - 512 && K < (1ll << 31) - 512, ZIB_ERR_TOO_LARGE,
+                 "%s: M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
+  ZIB_HOST_CHECK(ldq % 16 == 0 && ldw % 16 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)w % 16 == 0,
+                 ZIB_ERR_ALIGNMENT, "%s: q and w need 16-byte aligned rows", what);
+  if (M == 0) return ZIB_OK;
+  ZIB_HOST_CHECK(q && sx && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+  fp8::GemmParams p{};
+  p.M = (int)M; p.N = (int)N;
+  p.sx = sx; p.sx_m = sx_m; p.sx_k = sx_k;
+  p.sw = sw; p.sw_n = sw_n; p.sw_k = sw_k;
+  p.bias = bias; p.y = y; p.ldy = ldy;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == ZIB_BF16) return fp8::gemm<__nv_bfloat16>(p, q, ldq, w, ldw, K, st, what);
+  if (dtype == ZIB_F16) return fp8::gemm<__half>(p, q, ldq, w, ldw, K, st, what);
+  return fp8::gemm<float>(p, q, ldq, w, ldw, K, st, what);
+}

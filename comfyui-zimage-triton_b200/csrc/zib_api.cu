@@ -45,6 +45,7 @@ int zib_err_read_clear_gemm();
 void zib_gemm_split_reset();
 int zib_err_read_clear_rows();
 int zib_err_read_clear_rotary();
+int zib_err_read_clear_fp8();
 
 extern "C" int zib_device_error_read_clear(void) {
   // every stream of the device, non-blocking ones included, has finished before the
@@ -54,8 +55,9 @@ extern "C" int zib_device_error_read_clear(void) {
   int a = zib_err_read_clear_gemm();
   int b = zib_err_read_clear_rows();
   int c = zib_err_read_clear_rotary();
+  int d = zib_err_read_clear_fp8();
   if (a) zib_gemm_split_reset();  // a stopped GEMM may have left split-K counters mid-count
-  return a ? a : b ? b : c;
+  return a ? a : b ? b : d ? d : c;
 }
 
 extern "C" int zib_device_check(int dev) {
