@@ -8,15 +8,21 @@
 // Design (persistent, warp-specialised, clusters of two CTAs, tiles of 256 rows x BN columns):
 //   warp 0     TMA producer: 128-byte swizzled K-major boxes, one K-block of 128 per stage (each CTA
 //              stages its 128 rows of q and half of the BN rows of w).
-//   warp 1     issues tcgen05.mma (cta_group::2, M = 256) from one thread of the leading CTA.  Every
-//              K-block starts a fresh accumulator; the 512 TMEM columns hold 512 / BN of them, so
-//              the MMAs run ahead of the warps that empty them.
-//   warps 2-9  add s * accumulator to their registers: the warps w and w + 4 share a TMEM lane
+//   warp 1     issues tcgen05.mma (cta_group::2, 256 x BN x 32).  Every K-block starts a fresh
+//              accumulator; the 512 TMEM columns hold 512 / BN of them, so the MMAs run ahead of the
+//              warps that empty them.  The whole warp waits and one elected thread issues: descriptors
+//              stay uniform, and four MMAs and two commits take 140 clocks instead of 380.
+//   warps 4-11 add s * accumulator to their registers: the warps w and w + 4 share a TMEM lane
 //              quarter (32 rows) and take half of the BN columns each.  A thread owns one row, so the
 //              row's scale is one value; its BN / 2 columns lie in one block of 128 weight rows, so
 //              that scale is one value too: one packed multiply-add per two elements and K-block.
 //              The output tile leaves through shared memory and TMA stores that drain while the
 //              next tile is summed.
+// What bounds it at 18432 x 11520 x 3840 (723 us, 2250 TFLOP/s): the way of one accumulator from MMA
+// to registers and back to the MMA, 1740 clocks of which the MMAs themselves take 820 (the same
+// pipeline without the sums between blocks runs at 590-650 us, bound by the operands' way to shared
+// memory).  Measured on that way: release at cluster scope 1805 us, one thread waiting and issuing
+// 840 us, accumulators of 128 columns in two halves of the tile 895 us (the rows of q are read twice).
 // Every mbarrier wait is bounded; on expiry the CTA records ZIB_ERR_TIMEOUT in a device error word,
 // drains its loads and MMAs, frees TMEM and exits.
 #include "rot_pack.cuh"
@@ -32,13 +38,16 @@ using namespace tc;
 
 constexpr int kBlock = 128;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = (2 + kEpiWarps) * 32;
+constexpr int kThreads = (4 + kEpiWarps) * 32;
 constexpr int kTmemCols = 512;
 constexpr int kABytes = 128 * kBlock;
 
 template <int BN>
 struct Cfg {
   static constexpr int BUFS = kTmemCols / BN;  // accumulators in flight
+  // Registers: 384 threads start with 168 each (64512); the first warpgroup keeps REGS_ISSUE, the two
+  // that sum take REGS_SUM: 128 * 40 + 256 * 232 = 128 * 56 + 256 * 224 = 64512.
+  static constexpr int REGS_ISSUE = BN == 256 ? 40 : 56, REGS_SUM = BN == 256 ? 232 : 224;
   static constexpr int STAGE = kABytes + BN / 2 * kBlock;
   static constexpr int STAGES = BN == 256 ? 5 : 6;
   static constexpr int XWARP = 8192;  // output staging per warp: two boxes of 32 rows x 128 bytes
@@ -65,23 +74,53 @@ struct GemmParams {
   int tma_store;  // y's rows are 16-byte aligned
 };
 
-__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+// one tcgen05.mma of K = 32; acc is a constant after unrolling
+__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  if (acc)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.eq.u32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc)
+        : "memory");
 }
 
-// waits for this thread's TMEM loads; r is tied in so that no use of it moves above the wait
-__device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
+// true in one thread of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
+
+// bounded wait of a converged warp: the same answer in every thread
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity) || mbar_wait_bounded(bar, parity, abort_flag));
+}
+
+// Arrival on a barrier of the cluster with the default (CTA-scope) release: the accumulator was
+// read by completed tcgen05.ld, ordered by the tcgen05 fence before it.  A release at cluster scope
+// also waits for the thread's global loads in flight (the coming scales): 1805 -> 840 us at
+// 18432 x 11520 x 3840, where every K-block arrives once.
+__device__ __forceinline__ void arrive_pair(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// waits for this thread's TMEM loads; the values are tied in so that no use of them moves above the wait
+#define ZIB_R8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), \
+                     "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void wait_ld(uint32_t (&a)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : ZIB_R8(a, 0), ZIB_R8(a, 8), ZIB_R8(a, 16), ZIB_R8(a, 24) : : "memory");
+}
+// the same tie for a second array of the same wait
+__device__ __forceinline__ void after_wait(uint32_t (&a)[32]) {
+  asm volatile("" : ZIB_R8(a, 0), ZIB_R8(a, 8), ZIB_R8(a, 16), ZIB_R8(a, 24));
+}
+#undef ZIB_R8
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
@@ -115,12 +154,12 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// acc[c * 8 .. c * 8 + 7] (pairs of columns) += s * r
+// acc[at .. at + 15] (pairs of columns) += s * r
 template <int N2>
-__device__ __forceinline__ void add_scaled(px::f2 (&acc)[N2], int c, const uint32_t (&r)[16], px::f2 s2) {
+__device__ __forceinline__ void add_scaled(px::f2 (&acc)[N2], int at, const uint32_t (&r)[32], px::f2 s2) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    acc[c * 8 + j] = px::fma(px::mk(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[c * 8 + j]);
+  for (int j = 0; j < 16; ++j)
+    acc[at + j] = px::fma(px::mk(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s2, acc[at + j]);
 }
 
 // This thread's CW columns of row `row` to y, through the warp's staging boxes (32 rows x 128 bytes,
@@ -242,8 +281,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_holder;
   bool aborted = false;
 
-  if (warp == 0) {
-    if (lane == 0) {  // ---- TMA producer (both CTAs)
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
+    if (warp == 0 && lane == 0) {  // ---- TMA producer (both CTAs)
       int stage = 0;
       uint32_t phase = 0, pend_mask = 0, pend_parity = 0;
       bool ok = true;
@@ -270,9 +310,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (pend_mask & (1u << s)) mbar_drain_wait(&full_bar[s], (pend_parity >> s) & 1u);
       }
     }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0 && leader) {  // ---- MMA issuer
+    if (warp == 1 && leader) {  // ---- MMA issuer: the whole warp waits, one elected thread issues
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       bool ok = true;
@@ -280,30 +318,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc = idesc_f8(256, BN);
       for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
         for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait_bounded(&tempty_bar[buf], buf_phase ^ 1u, abort_flag) ||
-              !mbar_wait_bounded(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t d = tmem_base + (uint32_t)(buf * BN);
+          if (!warp_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
           const uint64_t adesc = sdesc_sw128(base + stage * C::STAGE);
           const uint64_t bdesc = sdesc_sw128(base + stage * C::STAGE + kABytes);
+          if (!warp_wait(&tempty_bar[buf], buf_phase ^ 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem_base + (uint32_t)(buf * BN);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kBlock / 32; ++k)
-            umma_f8_pair(d, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k != 0 ? 1u : 0u);
-          umma_commit_pair(&empty_bar[stage], (uint16_t)3);  // frees the stage in both CTAs
-          umma_commit_pair(&tfull_bar[buf], (uint16_t)3);
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            for (int k = 0; k < kBlock / 32; ++k)
+              umma_f8_pair(d, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k != 0);
+            umma_commit_pair(&tfull_bar[buf], (uint16_t)3);
+            umma_commit_pair(&empty_bar[stage], (uint16_t)3);  // frees the stage in both CTAs
+          }
+          __syncwarp();
           if (++buf == BUFS) { buf = 0; buf_phase ^= 1u; }
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
       }
       if (!ok) aborted = true;
-      umma_commit_pair(mma_done_bar, (uint16_t)1);
-      mbar_drain_wait(mma_done_bar, 0);
+      if (elect_one()) {
+        umma_commit_pair(mma_done_bar, (uint16_t)1);
+        mbar_drain_wait(mma_done_bar, 0);
+      }
     }
     __syncwarp();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SUM));
     // ---- sums over K-blocks and output (both CTAs)
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* xw = xbuf + (warp - 2) * C::XWARP;
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* xw = xbuf + (warp - 4) * C::XWARP;
     const uint32_t t_warp = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * CW);
     int buf = 0;
     uint32_t buf_phase = 0;
@@ -333,30 +377,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           sx = px_ ? __ldg(px_ + (kb + 1) * p.sx_k) : 0.0f;
           sw = pw_ ? __ldg(pw_ + (kb + 1) * p.sw_k) : 0.0f;
         }
-        int got = 1;
-        if (lane == 0) got = mbar_wait_bounded(&tfull_bar[buf], buf_phase, abort_flag) ? 1 : 0;
-        got = __shfl_sync(0xFFFFFFFFu, got, 0);
-        if (!got) { ok = false; break; }
+        if (!warp_wait(&tfull_bar[buf], buf_phase, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const uint32_t ta = t_warp + (uint32_t)(buf * BN);
-        uint32_t r0[16], r1[16];
-        tmem_ld16(ta, r0);
+        uint32_t r0[32], r1[32];
+        tmem_ld32(ta, r0);
+        tmem_ld32(ta + 32u, r1);
         wait_ld(r0);
-#pragma unroll
-        for (int c = 0; c < CW / 16; c += 2) {
-          tmem_ld16(ta + (uint32_t)((c + 1) * 16), r1);
-          add_scaled(acc, c, r0, s2);
-          wait_ld(r1);
-          if (c + 2 < CW / 16) {
-            tmem_ld16(ta + (uint32_t)((c + 2) * 16), r0);
-          } else {  // read: the accumulator may be filled again
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_rank(smem_u32(&tempty_bar[buf]), 0));
-          }
-          add_scaled(acc, c + 1, r1, s2);
-          if (c + 2 < CW / 16) wait_ld(r0);
+        after_wait(r1);
+        if constexpr (CW == 128) {
+          add_scaled(acc, 0, r0, s2);
+          tmem_ld32(ta + 64u, r0);
+          add_scaled(acc, 16, r1, s2);
+          tmem_ld32(ta + 96u, r1);
+          wait_ld(r0);
+          after_wait(r1);
         }
+        // read: the accumulator may be filled again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_pair(mapa_rank(smem_u32(&tempty_bar[buf]), 0));
+        add_scaled(acc, CW / 2 - 32, r0, s2);
+        add_scaled(acc, CW / 2 - 16, r1, s2);
         if (++buf == BUFS) { buf = 0; buf_phase ^= 1u; }
       }
       if (!ok) break;
