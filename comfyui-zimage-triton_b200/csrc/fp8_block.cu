@@ -29,60 +29,105 @@ __device__ __forceinline__ float inverse_scale(float s) {
   const uint32_t b = __float_as_uint(s);
   return b >= 0x7F800000u ? s : __uint_as_float((254u << 23) - b);
 }
-__device__ __forceinline__ uint8_t to_e4m3(float v) {
-  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+// 8 consecutive values from column k of a row of K (16-byte accesses where VEC), 0 past the end
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t k, int64_t K, float (&v)[8]) {
+  if constexpr (VEC) {  // K % 8 == 0: all eight or none
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / E; ++h) {
+      Pack<T, E> t{};
+      if (k < K) t = *reinterpret_cast<const Pack<T, E>*>(row + k + h * E);
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[h * E + j] = to_f32(t.v[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_f32(row[k + j]) : 0.0f;
+  }
 }
-// one warp per (row, block)
-template <typename T>
+
+// The largest magnitude of 8 values, as its bits.
+__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  return a;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t* __restrict__ row, int64_t k, int64_t K, const float (&v)[8],
+                                       float inv) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h] * inv, v[4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h + 2] * inv, v[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    w[h] = lo | (hi << 16);
+  }
+  if constexpr (VEC) {
+    if (k < K) *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < K) row[k + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
+  }
+}
+
+// Activation rows.  Bound by memory (3 bytes per 16-bit element): a warp takes 8 rows of two blocks,
+// 16 lanes x 8 values to a block, with all its loads in flight before the first is used; the 8 rows
+// give each block one whole 32-byte sector of the scales, which lie row after row.
+constexpr int kRowsPerWarp = 8;
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
                                                          int64_t ldq, float* __restrict__ s, int64_t s_m, int64_t s_k,
                                                          int64_t M, int64_t K) {
   const int lane = threadIdx.x & 31;
-  const int64_t kb = (K + kBlock - 1) / kBlock;
+  const int64_t pairs = (K + 2 * kBlock - 1) / (2 * kBlock);
   const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (id >= M * kb) return;
-  const int64_t m = id / kb, b = id - m * kb;
-  float v[4];
-  uint32_t a = 0;
+  const int64_t m0 = id / pairs * kRowsPerWarp;
+  if (m0 >= M) return;
+  const int64_t b = 2 * (id % pairs) + (lane >> 4), k = b * kBlock + (lane & 15) * 8;
+  float v[kRowsPerWarp][8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t k = b * kBlock + lane + 32 * i;
-    v[i] = k < K ? to_f32(x[m * ldx + k]) : 0.0f;
-    const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-    a = bits > a ? bits : a;
-  }
-  a = __reduce_max_sync(0xFFFFFFFFu, a);
-  const float sc = block_scale(a), inv = inverse_scale(sc);
+  for (int r = 0; r < kRowsPerWarp; ++r) load8<T, VEC>(x + (m0 + r) * ldx, k, m0 + r < M ? K : 0, v[r]);
+  float mine = 0.0f;  // lane r of each half warp keeps the scale of row r
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t k = b * kBlock + lane + 32 * i;
-    if (k < K) q[m * ldq + k] = to_e4m3(v[i] * inv);
+  for (int r = 0; r < kRowsPerWarp; ++r) {
+    uint32_t a = amax8(v[r]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+    const float sc = block_scale(a);
+    if ((lane & 15) == r) mine = sc;
+    store8<VEC>(q + (m0 + r) * ldq, k, m0 + r < M ? K : 0, v[r], inverse_scale(sc));
   }
-  if (lane == 0) s[m * s_m + b * s_k] = sc;
+  const int r = lane & 15;
+  if (r < kRowsPerWarp && m0 + r < M && b * kBlock < K) s[(m0 + r) * s_m + b * s_k] = mine;
 }
 
-// one CTA per 128 x 128 block
-template <typename T>
+// Weights: one CTA per block of 128 x 128, held in registers between its maximum and its values.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quant_blocks_kernel(const T* __restrict__ w, int64_t ldw,
                                                            uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s,
                                                            int64_t s_n, int64_t s_k, int64_t N, int64_t K) {
   __shared__ uint32_t red[8];
-  const int64_t n0 = (int64_t)blockIdx.y * kBlock, k = (int64_t)blockIdx.x * kBlock + (threadIdx.x & 127);
+  const int64_t n0 = (int64_t)blockIdx.y * kBlock + (threadIdx.x >> 4);
+  const int64_t k = (int64_t)blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
+  float v[8][8];
   uint32_t a = 0;
-  for (int r = threadIdx.x >> 7; r < kBlock; r += 2) {
-    if (n0 + r < N && k < K) {
-      const uint32_t bits = __float_as_uint(to_f32(w[(n0 + r) * ldw + k])) & 0x7FFFFFFFu;
-      a = bits > a ? bits : a;
-    }
-  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load8<T, VEC>(w + (n0 + 16 * i) * ldw, k, n0 + 16 * i < N ? K : 0, v[i]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, amax8(v[i]));
   a = __reduce_max_sync(0xFFFFFFFFu, a);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = red[i] > a ? red[i] : a;
+  for (int i = 0; i < 8; ++i) a = max(a, red[i]);
   const float sc = block_scale(a), inv = inverse_scale(sc);
-  for (int r = threadIdx.x >> 7; r < kBlock; r += 2)
-    if (n0 + r < N && k < K) q[(n0 + r) * ldq + k] = to_e4m3(to_f32(w[(n0 + r) * ldw + k]) * inv);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) store8<VEC>(q + (n0 + 16 * i) * ldq, k, n0 + 16 * i < N ? K : 0, v[i], inv);
   if (threadIdx.x == 0) s[blockIdx.y * s_n + blockIdx.x * s_k] = sc;
 }
 
@@ -126,6 +171,12 @@ __global__ void __launch_bounds__(256) col_sum_kernel(const float* __restrict__ 
 
 constexpr int kMaxSlabs = 64;
 
+// eight values per access: columns, strides and addresses of input and output allow it
+static bool whole_vectors(const void* x, int64_t ldx, int size, const void* q, int64_t ldq, int64_t rows, int64_t K) {
+  return K % 8 == 0 && (uintptr_t)x % 16 == 0 && (ldx * size % 16 == 0 || rows == 1) && (uintptr_t)q % 8 == 0 &&
+         (ldq % 8 == 0 || rows == 1);
+}
+
 }  // namespace fp8
 }  // namespace zib
 
@@ -139,16 +190,18 @@ extern "C" int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q
                  (long long)M, (long long)K);
   if (M == 0) return ZIB_OK;
   ZIB_HOST_CHECK(x && q && s, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
-  const int64_t grid = ceil_div(M * ceil_div(K, fp8::kBlock), 8);
+  const int64_t grid = ceil_div(ceil_div(M, fp8::kRowsPerWarp) * ceil_div(K, 2 * fp8::kBlock), 8);
   ZIB_HOST_CHECK(grid <= 0x7FFFFFFF, ZIB_ERR_TOO_LARGE, "%s: M=%lld K=%lld", what, (long long)M, (long long)K);
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned g = (unsigned)grid;
-  if (dtype == ZIB_BF16)
-    fp8::quant_rows_kernel<<<g, 256, 0, st>>>((const __nv_bfloat16*)x, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
-  else if (dtype == ZIB_F16)
-    fp8::quant_rows_kernel<<<g, 256, 0, st>>>((const __half*)x, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
-  else
-    fp8::quant_rows_kernel<<<g, 256, 0, st>>>((const float*)x, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
+  const bool vec = fp8::whole_vectors(x, ldx, dtype_bytes(dtype), q, ldq, M, K);
+  auto go = [&](auto kernel, auto* xt) {
+    kernel<<<(unsigned)grid, 256, 0, st>>>(xt, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
+  };
+  using B = __nv_bfloat16;
+  using H = __half;
+  if (dtype == ZIB_BF16) go(vec ? fp8::quant_rows_kernel<B, true> : fp8::quant_rows_kernel<B, false>, (const B*)x);
+  else if (dtype == ZIB_F16) go(vec ? fp8::quant_rows_kernel<H, true> : fp8::quant_rows_kernel<H, false>, (const H*)x);
+  else go(vec ? fp8::quant_rows_kernel<float, true> : fp8::quant_rows_kernel<float, false>, (const float*)x);
   return zib_check_launch(what);
 }
 
@@ -163,12 +216,15 @@ extern "C" int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void*
   ZIB_HOST_CHECK(nb <= 65535, ZIB_ERR_TOO_LARGE, "%s: N=%lld", what, (long long)N);
   cudaStream_t st = (cudaStream_t)stream;
   const dim3 g((unsigned)kb, (unsigned)nb);
-  if (dtype == ZIB_BF16)
-    fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const __nv_bfloat16*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
-  else if (dtype == ZIB_F16)
-    fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const __half*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
-  else
-    fp8::quant_blocks_kernel<<<g, 256, 0, st>>>((const float*)w, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
+  const bool vec = fp8::whole_vectors(w, ldw, dtype_bytes(dtype), q, ldq, N, K);
+  auto go = [&](auto kernel, auto* wt) {
+    kernel<<<g, 256, 0, st>>>(wt, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
+  };
+  using B = __nv_bfloat16;
+  using H = __half;
+  if (dtype == ZIB_BF16) go(vec ? fp8::quant_blocks_kernel<B, true> : fp8::quant_blocks_kernel<B, false>, (const B*)w);
+  else if (dtype == ZIB_F16) go(vec ? fp8::quant_blocks_kernel<H, true> : fp8::quant_blocks_kernel<H, false>, (const H*)w);
+  else go(vec ? fp8::quant_blocks_kernel<float, true> : fp8::quant_blocks_kernel<float, false>, (const float*)w);
   return zib_check_launch(what);
 }
 
