@@ -9,19 +9,35 @@
 //   dx = r (w_c g - c1 - h c2),  c1 = sum_c w_c A_c / n,  c2 = sum_c w_c E_c / n over the group.
 //
 // Bound by memory: the floor is x in and y out (forward), x and dy in and dx out (backward); the
-// statistics need every value before the first output.
+// statistics need every value before the first output, so what does not stay in L2 between the two
+// passes is read twice.  The second pass walks each CTA's pixels backwards: the ones read last are
+// the ones still in L2.
 //
-// Sums.  Runs of a few values of one group are reduced in fp32 to their sum S and their squared
-// deviations from their own mean M; runs meet in fp64 as (sum S, sum M + S^2 / n_run), so a mean
-// that is large against the spread costs no precision.  All sums have a fixed order (no atomics).
-#include "zib_async.cuh"
+// Launches.  Clusters of 8 CTAs sum their pixels and join the sums through distributed shared memory.
+// Where one cluster holds a batch entry (a small tensor, where launches are what costs) it goes on to
+// the outputs: one launch.  Elsewhere the sums of the clusters go through memory and the second
+// launch adds them up in its first instructions (up to kDirectGroups groups; beyond, a small kernel
+// between the two does that once).  Dependent launches start early and wait for the one before them.
+//
+// Sums.  A thread subtracts a value of its own group first (the mean of its first pixel's channels),
+// adds the differences and their squares in fp32 over 8 pixels and joins them in fp64, so a mean that
+// is large against the spread costs no precision.  All sums have a fixed order (no atomics).
+//
+// Arithmetic is on packed pairs (f32x2): at 12 elements per clock and SM, the rate of HBM, single
+// operations left the SMs short of issue slots (79 us instead of TBD for the statistics of
+// [1, 1048576, 128]).
+#include "rot_pack.cuh"
+#include "zib_tcgen05.cuh"
 #include "zib_types.cuh"
 
 namespace zib {
 namespace gn {
 
 constexpr int kThreads = 256;
+constexpr int kCluster = 8;
 constexpr int kMaxChannels = 8192;  // one pixel's partial sums fit shared memory
+constexpr int kDirectGroups = 64;   // groups whose partial sums every CTA of the second pass adds itself
+constexpr int kMaxSmem = 232448;
 
 struct Params {
   const void* x;
@@ -36,282 +52,592 @@ struct Params {
   void* db;
   float* mean;  // [B, G]
   float* rstd;
-  double2* part;    // forward: [B, chunks, G] (sum x, sum x^2); backward: [B, chunks, C] (A, E) as float2
-  float2* coef;     // backward: [B, G] (c1, c2)
+  double2* gpart;  // [B, clusters, G]: (sum x, sum x^2) or (sum w A, sum w E)
+  float2* cpart;   // backward: [B, clusters, C]: (A, E)
+  float2* coef;    // backward: [B, G]: (c1, c2)
   int64_t B, P;
   int C, G, cpg;
-  int V;            // columns of VEC channels
-  int vlanes, rows; // threads: vlanes columns x rows pixels
-  int chunks;
-  int64_t chunk;    // pixels per chunk
+  int V;             // columns of VEC channels
+  int vlanes, rows;  // threads: vlanes columns x rows pixels
+  int clusters;      // per batch entry
+  int chunks;        // CTAs per batch entry (kCluster * clusters in the first pass)
+  int64_t chunk;     // pixels per CTA
   int act;
+  int direct;        // the second pass adds the clusters' sums itself
   float eps;
 };
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_down_sync(0xFFFFFFFFu, v, o);
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
 
-// --- statistics of the forward pass ----------------------------------------------
-
-// GV consecutive channels of a thread share a group (GV divides VEC); RUN pixels per run.
-template <typename T, int VEC, int GV, int RUN>
-__global__ void __launch_bounds__(kThreads) stats_kernel(const Params p) {
-  constexpr int NA = VEC / GV;
-  using V = Pack<T, VEC>;
-  extern __shared__ double2 sm[];  // [rows][V * NA]
-  const int64_t b = blockIdx.y;
-  const int vl = threadIdx.x % p.vlanes, r = threadIdx.x / p.vlanes;
-  const int64_t p0 = (int64_t)blockIdx.x * p.chunk;
-  const int64_t p1 = p0 + p.chunk < p.P ? p0 + p.chunk : p.P;
-  const T* x = reinterpret_cast<const T*>(p.x) + b * p.xsb;
-  if (r < p.rows) {
-    for (int v = vl; v < p.V; v += p.vlanes) {
-      double s[NA], q[NA];
-#pragma unroll
-      for (int a = 0; a < NA; ++a) s[a] = q[a] = 0.0;
-      int64_t i = p0 + r;
-      for (; i + (int64_t)(RUN - 1) * p.rows < p1; i += (int64_t)RUN * p.rows) {
-        V t[RUN];
-#pragma unroll
-        for (int k = 0; k < RUN; ++k)
-          t[k] = *reinterpret_cast<const V*>(x + (i + (int64_t)k * p.rows) * p.xsp + (int64_t)v * VEC);
-#pragma unroll
-        for (int a = 0; a < NA; ++a) {
-          float sum = 0.0f;
-#pragma unroll
-          for (int k = 0; k < RUN; ++k)
-#pragma unroll
-            for (int j = 0; j < GV; ++j) sum += to_f32(t[k].v[a * GV + j]);
-          const float m = sum * (1.0f / (RUN * GV));
-          float dev = 0.0f;
-#pragma unroll
-          for (int k = 0; k < RUN; ++k)
-#pragma unroll
-            for (int j = 0; j < GV; ++j) {
-              const float d = to_f32(t[k].v[a * GV + j]) - m;
-              dev = fmaf(d, d, dev);
-            }
-          // sum (x - m)^2 + 2 m sum - n m^2 for the rounded m, exact in fp64 but for its last bits
-          const double dm = m, ds = sum;
-          s[a] += ds;
-          q[a] += (double)dev + dm * (2.0 * ds - dm * (double)(RUN * GV));
-        }
-      }
-      for (; i < p1; i += p.rows) {
-        const V t = *reinterpret_cast<const V*>(x + i * p.xsp + (int64_t)v * VEC);
-#pragma unroll
-        for (int a = 0; a < NA; ++a)
-#pragma unroll
-          for (int j = 0; j < GV; ++j) {
-            const double d = to_f32(t.v[a * GV + j]);
-            s[a] += d;
-            q[a] = fma(d, d, q[a]);
-          }
-      }
-#pragma unroll
-      for (int a = 0; a < NA; ++a) sm[(int64_t)r * p.V * NA + v * NA + a] = make_double2(s[a], q[a]);
-    }
-  }
-  __syncthreads();
-  // a warp per group: its columns of every thread row, in a fixed order
-  const int cols = p.cpg / GV;  // accumulators per group and row
-  for (int g = threadIdx.x >> 5; g < p.G; g += kThreads / 32) {
-    double s = 0.0, q = 0.0;
-    for (int k = threadIdx.x & 31; k < cols * p.rows; k += 32) {
-      const double2 d = sm[(int64_t)(k / cols) * p.V * NA + g * cols + k % cols];
-      s += d.x;
-      q += d.y;
-    }
-    s = warp_sum(s);
-    q = warp_sum(q);
-    if ((threadIdx.x & 31) == 0) p.part[(b * p.chunks + blockIdx.x) * p.G + g] = make_double2(s, q);
-  }
+// all threads of the cluster (whose warps need not have converged)
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// one warp per (batch entry, group): partial sums to mean and 1 / sqrt(var + eps)
-__global__ void __launch_bounds__(kThreads) finish_stats_kernel(const Params p) {
-  const int64_t id = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (id >= p.B * p.G) return;
-  const int64_t b = id / p.G, g = id - b * p.G;
-  double s = 0.0, q = 0.0;
-  for (int k = threadIdx.x & 31; k < p.chunks; k += 32) {
-    const double2 d = p.part[(b * p.chunks + k) * p.G + g];
-    s += d.x;
-    q += d.y;
+__device__ __forceinline__ double2 ld_cluster(const double2* p, uint32_t rank) {
+  const uint32_t a = tc::mapa_rank(smem_u32(p), rank);
+  double2 v;
+  asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster(const float2* p, uint32_t rank) {
+  const uint32_t a = tc::mapa_rank(smem_u32(p), rank);
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+// a dependent launch may start (it still waits for this grid's memory), and that wait
+__device__ __forceinline__ void allow_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// --- packed pairs ------------------------------------------------------------------
+
+using px::f2;
+
+__device__ __forceinline__ f2 dup(float v) { return px::mk(v, v); }
+
+template <int VEC>
+constexpr int kPairs = VEC < 2 ? 1 : VEC / 2;
+
+// VEC elements as fp32 pairs (a single one with 0 beside it)
+__device__ __forceinline__ f2 pair_of(const __nv_bfloat16* v) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(v);
+  return px::mk(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ f2 pair_of(const __half* v) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(v));
+  return px::mk(f.x, f.y);
+}
+__device__ __forceinline__ f2 pair_of(const float* v) { return px::mk(v[0], v[1]); }
+
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Pack<T, VEC>& t, f2 (&o)[kPairs<VEC>]) {
+  if constexpr (VEC == 1) o[0] = px::mk(to_f32(t.v[0]), 0.0f);
+  else
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) o[i] = pair_of(t.v + 2 * i);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> pack(const f2 (&o)[kPairs<VEC>]) {
+  Pack<T, VEC> t;
+#pragma unroll
+  for (int i = 0; i < kPairs<VEC>; ++i) {
+    float lo, hi;
+    px::split(o[i], lo, hi);
+    t.v[2 * i] = from_f32<T>(lo);
+    if constexpr (VEC > 1) t.v[2 * i + 1] = from_f32<T>(hi);
   }
-  s = warp_sum(s);
-  q = warp_sum(q);
-  if ((threadIdx.x & 31) == 0) {
-    const double n = (double)p.P * (double)p.cpg;
-    const double m = s / n;
-    double var = q / n - m * m;
-    if (var < 0.0) var = 0.0;
-    p.mean[id] = (float)m;
-    p.rstd[id] = (float)(1.0 / sqrt(var + (double)p.eps));
-  }
+  return t;
 }
 
 // --- activation ------------------------------------------------------------------
 
-// 1 / (1 + e^-z): the fast exponential and division where the result is rounded to 16 bits, the
-// accurate ones where it is kept in 32
+// 1 / (1 + e^-z): the fast power of two and reciprocal where the result is rounded to 16 bits, the
+// accurate functions where it is kept in 32
 template <typename T>
-__device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (sizeof(T) == 2) return __fdividef(1.0f, 1.0f + __expf(-z));
-  else return 1.0f / (1.0f + expf(-z));
+__device__ __forceinline__ f2 sigmoid(f2 z) {
+  float a, b;
+  if constexpr (sizeof(T) == 2) {
+    px::split(px::mul(z, dup(-1.4426950408889634f)), a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    px::split(px::add(px::mk(a, b), dup(1.0f)), a, b);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  } else {
+    px::split(z, a, b);
+    a = 1.0f / (1.0f + expf(-a));
+    b = 1.0f / (1.0f + expf(-b));
+  }
+  return px::mk(a, b);
 }
 
 template <typename T>
-__device__ __forceinline__ float activate(float z, int act) {
-  return act == ZIB_ACT_SILU ? z * sigmoid<T>(z) : z;
+__device__ __forceinline__ f2 activate(f2 z, int act) {
+  return act == ZIB_ACT_SILU ? px::mul(z, sigmoid<T>(z)) : z;
 }
 
-// act'(z)
+// act'(z) = s (1 + z (1 - s))
 template <typename T>
-__device__ __forceinline__ float slope(float z, int act) {
-  if (act != ZIB_ACT_SILU) return 1.0f;
-  const float s = sigmoid<T>(z);
-  return s * fmaf(z, 1.0f - s, 1.0f);
+__device__ __forceinline__ f2 slope(f2 z, int act) {
+  if (act != ZIB_ACT_SILU) return dup(1.0f);
+  const f2 s = sigmoid<T>(z);
+  return px::mul(s, px::fma(z, px::sub(dup(1.0f), s), dup(1.0f)));
 }
 
-// per-thread constants of VEC channels from channel c0 of batch entry b
+// --- a thread's share of a CTA's pixels -------------------------------------------
+
+struct Slab {
+  int64_t b, p0, p1;  // batch entry, pixels [p0, p1)
+  int vl, r;          // column lane, pixel row
+  __device__ __forceinline__ Slab(const Params& p, int chunk) {
+    b = blockIdx.y;
+    vl = threadIdx.x % p.vlanes;
+    r = threadIdx.x / p.vlanes;
+    p0 = chunk * p.chunk;
+    p1 = p0 + p.chunk < p.P ? p0 + p.chunk : p.P;
+    if (p0 > p1) p0 = p1;
+  }
+};
+
+// --- forward statistics --------------------------------------------------------------
+
+// The sums of this CTA's pixels by group into sm[0 .. G) (sum x, sum x^2); scratch behind them.  GV
+// consecutive channels of a thread share a group; RUN pixels are in flight at a time.
+template <typename T, int VEC, int GV>
+__device__ __forceinline__ void slab_stats(const Params& p, const Slab& s, double2* sm) {
+  constexpr int NA = VEC / GV, NP = kPairs<VEC>, RUN = NA > 2 ? 4 : 8;
+  using V = Pack<T, VEC>;
+  const int cols = p.cpg / GV;  // sums per group and thread row
+  // [rows][V * NA]; with one sum per group it is the result
+  double2* scratch = cols * p.rows == 1 ? sm : sm + p.G;
+  const T* x = reinterpret_cast<const T*>(p.x) + s.b * p.xsb;
+  if (s.r < p.rows) {
+    for (int v = s.vl; v < p.V; v += p.vlanes) {
+      double sum[NA], sq[NA];
+      float piv[NA];
+#pragma unroll
+      for (int a = 0; a < NA; ++a) {
+        sum[a] = sq[a] = 0.0;
+        piv[a] = 0.0f;
+      }
+      const T* xv = x + (int64_t)v * VEC;
+      const int64_t p0 = s.p0 + s.r, step = p.rows * p.xsp;
+      if (p0 < s.p1) {
+        const V t = *reinterpret_cast<const V*>(xv + p0 * p.xsp);
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+#pragma unroll
+          for (int j = 0; j < GV; ++j) piv[a] += to_f32(t.v[a * GV + j]);
+          piv[a] *= 1.0f / GV;
+        }
+      }
+      f2 pv[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) pv[i] = VEC == 1 ? px::mk(piv[0], 0.0f) : px::mk(piv[2 * i / GV], piv[(2 * i + 1) / GV % NA]);
+      const int n = s.p1 > p0 ? (int)((s.p1 - p0 + p.rows - 1) / p.rows) : 0;  // this thread's pixels
+      const T* at = xv + p0 * p.xsp;
+      for (int i = 0; i < n; i += RUN, at += RUN * step) {
+        V t[RUN];
+#pragma unroll
+        for (int k = 0; k < RUN; ++k)
+          if (i + k < n) t[k] = *reinterpret_cast<const V*>(at + k * step);
+        f2 u[NP], w[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) u[j] = w[j] = 0ull;
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) {
+          if (i + k >= n) break;
+          f2 d[NP];
+          unpack<T, VEC>(t[k], d);
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            d[j] = px::sub(d[j], pv[j]);
+            u[j] = px::add(u[j], d[j]);
+            w[j] = px::fma(d[j], d[j], w[j]);
+          }
+        }
+        float us[2 * NP], ws[2 * NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          px::split(u[j], us[2 * j], us[2 * j + 1]);
+          px::split(w[j], ws[2 * j], ws[2 * j + 1]);
+        }
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+#pragma unroll
+          for (int j = 1; j < GV; ++j) {
+            us[a * GV] += us[a * GV + j];
+            ws[a * GV] += ws[a * GV + j];
+          }
+          sum[a] += (double)us[a * GV];
+          sq[a] += (double)ws[a * GV];
+        }
+      }
+      // back from the differences: sum x = sum d + n m, sum x^2 = sum d^2 + 2 m sum d + n m^2
+#pragma unroll
+      for (int a = 0; a < NA; ++a) {
+        const double m = piv[a], nm = (double)n * GV * m;
+        scratch[s.r * p.V * NA + v * NA + a] = make_double2(sum[a] + nm, sq[a] + m * (2.0 * sum[a] + nm));
+      }
+    }
+  }
+  if (scratch == sm) return;
+  __syncthreads();
+  // a warp per group: its columns of every thread row, in a fixed order
+  for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
+    double a = 0.0, q = 0.0;
+    for (int k = threadIdx.x & 31; k < cols * p.rows; k += 32) {
+      const double2 d = scratch[(k / cols) * p.V * NA + g * cols + k % cols];
+      a += d.x;
+      q += d.y;
+    }
+    a = warp_sum(a);
+    q = warp_sum(q);
+    if ((threadIdx.x & 31) == 0) sm[g] = make_double2(a, q);
+  }
+}
+
+// the cluster's sum of element g of an array that each of its CTAs holds
+template <typename D>
+__device__ __forceinline__ D cluster_sum(const D* sm, int g) {
+  D v[kCluster];
+#pragma unroll
+  for (int k = 0; k < kCluster; ++k) v[k] = ld_cluster(sm + g, k);
+#pragma unroll
+  for (int k = 1; k < kCluster; ++k) {
+    v[0].x += v[k].x;
+    v[0].y += v[k].y;
+  }
+  return v[0];
+}
+
+__device__ __forceinline__ void finish(const Params& p, double s, double q, float& mean, float& rstd) {
+  const double n = (double)p.P * (double)p.cpg;
+  const double m = s / n;
+  double var = q / n - m * m;
+  if (var < 0.0) var = 0.0;
+  mean = (float)m;
+  rstd = (float)(1.0 / sqrt(var + (double)p.eps));
+}
+
+// element g of the clusters' sums of batch entry b, added by a warp in a fixed order
+__device__ __forceinline__ double2 sum_clusters(const Params& p, int64_t b, int g) {
+  double s = 0.0, q = 0.0;
+  for (int k = threadIdx.x & 31; k < p.clusters; k += 32) {
+    const double2 d = __ldcg(p.gpart + (b * p.clusters + k) * p.G + g);
+    s += d.x;
+    q += d.y;
+  }
+  return make_double2(warp_sum(s), warp_sum(q));
+}
+
+// --- outputs -----------------------------------------------------------------------
+
+// mean, 1 / sqrt(var + eps), weight and bias of VEC channels from channel c0; mean and rstd by group
 template <int VEC>
 struct Affine {
-  float mu[VEC], r[VEC], w[VEC], b[VEC];
-  __device__ __forceinline__ void load(const Params& p, int64_t bi, int c0) {
+  f2 mu[kPairs<VEC>], r[kPairs<VEC>], w[kPairs<VEC>], b[kPairs<VEC>];
+  __device__ __forceinline__ void load(const Params& p, const float* mean, const float* rstd, int c0) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int c = c0 + j;
-      const int64_t g = bi * p.G + c / p.cpg;
-      mu[j] = p.mean[g];
-      r[j] = p.rstd[g];
-      w[j] = p.w ? load_as_f32(p.w, p.wdtype, c) : 1.0f;
-      b[j] = p.b ? load_as_f32(p.b, p.wdtype, c) : 0.0f;
+    for (int i = 0; i < kPairs<VEC>; ++i) {
+      float m[2] = {0.0f, 0.0f}, q[2] = {0.0f, 0.0f}, v[2] = {0.0f, 0.0f}, a[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < (VEC == 1 ? 1 : 2); ++j) {
+        const int c = c0 + 2 * i + j, g = c / p.cpg;
+        m[j] = mean[g];
+        q[j] = rstd[g];
+        v[j] = p.w ? load_as_f32(p.w, p.wdtype, c) : 1.0f;
+        a[j] = p.b ? load_as_f32(p.b, p.wdtype, c) : 0.0f;
+      }
+      mu[i] = px::mk(m[0], m[1]);
+      r[i] = px::mk(q[0], q[1]);
+      w[i] = px::mk(v[0], v[1]);
+      b[i] = px::mk(a[0], a[1]);
     }
   }
 };
 
+// y of a CTA's pixels, last ones first; U loads in flight before the first store
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) apply_kernel(const Params p) {
+__device__ __forceinline__ void slab_apply(const Params& p, const Slab& s, const float* mean, const float* rstd) {
   using V = Pack<T, VEC>;
-  const int64_t b = blockIdx.y;
-  const int vl = threadIdx.x % p.vlanes, r = threadIdx.x / p.vlanes;
-  if (r >= p.rows) return;
-  // last pixels first: the statistics pass read them last, so they are the ones still in L2
-  const int64_t p0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * p.chunk;
-  const int64_t p1 = p0 + p.chunk < p.P ? p0 + p.chunk : p.P;
-  const T* x = reinterpret_cast<const T*>(p.x) + b * p.xsb;
-  T* y = reinterpret_cast<T*>(p.out) + b * p.P * p.C;
-  for (int v = vl; v < p.V; v += p.vlanes) {
+  constexpr int U = 4, NP = kPairs<VEC>;
+  if (s.r >= p.rows) return;
+  const int64_t p0 = s.p0 + s.r;
+  const int n = s.p1 > p0 ? (int)((s.p1 - p0 + p.rows - 1) / p.rows) : 0;
+  const int64_t xstep = p.rows * p.xsp, ystep = (int64_t)p.rows * p.C;
+  for (int v = s.vl; v < p.V; v += p.vlanes) {
     Affine<VEC> f;
-    f.load(p, b, v * VEC);
-#pragma unroll 4
-    for (int64_t i = p0 + r; i < p1; i += p.rows) {
-      const V t = *reinterpret_cast<const V*>(x + i * p.xsp + (int64_t)v * VEC);
-      V o;
+    f.load(p, mean, rstd, v * VEC);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float h = (to_f32(t.v[j]) - f.mu[j]) * f.r[j];
-        o.v[j] = from_f32<T>(activate<T>(fmaf(h, f.w[j], f.b[j]), p.act));
+    for (int j = 0; j < NP; ++j) f.r[j] = px::mul(f.r[j], f.w[j]);
+    const T* xv = reinterpret_cast<const T*>(p.x) + s.b * p.xsb + (p0 + (int64_t)(n - 1) * p.rows) * p.xsp + (int64_t)v * VEC;
+    T* yv = reinterpret_cast<T*>(p.out) + (s.b * p.P + p0 + (int64_t)(n - 1) * p.rows) * p.C + (int64_t)v * VEC;
+    for (int i = 0; i < n; i += U, xv -= U * xstep, yv -= U * ystep) {
+      V t[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (i + k < n) t[k] = *reinterpret_cast<const V*>(xv - k * xstep);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i + k >= n) break;
+        f2 d[NP];
+        unpack<T, VEC>(t[k], d);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) d[j] = activate<T>(px::fma(px::sub(d[j], f.mu[j]), f.r[j], f.b[j]), p.act);
+        *reinterpret_cast<V*>(yv - k * ystep) = pack<T, VEC>(d);
       }
-      *reinterpret_cast<V*>(y + i * p.C + (int64_t)v * VEC) = o;
     }
   }
+}
+
+// FUSED: one cluster per batch entry, outputs included; else the clusters' sums to memory
+template <typename T, int VEC, int GV, bool FUSED>
+__global__ void __launch_bounds__(kThreads, 3) stats_kernel(const Params p) {
+  extern __shared__ double2 sm[];  // [G], then scratch
+  const Slab s(p, blockIdx.x);
+  slab_stats<T, VEC, GV>(p, s, sm);
+  cluster_barrier();
+  if constexpr (FUSED) {
+    float* mean = reinterpret_cast<float*>(sm + p.G);  // the scratch is free again
+    float* rstd = mean + p.G;
+    const bool first = tc::cluster_rank() == 0;
+    for (int g = threadIdx.x; g < p.G; g += blockDim.x) {
+      const double2 d = cluster_sum(sm, g);
+      float m, r;
+      finish(p, d.x, d.y, m, r);
+      mean[g] = m;
+      rstd[g] = r;
+      if (first) {
+        p.mean[s.b * p.G + g] = m;
+        p.rstd[s.b * p.G + g] = r;
+      }
+    }
+    __syncthreads();
+    slab_apply<T, VEC>(p, s, mean, rstd);
+  } else {
+    const int rank = (int)tc::cluster_rank();
+    for (int g = rank + kCluster * (int)threadIdx.x; g < p.G; g += kCluster * (int)blockDim.x)
+      p.gpart[(s.b * p.clusters + blockIdx.x / kCluster) * p.G + g] = cluster_sum(sm, g);
+    allow_dependents();
+  }
+  cluster_barrier();  // nobody leaves while its sums are read
+}
+
+// one warp per (batch entry, group)
+__global__ void __launch_bounds__(256) finish_stats_kernel(const Params p) {
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  wait_for_primary();
+  if (id < p.B * p.G) {
+    const int64_t b = id / p.G;
+    const double2 d = sum_clusters(p, b, (int)(id - b * p.G));
+    float m, r;
+    finish(p, d.x, d.y, m, r);
+    if ((threadIdx.x & 31) == 0) {
+      p.mean[id] = m;
+      p.rstd[id] = r;
+    }
+  }
+  allow_dependents();
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads, 4) apply_kernel(const Params p) {
+  __shared__ float mean[kDirectGroups], rstd[kDirectGroups];
+  const Slab s(p, blockIdx.x);
+  wait_for_primary();
+  if (!p.direct) {
+    slab_apply<T, VEC>(p, s, p.mean + s.b * p.G, p.rstd + s.b * p.G);
+    return;
+  }
+  for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
+    const double2 d = sum_clusters(p, s.b, g);
+    if ((threadIdx.x & 31) == 0) {
+      finish(p, d.x, d.y, mean[g], rstd[g]);
+      if (blockIdx.x == 0) {
+        p.mean[s.b * p.G + g] = mean[g];
+        p.rstd[s.b * p.G + g] = rstd[g];
+      }
+    }
+  }
+  __syncthreads();
+  slab_apply<T, VEC>(p, s, mean, rstd);
 }
 
 // --- backward --------------------------------------------------------------------
 
-// A_c and E_c of one chunk of pixels
+// A_c and E_c of a CTA's pixels into sm[0 .. C)
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) grad_stats_kernel(const Params p) {
+__device__ __forceinline__ void slab_grad_stats(const Params& p, const Slab& s, float2* sm) {
   using V = Pack<T, VEC>;
-  extern __shared__ double2 sm[];
-  float2* sf = reinterpret_cast<float2*>(sm);  // [rows][vlanes * VEC]
-  const int64_t b = blockIdx.y;
-  const int vl = threadIdx.x % p.vlanes, r = threadIdx.x / p.vlanes;
-  const int64_t p0 = (int64_t)blockIdx.x * p.chunk;
-  const int64_t p1 = p0 + p.chunk < p.P ? p0 + p.chunk : p.P;
-  const T* x = reinterpret_cast<const T*>(p.x) + b * p.xsb;
-  const T* dy = reinterpret_cast<const T*>(p.dy) + b * p.dsb;
-  float2* part = reinterpret_cast<float2*>(p.part) + (b * p.chunks + blockIdx.x) * p.C;
+  constexpr int U = sizeof(T) == 2 ? 4 : 2, NP = kPairs<VEC>;
+  float2* scratch = sm + p.C;  // [rows][vlanes * VEC]
   const int width = p.vlanes * VEC;
+  const int64_t p0 = s.p0 + s.r, xstep = p.rows * p.xsp, dstep = p.rows * p.dsp;
+  const int n = s.p1 > p0 ? (int)((s.p1 - p0 + p.rows - 1) / p.rows) : 0;
   for (int v0 = 0; v0 < p.V; v0 += p.vlanes) {
-    const int v = v0 + vl;
-    if (r < p.rows && v < p.V) {
+    const int v = v0 + s.vl;
+    if (s.r < p.rows && v < p.V) {
       Affine<VEC> f;
-      f.load(p, b, v * VEC);
-      float A[VEC], E[VEC];
+      f.load(p, p.mean + s.b * p.G, p.rstd + s.b * p.G, v * VEC);
+      const T* xv = reinterpret_cast<const T*>(p.x) + s.b * p.xsb + p0 * p.xsp + (int64_t)v * VEC;
+      const T* dv = reinterpret_cast<const T*>(p.dy) + s.b * p.dsb + p0 * p.dsp + (int64_t)v * VEC;
+      f2 A[NP], E[NP];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) A[j] = E[j] = 0.0f;
-#pragma unroll 2
-      for (int64_t i = p0 + r; i < p1; i += p.rows) {
-        const V t = *reinterpret_cast<const V*>(x + i * p.xsp + (int64_t)v * VEC);
-        const V d = *reinterpret_cast<const V*>(dy + i * p.dsp + (int64_t)v * VEC);
+      for (int j = 0; j < NP; ++j) A[j] = E[j] = 0ull;
+      for (int i = 0; i < n; i += U, xv += U * xstep, dv += U * dstep) {
+        V t[U], d[U];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float h = (to_f32(t.v[j]) - f.mu[j]) * f.r[j];
-          const float g = to_f32(d.v[j]) * slope<T>(fmaf(h, f.w[j], f.b[j]), p.act);
-          A[j] += g;
-          E[j] = fmaf(g, h, E[j]);
+        for (int k = 0; k < U; ++k)
+          if (i + k < n) {
+            t[k] = *reinterpret_cast<const V*>(xv + k * xstep);
+            d[k] = *reinterpret_cast<const V*>(dv + k * dstep);
+          }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (i + k >= n) break;
+          f2 h[NP], g[NP];
+          unpack<T, VEC>(t[k], h);
+          unpack<T, VEC>(d[k], g);
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            h[j] = px::mul(px::sub(h[j], f.mu[j]), f.r[j]);
+            g[j] = px::mul(g[j], slope<T>(px::fma(h[j], f.w[j], f.b[j]), p.act));
+            A[j] = px::add(A[j], g[j]);
+            E[j] = px::fma(g[j], h[j], E[j]);
+          }
         }
       }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sf[r * width + vl * VEC + j] = make_float2(A[j], E[j]);
+      for (int j = 0; j < NP; ++j) {
+        float a0, a1, e0, e1;
+        px::split(A[j], a0, a1);
+        px::split(E[j], e0, e1);
+        float2* at = scratch + s.r * width + s.vl * VEC + 2 * j;
+        at[0] = make_float2(a0, e0);
+        if constexpr (VEC > 1) at[1] = make_float2(a1, e1);
+      }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < width && v0 * VEC + c < p.C; c += kThreads) {
+    for (int c = threadIdx.x; c < width && v0 * VEC + c < p.C; c += blockDim.x) {
       double A = 0.0, E = 0.0;
       for (int k = 0; k < p.rows; ++k) {
-        const float2 s = sf[k * width + c];
-        A += s.x;
-        E += s.y;
+        const float2 t = scratch[k * width + c];
+        A += t.x;
+        E += t.y;
       }
-      part[v0 * VEC + c] = make_float2((float)A, (float)E);
+      sm[v0 * VEC + c] = make_float2((float)A, (float)E);
     }
     __syncthreads();
   }
 }
 
-// one CTA per group: its channels' sums over chunks, c1 and c2 per batch entry, dw and db
-__global__ void __launch_bounds__(kThreads) finish_grad_kernel(const Params p) {
-  __shared__ double red[2][kThreads / 32];
-  const int g = blockIdx.x;
-  const float2* part = reinterpret_cast<const float2*>(p.part);
-  const double n = (double)p.P * (double)p.cpg;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // c1, c2
-  if (p.coef) {
-    for (int64_t b = 0; b < p.B; ++b) {
-      double s1 = 0.0, s2 = 0.0;
-      for (int64_t k = threadIdx.x; k < (int64_t)p.chunks * p.cpg; k += kThreads) {
-        const int c = g * p.cpg + (int)(k % p.cpg);
-        const float2 a = part[(b * p.chunks + k / p.cpg) * p.C + c];
-        const double w = p.w ? (double)load_as_f32(p.w, p.wdtype, c) : 1.0;
-        s1 += w * a.x;
-        s2 += w * a.y;
+// dx of a CTA's pixels, last ones first
+template <typename T, int VEC>
+__device__ __forceinline__ void slab_grad_apply(const Params& p, const Slab& s, const float2* coef) {
+  using V = Pack<T, VEC>;
+  constexpr int U = sizeof(T) == 2 ? 4 : 2, NP = kPairs<VEC>;
+  if (s.r >= p.rows) return;
+  const int64_t p0 = s.p0 + s.r;
+  const int n = s.p1 > p0 ? (int)((s.p1 - p0 + p.rows - 1) / p.rows) : 0;
+  const int64_t last = p0 + (int64_t)(n - 1) * p.rows;
+  const int64_t xstep = p.rows * p.xsp, dstep = p.rows * p.dsp, ostep = (int64_t)p.rows * p.C;
+  for (int v = s.vl; v < p.V; v += p.vlanes) {
+    Affine<VEC> f;
+    f.load(p, p.mean + s.b * p.G, p.rstd + s.b * p.G, v * VEC);
+    f2 c1[NP], c2[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const float2 a = coef[(v * VEC + 2 * j) / p.cpg], b = VEC == 1 ? a : coef[(v * VEC + 2 * j + 1) / p.cpg];
+      c1[j] = px::mk(-a.x, -b.x);
+      c2[j] = px::mk(-a.y, -b.y);
+    }
+    const T* xv = reinterpret_cast<const T*>(p.x) + s.b * p.xsb + last * p.xsp + (int64_t)v * VEC;
+    const T* dv = reinterpret_cast<const T*>(p.dy) + s.b * p.dsb + last * p.dsp + (int64_t)v * VEC;
+    T* ov = reinterpret_cast<T*>(p.out) + (s.b * p.P + last) * p.C + (int64_t)v * VEC;
+    for (int i = 0; i < n; i += U, xv -= U * xstep, dv -= U * dstep, ov -= U * ostep) {
+      V t[U], d[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (i + k < n) {
+          t[k] = *reinterpret_cast<const V*>(xv - k * xstep);
+          d[k] = *reinterpret_cast<const V*>(dv - k * dstep);
+        }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i + k >= n) break;
+        f2 h[NP], g[NP];
+        unpack<T, VEC>(t[k], h);
+        unpack<T, VEC>(d[k], g);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          h[j] = px::mul(px::sub(h[j], f.mu[j]), f.r[j]);
+          g[j] = px::mul(g[j], slope<T>(px::fma(h[j], f.w[j], f.b[j]), p.act));
+          g[j] = px::mul(f.r[j], px::fma(h[j], c2[j], px::fma(f.w[j], g[j], c1[j])));
+        }
+        *reinterpret_cast<V*>(ov - k * ostep) = pack<T, VEC>(g);
       }
-      s1 = warp_sum(s1);
-      s2 = warp_sum(s2);
-      if (lane == 0) { red[0][warp] = s1; red[1][warp] = s2; }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        double t1 = 0.0, t2 = 0.0;
-        for (int k = 0; k < kThreads / 32; ++k) { t1 += red[0][k]; t2 += red[1][k]; }
-        p.coef[b * p.G + g] = make_float2((float)(t1 / n), (float)(t2 / n));
-      }
-      __syncthreads();
     }
   }
-  if (!p.dw && !p.db) return;
-  for (int c = g * p.cpg + warp; c < (g + 1) * p.cpg; c += kThreads / 32) {
+}
+
+// (sum w A, sum w E) of group g over channel sums ae[0 .. C), by a warp
+__device__ __forceinline__ double2 group_sums(const Params& p, const float2* ae, int g) {
+  double a = 0.0, e = 0.0;
+  for (int k = threadIdx.x & 31; k < p.cpg; k += 32) {
+    const int c = g * p.cpg + k;
+    const double w = p.w ? (double)load_as_f32(p.w, p.wdtype, c) : 1.0;
+    a += w * ae[c].x;
+    e += w * ae[c].y;
+  }
+  return make_double2(warp_sum(a), warp_sum(e));
+}
+
+template <typename T, int VEC, bool FUSED>
+__global__ void __launch_bounds__(kThreads, 3) grad_stats_kernel(const Params p) {
+  extern __shared__ double2 sm[];
+  float2* ae = reinterpret_cast<float2*>(sm);  // [C] of this CTA, [C] scratch or the cluster's sums
+  const Slab s(p, blockIdx.x);
+  const int rank = (int)tc::cluster_rank();
+  const int64_t cl = s.b * p.clusters + blockIdx.x / kCluster;
+  slab_grad_stats<T, VEC>(p, s, ae);
+  cluster_barrier();
+  float2* all = ae + p.C;
+  for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
+    const float2 t = cluster_sum(ae, c);
+    all[c] = t;
+    if (c % kCluster == rank) p.cpart[cl * p.C + c] = t;
+  }
+  __syncthreads();
+  const double n = (double)p.P * (double)p.cpg;
+  float2* coef = all + p.C;
+  if (p.out) {
+    for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
+      if (!FUSED && g % kCluster != rank) continue;
+      const double2 t = group_sums(p, all, g);
+      if ((threadIdx.x & 31) == 0) {
+        if constexpr (FUSED) coef[g] = make_float2((float)(t.x / n), (float)(t.y / n));
+        else p.gpart[cl * p.G + g] = t;
+      }
+    }
+  }
+  allow_dependents();
+  if constexpr (FUSED) {
+    __syncthreads();
+    if (p.out) slab_grad_apply<T, VEC>(p, s, coef);
+  }
+  cluster_barrier();  // nobody leaves while its sums are read
+}
+
+// one warp per (batch entry, group): c1, c2
+__global__ void __launch_bounds__(256) finish_grad_kernel(const Params p) {
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  wait_for_primary();
+  if (id < p.B * p.G) {
+    const int64_t b = id / p.G;
+    const double n = (double)p.P * (double)p.cpg;
+    const double2 t = sum_clusters(p, b, (int)(id - b * p.G));
+    if ((threadIdx.x & 31) == 0) p.coef[id] = make_float2((float)(t.x / n), (float)(t.y / n));
+  }
+  allow_dependents();
+}
+
+// dw and db of channels from c0 on, a warp to a channel: sums over batch entries and clusters
+__device__ __forceinline__ void param_grads(const Params& p, int c0, int step) {
+  const int lane = threadIdx.x & 31;
+  for (int c = c0 + (int)(threadIdx.x >> 5); c < p.C; c += step) {
     double A = 0.0, E = 0.0;
-    for (int64_t k = lane; k < p.B * p.chunks; k += 32) {
-      const float2 a = part[k * p.C + c];
-      A += a.x;
-      E += a.y;
+    for (int64_t k = lane; k < p.B * p.clusters; k += 32) {
+      const float2 t = __ldcg(p.cpart + k * p.C + c);
+      A += t.x;
+      E += t.y;
     }
     A = warp_sum(A);
     E = warp_sum(E);
@@ -322,41 +648,36 @@ __global__ void __launch_bounds__(kThreads) finish_grad_kernel(const Params p) {
   }
 }
 
+// dw and db alone
+__global__ void __launch_bounds__(256) param_grad_kernel(const Params p) {
+  wait_for_primary();
+  param_grads(p, (int)blockIdx.x * 8, (int)gridDim.x * 8);
+}
+
+// dx; the CTAs behind the last chunk of batch entry 0 form dw and db
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) grad_apply_kernel(const Params p) {
-  using V = Pack<T, VEC>;
-  const int64_t b = blockIdx.y;
-  const int vl = threadIdx.x % p.vlanes, r = threadIdx.x / p.vlanes;
-  if (r >= p.rows) return;
-  const int64_t p0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * p.chunk;
-  const int64_t p1 = p0 + p.chunk < p.P ? p0 + p.chunk : p.P;
-  const T* x = reinterpret_cast<const T*>(p.x) + b * p.xsb;
-  const T* dy = reinterpret_cast<const T*>(p.dy) + b * p.dsb;
-  T* dx = reinterpret_cast<T*>(p.out) + b * p.P * p.C;
-  for (int v = vl; v < p.V; v += p.vlanes) {
-    Affine<VEC> f;
-    f.load(p, b, v * VEC);
-    float c1[VEC], c2[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float2 c = p.coef[b * p.G + (v * VEC + j) / p.cpg];
-      c1[j] = c.x;
-      c2[j] = c.y;
+__global__ void __launch_bounds__(kThreads, 3) grad_apply_kernel(const Params p) {
+  __shared__ float2 coef[kDirectGroups];
+  wait_for_primary();
+  if ((int)blockIdx.x >= p.chunks) {
+    if (blockIdx.y == 0) {
+      const int warps = (int)blockDim.x >> 5;
+      param_grads(p, ((int)blockIdx.x - p.chunks) * warps, ((int)gridDim.x - p.chunks) * warps);
     }
-#pragma unroll 2
-    for (int64_t i = p0 + r; i < p1; i += p.rows) {
-      const V t = *reinterpret_cast<const V*>(x + i * p.xsp + (int64_t)v * VEC);
-      const V d = *reinterpret_cast<const V*>(dy + i * p.dsp + (int64_t)v * VEC);
-      V o;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float h = (to_f32(t.v[j]) - f.mu[j]) * f.r[j];
-        const float g = to_f32(d.v[j]) * slope<T>(fmaf(h, f.w[j], f.b[j]), p.act);
-        o.v[j] = from_f32<T>(f.r[j] * (fmaf(f.w[j], g, -c1[j]) - h * c2[j]));
-      }
-      *reinterpret_cast<V*>(dx + i * p.C + (int64_t)v * VEC) = o;
-    }
+    return;
   }
+  const Slab s(p, blockIdx.x);
+  if (!p.direct) {
+    slab_grad_apply<T, VEC>(p, s, p.coef + s.b * p.G);
+    return;
+  }
+  const double n = (double)p.P * (double)p.cpg;
+  for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
+    const double2 t = sum_clusters(p, s.b, g);
+    if ((threadIdx.x & 31) == 0) coef[g] = make_float2((float)(t.x / n), (float)(t.y / n));
+  }
+  __syncthreads();
+  slab_grad_apply<T, VEC>(p, s, coef);
 }
 
 // --- host ------------------------------------------------------------------------
@@ -366,57 +687,129 @@ static int gcd(int a, int b) {
   return a;
 }
 
-// Splits P pixels into chunks: about four CTAs per SM over the batch, at least 8 pixels per thread.
-static void plan(Params& p, int vec) {
+// clusters per batch entry: four CTAs per SM in all, at most one per 8 pixels
+static int64_t most_clusters(int64_t B, int64_t P) {
+  if (B < 1 || P < 1) return 1;
+  int64_t c = (int64_t)sm_count() * 4 / (kCluster * B);
+  const int64_t m = ceil_div(P, kCluster * 8);
+  if (c > m) c = m;
+  return c < 1 ? 1 : c;
+}
+
+// One cluster per batch entry is enough up to this many bytes of x: 8 CTAs read 32 KB each in about
+// the time of the second launch that they save.
+constexpr int64_t kFusedBytes = 256 * 1024;
+
+struct Plan {
+  bool fused;
+  unsigned threads;
+};
+
+static Plan plan(Params& p, int vec, int size) {
   p.V = p.C / vec;
   p.vlanes = p.V < kThreads ? p.V : kThreads;
   p.rows = kThreads / p.vlanes;
-  int64_t chunks = ceil_div((int64_t)sm_count() * 4, p.B);
-  const int64_t most = ceil_div(p.P, (int64_t)p.rows * 8);
-  if (chunks > most) chunks = most;
-  if (chunks < 1) chunks = 1;
-  p.chunk = ceil_div(p.P, chunks);
-  p.chunks = (int)ceil_div(p.P, p.chunk);
+  const bool fused = p.P * p.C * size <= kFusedBytes;
+  int64_t clusters = fused ? 1 : most_clusters(p.B, p.P);
+  // at least 16 pixels per thread row, so that runs fill
+  const int64_t most = ceil_div(p.P, (int64_t)kCluster * p.rows * 16);
+  if (clusters > most) clusters = most;
+  p.clusters = (int)clusters;
+  p.chunks = kCluster * p.clusters;
+  p.chunk = ceil_div(p.P, p.chunks);
+  p.direct = p.G <= kDirectGroups;
+  return {fused, (unsigned)(ceil_div((int64_t)p.vlanes * p.rows, 32) * 32)};
 }
 
-template <typename T, int VEC, int GV>
-static int launch_stats(const Params& p, cudaStream_t st) {
-  constexpr int RUN = sizeof(T) == 2 ? 4 : 4;
-  const size_t smem = (size_t)p.rows * p.V * (VEC / GV) * sizeof(double2);
-  static bool set[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (smem > 48 * 1024 && dev >= 0 && dev < 64 && !set[dev]) {
-    if (cudaFuncSetAttribute(stats_kernel<T, VEC, GV, RUN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) !=
-        cudaSuccess)
-      return zib_check_launch("zib_group_norm");
-    set[dev] = true;
+// Launches with clusters of `cluster` CTAs (0: none); dependent: may start before the launch before
+// it has ended, and waits for it in the kernel.
+static int launch(void (*kernel)(Params), dim3 grid, unsigned threads, size_t smem, int cluster, bool dependent,
+                  const Params& p, cudaStream_t st, const char* what) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    ZIB_HOST_CHECK(e == cudaSuccess, ZIB_ERR_LAUNCH, "%s: cudaFuncSetAttribute failed: %s", what,
+                   cudaGetErrorString(e));
   }
-  stats_kernel<T, VEC, GV, RUN><<<dim3(p.chunks, (unsigned)p.B), kThreads, smem, st>>>(p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (dependent) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    zib_set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
+    return ZIB_ERR_LAUNCH;
+  }
   return ZIB_OK;
 }
 
-template <typename T, int VEC>
-static int forward_v(const Params& p, cudaStream_t st) {
-  int rc = ZIB_OK;
-  const int gv = gcd(p.cpg, VEC);
-  if (gv == 8) { if constexpr (VEC == 8) rc = launch_stats<T, VEC, 8>(p, st); }
-  else if (gv == 4) { if constexpr (VEC >= 4) rc = launch_stats<T, VEC, 4>(p, st); }
-  else if (gv == 2) { if constexpr (VEC >= 2) rc = launch_stats<T, VEC, 2>(p, st); }
-  else rc = launch_stats<T, VEC, 1>(p, st);
-  if (rc) return rc;
-  finish_stats_kernel<<<(unsigned)ceil_div(p.B * p.G, kThreads / 32), kThreads, 0, st>>>(p);
-  apply_kernel<T, VEC><<<dim3(p.chunks, (unsigned)p.B), kThreads, 0, st>>>(p);
-  return zib_check_launch("zib_group_norm");
+template <typename T, int VEC, int GV>
+static int forward_g(Params& p, cudaStream_t st) {
+  const char* what = "zib_group_norm";
+  const Plan pl = plan(p, VEC, sizeof(T));
+  const size_t sums = (size_t)p.rows * p.V * (VEC / GV);
+  size_t smem = ((p.cpg / GV * p.rows == 1 ? 0 : (size_t)p.G) + sums) * sizeof(double2);
+  const size_t stats = (size_t)p.G * (sizeof(double2) + 2 * sizeof(float));
+  if (smem < stats) smem = stats;
+  ZIB_HOST_CHECK(smem <= kMaxSmem, ZIB_ERR_TOO_LARGE, "%s: %d channels", what, p.C);
+  const dim3 grid(p.chunks, (unsigned)p.B);
+  if (pl.fused) return launch(stats_kernel<T, VEC, GV, true>, grid, pl.threads, smem, kCluster, false, p, st, what);
+  int rc = launch(stats_kernel<T, VEC, GV, false>, grid, pl.threads, smem, kCluster, false, p, st, what);
+  if (!rc && !p.direct)
+    rc = launch(finish_stats_kernel, dim3((unsigned)ceil_div(p.B * p.G, 8)), 256, 0, 0, true, p, st, what);
+  if (!rc) rc = launch(apply_kernel<T, VEC>, grid, pl.threads, 0, 0, true, p, st, what);
+  return rc;
 }
 
 template <typename T, int VEC>
-static int backward_v(const Params& p, cudaStream_t st) {
-  const size_t smem = (size_t)p.rows * p.vlanes * VEC * sizeof(float2);
-  grad_stats_kernel<T, VEC><<<dim3(p.chunks, (unsigned)p.B), kThreads, smem, st>>>(p);
-  finish_grad_kernel<<<(unsigned)p.G, kThreads, 0, st>>>(p);
-  if (p.out) grad_apply_kernel<T, VEC><<<dim3(p.chunks, (unsigned)p.B), kThreads, 0, st>>>(p);
-  return zib_check_launch("zib_group_norm_backward");
+static int forward_v(Params& p, cudaStream_t st) {
+  const int gv = gcd(p.cpg, VEC);
+  if constexpr (VEC == 8) if (gv == 8) return forward_g<T, VEC, 8>(p, st);
+  if constexpr (VEC >= 4) if (gv == 4) return forward_g<T, VEC, 4>(p, st);
+  if constexpr (VEC >= 2) if (gv == 2) return forward_g<T, VEC, 2>(p, st);
+  return forward_g<T, VEC, 1>(p, st);
+}
+
+template <typename T, int VEC>
+static int backward_v(Params& p, cudaStream_t st) {
+  const char* what = "zib_group_norm_backward";
+  const Plan pl = plan(p, VEC, 2 * sizeof(T));  // x and dy
+  size_t smem = ((size_t)p.C + (size_t)p.rows * p.vlanes * VEC) * sizeof(float2);
+  const size_t sums = ((size_t)2 * p.C + p.G) * sizeof(float2);
+  if (smem < sums) smem = sums;
+  const dim3 grid(p.chunks, (unsigned)p.B);
+  const bool params = p.dw || p.db;
+  int rc;
+  if (pl.fused || !p.out) {
+    rc = launch(pl.fused ? grad_stats_kernel<T, VEC, true> : grad_stats_kernel<T, VEC, false>, grid, pl.threads, smem,
+                kCluster, false, p, st, what);
+    if (!rc && params)
+      rc = launch(param_grad_kernel, dim3((unsigned)ceil_div(p.C, 8)), 256, 0, 0, true, p, st, what);
+    return rc;
+  }
+  rc = launch(grad_stats_kernel<T, VEC, false>, grid, pl.threads, smem, kCluster, false, p, st, what);
+  if (!rc && !p.direct)
+    rc = launch(finish_grad_kernel, dim3((unsigned)ceil_div(p.B * p.G, 8)), 256, 0, 0, true, p, st, what);
+  const unsigned extra = params ? (unsigned)ceil_div(p.C, (int64_t)pl.threads / 32) : 0;
+  if (!rc)
+    rc = launch(grad_apply_kernel<T, VEC>, dim3(p.chunks + extra, (unsigned)p.B), pl.threads, 0, 0, true, p, st, what);
+  return rc;
 }
 
 static int check(const Params& p, int64_t C, int64_t G, int dtype, const char* what) {
@@ -431,13 +824,31 @@ static int check(const Params& p, int64_t C, int64_t G, int dtype, const char* w
   return ZIB_OK;
 }
 
-// whole 16-byte accesses where channels, strides and addresses allow them, else single elements
-static bool vector_ok(const Params& p, int size) {
-  const int v = 16 / size;
-  auto ok = [&](const void* x, int64_t sb, int64_t sp) {
-    return !x || ((uintptr_t)x % 16 == 0 && (sb % v == 0 || p.B == 1) && (sp % v == 0 || p.P == 1));
+// elements per access: as many as divide the channels, the strides and the addresses
+static int vector_width(const Params& p, int size) {
+  auto ok = [&](const void* x, int64_t sb, int64_t sp, int v) {
+    return !x || ((uintptr_t)x % (v * size) == 0 && (sb % v == 0 || p.B == 1) && (sp % v == 0 || p.P == 1));
   };
-  return p.C % v == 0 && ok(p.x, p.xsb, p.xsp) && ok(p.dy, p.dsb, p.dsp) && ok(p.out, 0, 0);
+  int v = 16 / size;
+  while (v > 1 && !(p.C % v == 0 && ok(p.x, p.xsb, p.xsp, v) && ok(p.dy, p.dsb, p.dsp, v) && ok(p.out, 0, 0, v)))
+    v >>= 1;
+  return v;
+}
+
+template <typename T>
+static int forward(Params& p, int v, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) if (v == 8) return forward_v<T, 8>(p, st);
+  if (v == 4) return forward_v<T, 4>(p, st);
+  if (v == 2) return forward_v<T, 2>(p, st);
+  return forward_v<T, 1>(p, st);
+}
+
+// four channels per access at most: two inputs, four constants and two sums per channel are registers
+template <typename T>
+static int backward(Params& p, int v, cudaStream_t st) {
+  if (v >= 4) return backward_v<T, 4>(p, st);
+  if (v == 2) return backward_v<T, 2>(p, st);
+  return backward_v<T, 1>(p, st);
 }
 
 }  // namespace gn
@@ -445,18 +856,11 @@ static bool vector_ok(const Params& p, int size) {
 
 using namespace zib;
 
-// chunks a launch may use at most, whatever vector width it takes
-static int64_t most_chunks(int64_t B, int64_t P) {
-  if (B < 1 || P < 1) return 1;
-  const int64_t c = ceil_div((int64_t)sm_count() * 4, B), m = ceil_div(P, 8);
-  return c < m ? c : m;
-}
-
 extern "C" int64_t zib_group_norm_workspace(int64_t B, int64_t P, int64_t C, int64_t G, int backward) {
   if (B < 0 || P < 0 || C < 1 || G < 1) return 0;
-  const int64_t n = B * most_chunks(B, P);
-  return backward ? n * C * (int64_t)sizeof(float2) + B * G * (int64_t)sizeof(float2)
-                  : n * G * (int64_t)sizeof(double2);
+  const int64_t n = B * gn::most_clusters(B, P);
+  const int64_t groups = n * G * (int64_t)sizeof(double2);
+  return backward ? groups + (n * C + B * G) * (int64_t)sizeof(float2) : groups;
 }
 
 extern "C" int zib_group_norm(const void* x, int64_t xsb, int64_t xsp, void* y, const void* w, const void* b,
@@ -466,9 +870,9 @@ extern "C" int zib_group_norm(const void* x, int64_t xsb, int64_t xsp, void* y, 
   const char* what = "zib_group_norm";
   gn::Params p{};
   p.x = x; p.xsb = xsb; p.xsp = xsp; p.out = y; p.w = w; p.b = b; p.wdtype = wdtype;
-  p.mean = mean; p.rstd = rstd; p.part = (double2*)workspace;
+  p.mean = mean; p.rstd = rstd; p.gpart = (double2*)workspace;
   p.B = B; p.P = P; p.act = act; p.eps = eps;
-  int rc = gn::check(p, C, G, dtype, what);
+  const int rc = gn::check(p, C, G, dtype, what);
   if (rc) return rc;
   if (B == 0 || P == 0) return ZIB_OK;
   ZIB_HOST_CHECK(x && y && mean && rstd && workspace, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
@@ -477,12 +881,10 @@ extern "C" int zib_group_norm(const void* x, int64_t xsb, int64_t xsp, void* y, 
                  (long long)zib_group_norm_workspace(B, P, C, G, 0));
   p.C = (int)C; p.G = (int)G; p.cpg = (int)(C / G);
   cudaStream_t st = (cudaStream_t)stream;
-  const bool vec = gn::vector_ok(p, dtype_bytes(dtype));
-  gn::plan(p, vec ? 16 / dtype_bytes(dtype) : 1);
-  if (dtype == ZIB_BF16)
-    return vec ? gn::forward_v<__nv_bfloat16, 8>(p, st) : gn::forward_v<__nv_bfloat16, 1>(p, st);
-  if (dtype == ZIB_F16) return vec ? gn::forward_v<__half, 8>(p, st) : gn::forward_v<__half, 1>(p, st);
-  return vec ? gn::forward_v<float, 4>(p, st) : gn::forward_v<float, 1>(p, st);
+  const int v = gn::vector_width(p, dtype_bytes(dtype));
+  if (dtype == ZIB_BF16) return gn::forward<__nv_bfloat16>(p, v, st);
+  if (dtype == ZIB_F16) return gn::forward<__half>(p, v, st);
+  return gn::forward<float>(p, v, st);
 }
 
 extern "C" int zib_group_norm_backward(const void* x, int64_t xsb, int64_t xsp, const void* dy, int64_t dsb,
@@ -496,21 +898,22 @@ extern "C" int zib_group_norm_backward(const void* x, int64_t xsb, int64_t xsp, 
   p.w = w; p.b = b; p.wdtype = wdtype; p.dw = dw; p.db = db;
   p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
   p.B = B; p.P = P; p.act = act;
-  int rc = gn::check(p, C, G, dtype, what);
+  const int rc = gn::check(p, C, G, dtype, what);
   if (rc) return rc;
   ZIB_HOST_CHECK(B > 0 && P > 0, ZIB_ERR_INVALID_ARG, "%s: empty input", what);
   ZIB_HOST_CHECK(x && dy && mean && rstd && workspace, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
   ZIB_HOST_CHECK(workspace_bytes >= zib_group_norm_workspace(B, P, C, G, 1) && (uintptr_t)workspace % 16 == 0,
                  ZIB_ERR_INVALID_ARG, "%s: workspace of %lld bytes, 16-byte aligned, needed", what,
                  (long long)zib_group_norm_workspace(B, P, C, G, 1));
+  if (!dx && !dw && !db) return ZIB_OK;
   p.C = (int)C; p.G = (int)G; p.cpg = (int)(C / G);
-  p.part = (double2*)workspace;
-  p.coef = dx ? (float2*)((char*)workspace + B * most_chunks(B, P) * C * sizeof(float2)) : nullptr;
+  const int64_t n = B * gn::most_clusters(B, P);
+  p.gpart = (double2*)workspace;
+  p.cpart = (float2*)(p.gpart + n * G);
+  p.coef = p.cpart + n * C;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool vec = gn::vector_ok(p, dtype_bytes(dtype));
-  gn::plan(p, vec ? 16 / dtype_bytes(dtype) : 1);
-  if (dtype == ZIB_BF16)
-    return vec ? gn::backward_v<__nv_bfloat16, 8>(p, st) : gn::backward_v<__nv_bfloat16, 1>(p, st);
-  if (dtype == ZIB_F16) return vec ? gn::backward_v<__half, 8>(p, st) : gn::backward_v<__half, 1>(p, st);
-  return vec ? gn::backward_v<float, 4>(p, st) : gn::backward_v<float, 1>(p, st);
+  const int v = gn::vector_width(p, dtype_bytes(dtype));
+  if (dtype == ZIB_BF16) return gn::backward<__nv_bfloat16>(p, v, st);
+  if (dtype == ZIB_F16) return gn::backward<__half>(p, v, st);
+  return gn::backward<float>(p, v, st);
 }

@@ -7,10 +7,13 @@
 // so the gradient is the same kernel with sin negated.
 //
 // Bound by memory: each element is read and written once (4 bytes in 16-bit types) against three
-// fp32 operations.  A thread keeps one unit of a head (VEC pairs in the half layout, VEC features
-// in the interleaved one) and walks over the heads of its token, queries and keys alike, so the
-// cos and sin of a unit are read once per token, not once per head: at 30 + 30 heads the fp32
-// table would otherwise be as many bytes as the data.
+// fp32 operations.  A thread keeps one unit of a head (two vectors of VEC features: the halves of
+// VEC pairs in the half layout, neighbours where features pass through; one vector in the interleaved
+// layout) and walks over heads of its token, queries and keys in one count, so the cos and sin of a
+// unit are read once for a few heads: the fp32 table would otherwise be as many bytes as the data.
+// A thread's chain is long (position, table row, data), so what hides it is many threads: more loads
+// per thread at the price of registers (four heads in flight, 25 to 37% occupancy) measured slower,
+// 97 instead of TBD us for [2, 4608, 30 + 30, 128].
 #include "zib_async.cuh"
 #include "zib_types.cuh"
 
@@ -35,94 +38,105 @@ struct Params {
   int pos64;           // 1: int64 positions, 0: int32
   int64_t ps_b, ps_s;
   int64_t L;           // table rows
-  int64_t S, tokens;   // tokens = B * S
+  int64_t S;
   int D, R;
   int units;           // units per head: rotated ones, then pass-through ones
   int rot_units;
-  int head_lanes, token_lanes;
+  int table_vec;       // the tables' rows allow 16-byte (or a unit's) accesses
   float sign;
 };
 
-// Loads unit u of one head, rotates, stores.
-template <typename T, int VEC, bool HALF>
-__device__ __forceinline__ void turn(const T* __restrict__ x, T* __restrict__ o, int at, int half, const float* c,
-                                     const float* s) {
-  using V = Pack<T, VEC>;
-  if constexpr (HALF) {
-    const V a = *reinterpret_cast<const V*>(x + at), b = *reinterpret_cast<const V*>(x + at + half);
-    V ra, rb;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float fa = to_f32(a.v[i]), fb = to_f32(b.v[i]);
-      ra.v[i] = from_f32<T>(fmaf(fa, c[i], -(fb * s[i])));
-      rb.v[i] = from_f32<T>(fmaf(fb, c[i], fa * s[i]));
-    }
-    *reinterpret_cast<V*>(o + at) = ra;
-    *reinterpret_cast<V*>(o + at + half) = rb;
-  } else {
-    const V a = *reinterpret_cast<const V*>(x + at);
-    V r;
-#pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) {
-      const float fa = to_f32(a.v[2 * i]), fb = to_f32(a.v[2 * i + 1]);
-      r.v[2 * i] = from_f32<T>(fmaf(fa, c[i], -(fb * s[i])));
-      r.v[2 * i + 1] = from_f32<T>(fmaf(fb, c[i], fa * s[i]));
-    }
-    *reinterpret_cast<V*>(o + at) = r;
-  }
-}
-
 // VEC: elements per access.  The interleaved layout turns VEC / 2 pairs per unit, the half layout VEC.
+// threadIdx: (unit, head lane, token lane); blockIdx: (tokens of a batch entry, batch entry).
 template <typename T, int VEC, bool HALF>
-__global__ void __launch_bounds__(1024) rotary_kernel(const Params p) {
+__global__ void __launch_bounds__(512, 3) rotary_kernel(const Params p) {
   using V = Pack<T, VEC>;
   constexpr int NP = HALF ? VEC : VEC / 2;  // pairs per unit
-  const int tid = threadIdx.x;
-  const int u = tid % p.units;
-  const int hl = (tid / p.units) % p.head_lanes;
-  const int64_t token = (int64_t)blockIdx.x * p.token_lanes + tid / (p.units * p.head_lanes);
-  if (token >= p.tokens) return;
-  const int64_t b = token / p.S, s = token - b * p.S;
+  const int u = threadIdx.x;
+  const int64_t s = (int64_t)blockIdx.x * blockDim.z + threadIdx.z, b = blockIdx.y;
+  if (s >= p.S) return;
   const bool rot = u < p.rot_units;
+  int64_t l = s;
+  if (p.pos && rot) {
+    const int64_t i = b * p.ps_b + s * p.ps_s;
+    l = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[i] : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[i];
+  }
+  // the unit's first vector, the distance to its second one, and whether it has that
+  const int at = rot ? u * VEC : p.R + (u - p.rot_units) * VEC;
+  const int second = rot ? p.R >> 1 : (p.units - p.rot_units) * VEC;
+  const bool two = HALF && at + second < p.D;
+  const T* xq = reinterpret_cast<const T*>(p.q.x) + b * p.q.sb + s * p.q.ss + at;
+  const T* xk = reinterpret_cast<const T*>(p.k.x) + b * p.k.sb + s * p.k.ss + at;
+  T* oq = reinterpret_cast<T*>(p.q.out) + (b * p.S + s) * p.q.H * p.D + at;
+  T* ok = reinterpret_cast<T*>(p.k.out) + (b * p.S + s) * p.k.H * p.D + at;
   float c[NP], sn[NP];
   if (rot) {
-    int64_t l = s;
-    if (p.pos) {
-      const int64_t i = b * p.ps_b + s * p.ps_s;
-      l = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[i] : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[i];
-    }
     if (l < 0 || l >= p.L) {
       // a position outside the table: the rotated features read NaN and the host learns of it
       atomicExch(&g_zib_err_word, (int)ZIB_ERR_INVALID_ARG);
 #pragma unroll
       for (int i = 0; i < NP; ++i) c[i] = sn[i] = __uint_as_float(0x7FC00000u);
     } else {
+      constexpr int FN = NP >= 4 ? 4 : NP;
+      using F = Pack<float, FN>;
       const float* cp = p.cos + b * p.cs_b + l * p.cs_l + u * NP;
       const float* sp = p.sin + b * p.cs_b + l * p.cs_l + u * NP;
+      if (p.table_vec) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        c[i] = __ldg(cp + i);
-        sn[i] = p.sign * __ldg(sp + i);
+        for (int i = 0; i < NP; i += FN) {
+          const F fc = *reinterpret_cast<const F*>(cp + i), fs = *reinterpret_cast<const F*>(sp + i);
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            c[i + j] = fc.v[j];
+            sn[i + j] = fs.v[j];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          c[i] = cp[i];
+          sn[i] = sp[i];
+        }
       }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) sn[i] *= p.sign;
     }
   }
-  const int at = rot ? u * VEC : p.R + (u - p.rot_units) * VEC;
-  const int half = p.R >> 1;
-#pragma unroll 1
-  for (int t = 0; t < 2; ++t) {
-    const Heads& hd = t ? p.k : p.q;
-    const T* x = reinterpret_cast<const T*>(hd.x) + b * hd.sb + s * hd.ss;
-    T* o = reinterpret_cast<T*>(hd.out) + token * hd.H * p.D;
-#pragma unroll 2
-    for (int h = hl; h < hd.H; h += p.head_lanes) {
-      if (rot) turn<T, VEC, HALF>(x + h * hd.sh, o + (int64_t)h * p.D, at, half, c, sn);
-      else *reinterpret_cast<V*>(o + (int64_t)h * p.D + at) = *reinterpret_cast<const V*>(x + h * hd.sh + at);
+  const int heads = p.q.H + p.k.H;
+  constexpr int U = HALF ? 1 : 2;  // heads in flight
+  for (int h0 = threadIdx.y; h0 < heads; h0 += U * blockDim.y) {
+    V a[U], d[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int h = h0 + i * blockDim.y;
+      if (h >= heads) break;
+      const T* x = h < p.q.H ? xq + h * p.q.sh : xk + (h - p.q.H) * p.k.sh;
+      a[i] = *reinterpret_cast<const V*>(x);
+      if constexpr (HALF) if (two) d[i] = *reinterpret_cast<const V*>(x + second);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int h = h0 + i * blockDim.y;
+      if (h >= heads) break;
+      T* o = h < p.q.H ? oq + (int64_t)h * p.D : ok + (int64_t)(h - p.q.H) * p.D;
+      if (rot) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          T& ta = HALF ? a[i].v[j] : a[i].v[2 * j];
+          T& tb = HALF ? d[i].v[j] : a[i].v[2 * j + 1];
+          const float fa = to_f32(ta), fb = to_f32(tb);
+          ta = from_f32<T>(fmaf(fa, c[j], -(fb * sn[j])));
+          tb = from_f32<T>(fmaf(fb, c[j], fa * sn[j]));
+        }
+      }
+      *reinterpret_cast<V*>(o) = a[i];
+      if constexpr (HALF) if (two) *reinterpret_cast<V*>(o + second) = d[i];
     }
   }
 }
 
 template <typename T, bool HALF>
-static void launch(int vec, unsigned grid, int threads, const Params& p, cudaStream_t st) {
+static void launch(int vec, dim3 grid, dim3 threads, const Params& p, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
     if (vec == 8) { rotary_kernel<T, 8, HALF><<<grid, threads, 0, st>>>(p); return; }
   }
@@ -146,11 +160,14 @@ struct TableParams {
   float* sin;
 };
 
-// cos and sin of p f_j, f_j = theta^(-2j/dim) scaled.  The angle is formed in turns in fp64 (a far
-// position times a frequency needs more than 24 bits), its whole turns are dropped there, and the
-// rest is split into an fp32 value and a correction d for the first-order step
-// cos(x + d) = cos x - d sin x, so each entry is within about 2 ulp.  A thread keeps one frequency
-// and walks over positions, so the fp64 exp is paid once per thread.
+// cos and sin of p f_j, f_j = theta^(-2j/dim) scaled.  The angle is formed in turns, in fixed point of
+// 64 bits: a whole position times a frequency, modulo whole turns, is one wrapping 64-bit product (the
+// frequency is rounded to 2^-64 turns, so a position below 2^31 is off by less than 2^-33 turns; the
+// fp64 frequency behind it by less than 2^-55 turns a position).  The upper 32 bits of the signed rest
+// split into an fp32 value and a correction d for the first-order step cos(x + d) = cos x - d sin x,
+// so each entry is within about 2 ulp.  A thread keeps one frequency and walks over positions, so the
+// fp64 exp is paid once per thread.  Forming the angle in fp64 instead, with its conversions, measured
+// 28 us at 131072 x 64.
 __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) {
   const int j = blockIdx.y * blockDim.x + threadIdx.x;
   if (j >= p.half) return;
@@ -162,19 +179,22 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) 
     const double keep = fmin(1.0, fmax(0.0, (turns - p.beta_slow) / (p.beta_fast - p.beta_slow)));
     f = (1.0 - keep) * f * p.inv_factor + keep * f;
   }
-  const double ft = f * 0.15915494309189535;  // turns per position
+  double ft = f * 0.15915494309189535;  // turns per position; whole ones do not matter
+  ft -= floor(ft);
+  const uint64_t step_turns = (uint64_t)(ft * 18446744073709551616.0);
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
+#pragma unroll 4
   for (int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; t < p.T; t += step) {
     int64_t pos = p.start + t;
     if (p.pos)
       pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[t * p.ps]
                     : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[t * p.ps];
-    const double a = (double)pos * ft;
-    const double r = 2.0 * (a - rint(a));  // angle / pi, in [-1, 1]
-    const float hi = (float)r;
-    const float d = (float)((r - (double)hi) * 3.141592653589793);
+    const int32_t a = (int32_t)(((uint64_t)pos * step_turns) >> 32);  // 2^-32 turns, in [-1/2, 1/2)
+    const float hi = (float)a;
+    // the rest of a below hi; a + 128 may round up to 2^31, which a float holds and an int does not
+    const float d = (float)(int32_t)((uint32_t)a - (uint32_t)(int64_t)hi) * 1.4629180792671596e-09f;  // 2 pi / 2^32
     float s, c;
-    sincospif(hi, &s, &c);
+    sincospif(hi * 4.656612873077393e-10f, &s, &c);  // 2 / 2^32: angle / pi
     p.cos[t * p.half + j] = p.mscale * fmaf(-d, s, c);
     p.sin[t * p.half + j] = p.mscale * fmaf(d, c, s);
   }
@@ -223,21 +243,30 @@ extern "C" int zib_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_s
   p.k = {k, k_out, k_sb, k_ss, k_sh, (int)Hk};
   p.cos = cos; p.sin = sin; p.cs_b = cs_b; p.cs_l = cs_l; p.L = L;
   p.pos = positions; p.pos64 = pos64; p.ps_b = ps_b; p.ps_s = ps_s;
-  p.S = S; p.tokens = B * S; p.D = (int)D; p.R = (int)R;
+  p.S = S; p.D = (int)D; p.R = (int)R;
   p.rot_units = (int)(part / vec);
-  p.units = p.rot_units + (int)((D - R) / vec);
+  p.units = p.rot_units + (int)ceil_div(D - R, half_layout ? 2 * vec : vec);
   p.sign = inverse ? -1.0f : 1.0f;
-  const int most = (int)(Hq > Hk ? Hq : Hk);
-  p.head_lanes = 256 / p.units;
-  if (p.head_lanes < 1) p.head_lanes = 1;
-  if (p.head_lanes > most) p.head_lanes = most;
-  p.token_lanes = 256 / (p.units * p.head_lanes);
-  if (p.token_lanes < 1) p.token_lanes = 1;
-  const int threads = p.units * p.head_lanes * p.token_lanes;
-  const int64_t grid = ceil_div(p.tokens, p.token_lanes);
-  ZIB_HOST_CHECK(grid <= 0x7FFFFFFF, ZIB_ERR_TOO_LARGE, "%s: %lld tokens", what, (long long)p.tokens);
+  const int np = half_layout ? vec : vec / 2, fn = np >= 4 ? 4 : np;
+  p.table_vec = ((uintptr_t)cos % (4 * fn) == 0 && (uintptr_t)sin % (4 * fn) == 0 && cs_l % fn == 0 && cs_b % fn == 0);
+  // heads per thread: one where the tokens alone do not fill the SMs (latency), else up to four
+  const int64_t heads = Hq + Hk;
+  int64_t per = 1;
+  if (B * S >= 4 * sm_count()) {
+    per = (heads * p.units + 128) / 256;
+    if (per < 1) per = 1;
+    if (per > 4) per = 4;
+  }
+  int64_t lanes = ceil_div(heads, per);
+  if (lanes * p.units > 512) lanes = 512 / p.units;  // units <= 512: a unit has two features at least
+  int64_t tokens = 256 / (p.units * lanes);
+  if (tokens > S) tokens = S;
+  if (tokens > 64) tokens = 64;
+  if (tokens < 1) tokens = 1;
+  const dim3 threads(p.units, (unsigned)lanes, (unsigned)tokens), g((unsigned)ceil_div(S, tokens), (unsigned)B);
+  ZIB_HOST_CHECK(ceil_div(S, tokens) <= 0x7FFFFFFF && B <= 65535, ZIB_ERR_TOO_LARGE,
+                 "%s: at most 65535 batch entries, got %lld", what, (long long)B);
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned g = (unsigned)grid;
   if (dtype == ZIB_BF16) {
     if (half_layout) rotary::launch<__nv_bfloat16, true>(vec, g, threads, p, st);
     else rotary::launch<__nv_bfloat16, false>(vec, g, threads, p, st);
