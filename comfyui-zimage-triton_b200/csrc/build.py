@@ -20,7 +20,7 @@ PKG = CSRC.parent / "zimage_b200"
 INCLUDE = CSRC.parent.parent / "include"
 OUT = PKG / "libzimage_b200.so"
 SOURCES = ["zib_api.cu", "rowops.cu", "gemm_w8a8.cu", "rotary.cu", "group_norm.cu", "fp8_block.cu",
-           "fp8_gemm.cu"]
+           "fp8_gemm.cu", "fp8_linear.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden",
          "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills"]

@@ -1,78 +1,9 @@
-// Operands of matrix products in 8-bit floating point (e4m3) with one scale for each block of 128.
-//
-// Quantiser: a block of values (1 x 128 of an activation row, 128 x 128 of a weight) with largest
-// magnitude a is held as e4m3 values q = x / s, s = 2^e with the least e >= -120 such that
-// a <= 448 s.  A power of two makes the division exact, so q is the one rounding of x to e4m3's
-// 4-bit mantissa (ties to even) and any implementation gives the same bits; as the format floats,
-// scales between the powers would gain no precision but at the bottom of its range.  A block with
-// an infinity or a NaN gets NaN for its scale and its values.
-#include "zib_async.cuh"
-#include "zib_types.cuh"
-
-#include <cuda_fp8.h>
+// Operands of matrix products in 8-bit floating point (e4m3) with one scale for each block of 128:
+// quantisers, transposed weights, and the column sums of a bias gradient.
+#include "fp8_quant.cuh"
 
 namespace zib {
 namespace fp8 {
-
-constexpr int kBlock = 128;
-
-// e with s = 2^e for a block's largest magnitude (given as its fp32 bits: NaN > infinity > finite)
-__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
-  if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
-  // a = m 2^k with m in [1, 2); 448 = 1.75 * 2^8
-  int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  if (e < -120) e = -120;
-  return __uint_as_float((uint32_t)(e + 127) << 23);
-}
-// 1 / s, exact for a power of two
-__device__ __forceinline__ float inverse_scale(float s) {
-  const uint32_t b = __float_as_uint(s);
-  return b >= 0x7F800000u ? s : __uint_as_float((254u << 23) - b);
-}
-// 8 consecutive values from column k of a row of K (16-byte accesses where VEC), 0 past the end
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t k, int64_t K, float (&v)[8]) {
-  if constexpr (VEC) {  // K % 8 == 0: all eight or none
-    constexpr int E = 16 / sizeof(T);
-#pragma unroll
-    for (int h = 0; h < 8 / E; ++h) {
-      Pack<T, E> t{};
-      if (k < K) t = *reinterpret_cast<const Pack<T, E>*>(row + k + h * E);
-#pragma unroll
-      for (int j = 0; j < E; ++j) v[h * E + j] = to_f32(t.v[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_f32(row[k + j]) : 0.0f;
-  }
-}
-
-// The largest magnitude of 8 values, as its bits.
-__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
-  uint32_t a = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-  return a;
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t* __restrict__ row, int64_t k, int64_t K, const float (&v)[8],
-                                       float inv) {
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h] * inv, v[4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h + 2] * inv, v[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-    w[h] = lo | (hi << 16);
-  }
-  if constexpr (VEC) {
-    if (k < K) *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (k + j < K) row[k + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-  }
-}
 
 // Activation rows.  Bound by memory (3 bytes per 16-bit element): a warp takes 8 rows of two blocks,
 // 16 lanes x 8 values to a block, with all its loads in flight before the first is used; the 8 rows
@@ -104,6 +35,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const T* __restrict__ x
   }
   const int r = lane & 15;
   if (r < kRowsPerWarp && m0 + r < M && b * kBlock < K) s[(m0 + r) * s_m + b * s_k] = mine;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product may start and wait
 }
 
 // Weights: one CTA per block of 128 x 128, held in registers between its maximum and its values.
@@ -182,17 +114,10 @@ static bool whole_vectors(const void* x, int64_t ldx, int size, const void* q, i
 
 using namespace zib;
 
-extern "C" int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m,
-                                  int64_t s_k, int64_t M, int64_t K, void* stream) {
-  const char* what = "zib_fp8_quant_rows";
-  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
-  ZIB_HOST_CHECK(M >= 0 && K >= 1 && ldx >= K && ldq >= K, ZIB_ERR_INVALID_ARG, "%s: bad shape M=%lld K=%lld", what,
-                 (long long)M, (long long)K);
-  if (M == 0) return ZIB_OK;
-  ZIB_HOST_CHECK(x && q && s, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+int zib::fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m, int64_t s_k,
+                        int64_t M, int64_t K, cudaStream_t st, const char* what) {
   const int64_t grid = ceil_div(ceil_div(M, fp8::kRowsPerWarp) * ceil_div(K, 2 * fp8::kBlock), 8);
   ZIB_HOST_CHECK(grid <= 0x7FFFFFFF, ZIB_ERR_TOO_LARGE, "%s: M=%lld K=%lld", what, (long long)M, (long long)K);
-  cudaStream_t st = (cudaStream_t)stream;
   const bool vec = fp8::whole_vectors(x, ldx, dtype_bytes(dtype), q, ldq, M, K);
   auto go = [&](auto kernel, auto* xt) {
     kernel<<<(unsigned)grid, 256, 0, st>>>(xt, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
@@ -203,6 +128,17 @@ extern "C" int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q
   else if (dtype == ZIB_F16) go(vec ? fp8::quant_rows_kernel<H, true> : fp8::quant_rows_kernel<H, false>, (const H*)x);
   else go(vec ? fp8::quant_rows_kernel<float, true> : fp8::quant_rows_kernel<float, false>, (const float*)x);
   return zib_check_launch(what);
+}
+
+extern "C" int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m,
+                                  int64_t s_k, int64_t M, int64_t K, void* stream) {
+  const char* what = "zib_fp8_quant_rows";
+  ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
+  ZIB_HOST_CHECK(M >= 0 && K >= 1 && ldx >= K && ldq >= K, ZIB_ERR_INVALID_ARG, "%s: bad shape M=%lld K=%lld", what,
+                 (long long)M, (long long)K);
+  if (M == 0) return ZIB_OK;
+  ZIB_HOST_CHECK(x && q && s, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
+  return fp8_quant_rows(x, ldx, dtype, q, ldq, s, s_m, s_k, M, K, (cudaStream_t)stream, what);
 }
 
 extern "C" int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void* q, int64_t ldq, float* s, int64_t s_n,

@@ -25,9 +25,9 @@
 // 840 us, accumulators of 128 columns in two halves of the tile 895 us (the rows of q are read twice).
 // Every mbarrier wait is bounded; on expiry the CTA records ZIB_ERR_TIMEOUT in a device error word,
 // drains its loads and MMAs, frees TMEM and exits.
+#include "fp8_quant.cuh"
 #include "rot_pack.cuh"
 #include "zib_tcgen05.cuh"
-#include "zib_types.cuh"
 
 ZIB_DEFINE_ERROR_READER(zib_err_read_clear_fp8)
 
@@ -36,7 +36,6 @@ namespace fp8 {
 
 using namespace tc;
 
-constexpr int kBlock = 128;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (4 + kEpiWarps) * 32;
 constexpr int kTmemCols = 512;
@@ -498,6 +497,19 @@ static int gemm(const GemmParams& p, const void* q, int64_t ldq, const void* w, 
 
 using namespace zib;
 
+int zib::fp8_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k, const void* w, int64_t ldw,
+                  const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, int dtype,
+                  int64_t M, int64_t N, int64_t K, cudaStream_t st, const char* what) {
+  fp8::GemmParams p{};
+  p.M = (int)M; p.N = (int)N;
+  p.sx = sx; p.sx_m = sx_m; p.sx_k = sx_k;
+  p.sw = sw; p.sw_n = sw_n; p.sw_k = sw_k;
+  p.bias = bias; p.y = y; p.ldy = ldy;
+  if (dtype == ZIB_BF16) return fp8::gemm<__nv_bfloat16>(p, q, ldq, w, ldw, K, st, what);
+  if (dtype == ZIB_F16) return fp8::gemm<__half>(p, q, ldq, w, ldw, K, st, what);
+  return fp8::gemm<float>(p, q, ldq, w, ldw, K, st, what);
+}
+
 extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
                                   const void* w, int64_t ldw, const float* sw, int64_t sw_n, int64_t sw_k,
                                   const void* bias, void* y, int64_t ldy, int dtype, int64_t M, int64_t N, int64_t K,
@@ -512,13 +524,6 @@ extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, i
                  ZIB_ERR_ALIGNMENT, "%s: q and w need 16-byte aligned rows", what);
   if (M == 0) return ZIB_OK;
   ZIB_HOST_CHECK(q && sx && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
-  fp8::GemmParams p{};
-  p.M = (int)M; p.N = (int)N;
-  p.sx = sx; p.sx_m = sx_m; p.sx_k = sx_k;
-  p.sw = sw; p.sw_n = sw_n; p.sw_k = sw_k;
-  p.bias = bias; p.y = y; p.ldy = ldy;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == ZIB_BF16) return fp8::gemm<__nv_bfloat16>(p, q, ldq, w, ldw, K, st, what);
-  if (dtype == ZIB_F16) return fp8::gemm<__half>(p, q, ldq, w, ldw, K, st, what);
-  return fp8::gemm<float>(p, q, ldq, w, ldw, K, st, what);
+  return fp8_gemm(q, ldq, sx, sx_m, sx_k, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, (cudaStream_t)stream,
+                  what);
 }

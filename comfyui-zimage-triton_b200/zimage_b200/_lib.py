@@ -71,6 +71,9 @@ SIGNATURES: dict[str, list] = {
     "zib_fp8_quant_blocks": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP],
     "zib_fp8_block_gemm": [_VP, _I64, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _I32, _I64,
                            _I64, _I64, _VP],
+    "zib_fp8_block_linear_scratch": [_I64, _I64],
+    "zib_fp8_block_linear": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _I64, _I64, _I64,
+                             _I64, _VP],
     "zib_fp8_transpose": [_VP, _I64, _VP, _I64, _I64, _I64, _VP],
     "zib_col_sum": [_VP, _I64, _I32, _VP, _VP, _I64, _I64, _I64, _VP],
     "zib_rotary": [_VP, _I64, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _VP, _I64, _I32, _VP, _VP, _I64,
@@ -84,7 +87,7 @@ SIGNATURES: dict[str, list] = {
                                 _I64, _I64, _I64, _I64, _I64, _I32, _I32, _VP],
 }
 _RESTYPES = {"zib_status_string": ctypes.c_char_p, "zib_last_error": ctypes.c_char_p,
-             "zib_group_norm_workspace": ctypes.c_int64}
+             "zib_group_norm_workspace": ctypes.c_int64, "zib_fp8_block_linear_scratch": ctypes.c_int64}
 
 # zib_dtype codes of the entry points that take several element types
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -179,14 +182,36 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
-def call_on(t: torch.Tensor, name: str, *args) -> None:
-    """``call`` on the device of ``t``, whichever device is current; the stream is appended."""
-    dev = t.get_device()
-    if dev == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-        return
-    with torch.cuda.device(dev):
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+_FN: dict[str, object] = {}  # entry points by name, bound once
+
+
+def call_on(dev: int, name: str, *args) -> None:
+    """``call`` on CUDA device ``dev``, whichever device is current; its current stream is appended.
+
+    The path of the operators that a latency-bound loop calls: the entry point is bound once and the
+    stream handle read without a Stream object (2 us each through ``torch.cuda.current_stream``).
+    """
+    global LAUNCHES
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(load(), name)
+    LAUNCHES += 1
+    if dev == _current_device():
+        status = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _raw_stream(dev))
+    if status != ZIB_OK:
+        check(status, name)
+
+
+def _raw_stream(dev: int) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+_current_device = torch.cuda.current_device
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle, without the object around it
+    _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def dtype_code(t: torch.Tensor, what: str) -> int:
@@ -197,11 +222,12 @@ def dtype_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def same_device(t: torch.Tensor, **others: torch.Tensor | None) -> None:
+def same_device(t: torch.Tensor, *others: torch.Tensor | None) -> None:
     """ValueError unless every given tensor lies on the device of ``t``."""
-    for name, o in others.items():
-        if o is not None and o.device != t.device:
-            raise ValueError(f"{name} is on {o.device}, expected {t.device}")
+    dev = t.device
+    for o in others:
+        if o is not None and o.device != dev:
+            raise ValueError(f"an operand is on {o.device}, expected {dev}")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import functools
+import math
+
 import torch
 
 from .. import _lib
@@ -10,62 +13,79 @@ ACTIVATIONS = {"none": 0, "silu": 1}
 MAX_CHANNELS = 8192
 
 
-def _rows(x: torch.Tensor, B: int, P: int, C: int) -> torch.Tensor:
-    """x as [B, P, C] with contiguous channels, a view where its strides allow one."""
-    x3 = x.reshape(B, P, C)
-    return x3 if x3.stride(2) == 1 or C == 1 else x3.contiguous()
+@functools.lru_cache(maxsize=4096)
+def _workspace(dev: int, B: int, P: int, C: int, G: int, backward: int) -> int:
+    """Bytes of workspace on device ``dev`` (a function of the sizes alone), whole 16-byte pieces."""
+    with torch.cuda.device(dev):
+        return -(-_lib.load().zib_group_norm_workspace(B, P, C, G, backward) // 16) * 16
 
 
-def _forward(x3, groups, weight, bias, eps, act):
-    B, P, C = x3.shape
-    y = torch.empty(B, P, C, dtype=x3.dtype, device=x3.device)
-    stats = torch.empty(2, B, groups, dtype=torch.float32, device=x3.device)
+def _strides(x: torch.Tensor, P: int, C: int) -> tuple[torch.Tensor, int, int]:
+    """x [B, ..., C] with its batch and position strides; a contiguous copy where it has no single one."""
+    if x.is_contiguous():
+        return x, P * C, C
+    if x.dim() != 3:
+        try:
+            x = x.view(x.shape[0], P, C)
+        except RuntimeError:
+            x = x.contiguous()
+            return x, P * C, C
+    if x.stride(2) != 1 and C != 1:
+        x = x.contiguous()
+        return x, P * C, C
+    return x, x.stride(0), x.stride(1)
+
+
+def _forward(x, weight, bias, G, eps, act, P):
+    """(y, buffer): y like x; the buffer starts with mean and 1/std, fp32 [B, G] each."""
+    B, C = x.shape[0], x.shape[-1]
+    dev = x.get_device()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = -(-8 * B * G // 16) * 16
+    n = _workspace(dev, B, P, C, G, 0)
+    buf = torch.empty(stats + n + 16, dtype=torch.uint8, device=x.device)
+    at = buf.data_ptr()
+    xs, sb, sp = _strides(x, P, C)
     wd = weight if weight is not None else bias
-    ws = torch.empty(max(16, _workspace(x3, B, P, C, groups, 0)), dtype=torch.uint8, device=x3.device)
-    _lib.call_on(x3, "zib_group_norm", x3.data_ptr(), x3.stride(0), x3.stride(1), y.data_ptr(), _lib.ptr(weight),
-                 _lib.ptr(bias), 0 if wd is None else _lib.DTYPES[wd.dtype], stats[0].data_ptr(),
-                 stats[1].data_ptr(), ws.data_ptr(), ws.numel(), B, P, C, groups, _lib.DTYPES[x3.dtype], eps, act)
-    return y, stats
-
-
-def _workspace(t, B, P, C, G, backward) -> int:
-    lib = _lib.load()
-    if t.get_device() == torch.cuda.current_device():
-        return lib.zib_group_norm_workspace(B, P, C, G, backward)
-    with torch.cuda.device(t.get_device()):
-        return lib.zib_group_norm_workspace(B, P, C, G, backward)
+    _lib.call_on(dev, "zib_group_norm", xs.data_ptr(), sb, sp, y.data_ptr(),
+                 None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                 0 if wd is None else _lib.DTYPES[wd.dtype], at, at + 4 * B * G, at + stats, n, B, P, C, G,
+                 _lib.DTYPES[x.dtype], eps, act)
+    return y, buf
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x3, weight, bias, groups, eps, act):
-        y, stats = _forward(x3, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x3, weight, bias, stats)
-        ctx.groups, ctx.act = groups, act
+    def forward(ctx, x, weight, bias, G, eps, act, P):
+        y, buf = _forward(x, weight, bias, G, eps, act, P)
+        ctx.save_for_backward(x, weight, bias, buf)
+        ctx.conf = G, act, P
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x3, weight, bias, stats = ctx.saved_tensors
-        B, P, C = x3.shape
-        G = ctx.groups
+        x, weight, bias, buf = ctx.saved_tensors
+        G, act, P = ctx.conf
+        B, C = x.shape[0], x.shape[-1]
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        if x3.numel() == 0:
-            return (torch.empty_like(x3) if want_x else None, torch.zeros_like(weight) if want_w else None,
-                    torch.zeros_like(bias) if want_b else None, None, None, None)
-        if dy.stride(2) != 1 and C != 1:
-            dy = dy.contiguous()
-        dx = torch.empty(B, P, C, dtype=x3.dtype, device=x3.device) if want_x else None
+        if x.numel() == 0:
+            return (torch.empty_like(x) if want_x else None, torch.zeros_like(weight) if want_w else None,
+                    torch.zeros_like(bias) if want_b else None, None, None, None, None)
+        dev = x.get_device()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
         dw = torch.empty_like(weight) if want_w else None
         db = torch.empty_like(bias) if want_b else None
+        n = _workspace(dev, B, P, C, G, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        xs, xsb, xsp = _strides(x, P, C)
+        ds, dsb, dsp = _strides(dy, P, C)
         wd = weight if weight is not None else bias
-        ws = torch.empty(_workspace(x3, B, P, C, G, 1), dtype=torch.uint8, device=x3.device)
-        _lib.call_on(x3, "zib_group_norm_backward", x3.data_ptr(), x3.stride(0), x3.stride(1), dy.data_ptr(),
-                     dy.stride(0), dy.stride(1), _lib.ptr(dx), _lib.ptr(weight), _lib.ptr(bias),
-                     0 if wd is None else _lib.DTYPES[wd.dtype], _lib.ptr(dw), _lib.ptr(db), stats[0].data_ptr(),
-                     stats[1].data_ptr(), ws.data_ptr(), ws.numel(), B, P, C, G, _lib.DTYPES[x3.dtype], ctx.act)
-        return dx, dw, db, None, None, None
+        _lib.call_on(dev, "zib_group_norm_backward", xs.data_ptr(), xsb, xsp, ds.data_ptr(), dsb, dsp, _lib.ptr(dx),
+                     _lib.ptr(weight), _lib.ptr(bias), 0 if wd is None else _lib.DTYPES[wd.dtype], _lib.ptr(dw),
+                     _lib.ptr(db), buf.data_ptr(), buf.data_ptr() + 4 * B * G, ws.data_ptr(), n, B, P, C, G,
+                     _lib.DTYPES[x.dtype], act)
+        return dx, dw, db, None, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
@@ -82,37 +102,35 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
-    if x.dim() < 2:
-        raise ValueError(f"x must be [B, ..., C], got {tuple(x.shape)}")
-    B, C = x.shape[0], x.shape[-1]
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"x must be [B, ..., C], got {tuple(shape)}")
+    C = shape[-1]
     if num_groups < 1 or C < 1 or C % num_groups:
         raise ValueError(f"{C} channels do not split into {num_groups} groups")
     if C > MAX_CHANNELS:
         raise RuntimeError(f"group_norm_act takes at most {MAX_CHANNELS} channels, got {C}")
     _lib.dtype_code(x, "x")
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.shape != (C,):
-            raise ValueError(f"{name} must have shape ({C},), got {tuple(t.shape)}")
         if t is not None:
+            if t.shape != (C,):
+                raise ValueError(f"{name} must have shape ({C},), got {tuple(t.shape)}")
             _lib.dtype_code(t, name)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise ValueError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
     _lib.require_device(x)
-    _lib.same_device(x, weight=weight, bias=bias)
-    P = 1
-    for n in x.shape[1:-1]:
-        P *= n
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    x3 = _rows(x, B, P, C)
+    _lib.same_device(x, weight, bias)
+    P = math.prod(shape[1:-1])
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        y = _GroupNorm.apply(x3, weight, bias, num_groups, float(eps), act)
-    else:
-        y = _forward(x3, num_groups, weight, bias, float(eps), act)[0]
-    return y.view(x.shape)
+        return _GroupNorm.apply(x, weight, bias, num_groups, float(eps), act, P)
+    return _forward(x, weight, bias, num_groups, float(eps), act, P)[0]
 
 
 class GroupNormAct(torch.nn.Module):

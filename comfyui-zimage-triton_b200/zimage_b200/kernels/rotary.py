@@ -60,37 +60,32 @@ def rotary_table(positions: torch.Tensor | int, dim: int, theta: float = 10000.0
         T, dev, ptr, pos64, ps = int(positions), torch.device(device), None, 0, 0
         if T < 0:
             raise ValueError(f"positions must not be negative, got {T}")
-    out = torch.empty(2, T, dim // 2, dtype=torch.float32, device=dev)
-    _lib.require_device(out)
-    cos, sin = out[0], out[1]
-    _lib.call_on(out, "zib_rotary_table", ptr, pos64, ps, 0, T, dim, float(theta), SCALINGS[kind], factor, original,
+    cos = torch.empty(T, dim // 2, dtype=torch.float32, device=dev)
+    sin = torch.empty(T, dim // 2, dtype=torch.float32, device=dev)
+    _lib.call_on(_lib.require_device(cos), "zib_rotary_table", ptr, pos64, ps, 0, T, dim, float(theta), SCALINGS[kind], factor, original,
                  fast, slow, attn, cos.data_ptr(), sin.data_ptr())
     return cos, sin
-
-
-def _heads(x: torch.Tensor) -> torch.Tensor:
-    """x [B, S, H, D] with contiguous features and no overlapping elements to write through."""
-    return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
 
 
 def _rotate(q, k, cos, sin, positions, half: int, inverse: int):
     """One launch over q and k (either may be None): fresh contiguous outputs."""
     ref = q if q is not None else k
     B, S, _, D = ref.shape
-    args, outs = [], []
+    code, device = _lib.DTYPES[ref.dtype], ref.device
+    args, outs, keep = [], [], []
     for t in (q, k):
         if t is None:
-            args += [None, 0, 0, 0, None, 0]
+            args += (None, 0, 0, 0, None, 0)
             outs.append(None)
             continue
-        t = _heads(t)
-        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        sb, ss, sh, _ = t.stride()
-        if half == 0 and (t.data_ptr() % (2 * t.element_size()) or (sb | ss | sh) & 1):
-            t = t.contiguous()  # a pair is one access
-            sb, ss, sh, _ = t.stride()
-        args += [t.data_ptr(), sb, ss, sh, o.data_ptr(), t.shape[2]]
-        outs.append((o, t))
+        sb, ss, sh, sd = t.stride()
+        if (sd != 1 and D != 1) or (half == 0 and ((sb | ss | sh) & 1 or t.data_ptr() % (2 * t.element_size()))):
+            t = t.contiguous()  # features side by side; interleaved, a pair is one access
+            sb, ss, sh, sd = t.stride()
+            keep.append(t)
+        o = torch.empty(t.shape, dtype=t.dtype, device=device)
+        args += (t.data_ptr(), sb, ss, sh, o.data_ptr(), t.shape[2])
+        outs.append(o)
     if cos.dim() == 3:
         cs_b, cs_l, L = (0 if cos.shape[0] == 1 else cos.stride(0)), cos.stride(1), cos.shape[1]
     else:
@@ -98,10 +93,10 @@ def _rotate(q, k, cos, sin, positions, half: int, inverse: int):
     if positions is None:
         pos = (None, 0, 0, 0)
     else:
-        pos = (positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(0), positions.stride(1))
-    _lib.call_on(ref, "zib_rotary", *args, _lib.DTYPES[ref.dtype], cos.data_ptr(), sin.data_ptr(), cs_b, cs_l, L,
-                 *pos, B, S, D, 2 * cos.shape[-1], half, inverse)
-    return tuple(None if o is None else o[0] for o in outs)
+        pos = (positions.data_ptr(), int(positions.dtype is torch.int64), *positions.stride())
+    _lib.call_on(ref.get_device(), "zib_rotary", *args, code, cos.data_ptr(), sin.data_ptr(), cs_b, cs_l, L, *pos, B,
+                 S, D, 2 * cos.shape[-1], half, inverse)
+    return tuple(outs)
 
 
 class _Rotary(torch.autograd.Function):
@@ -136,42 +131,50 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin
     """
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
-    if q.dim() != 4:
-        raise ValueError(f"q must be [B, S, H, D], got {tuple(q.shape)}")
-    B, S, _, D = q.shape
-    if k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != D or k.dtype != q.dtype):
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-    if cos.shape != sin.shape or cos.dim() not in (2, 3) or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    half = int(layout == "half")
+    qs = q.shape
+    if len(qs) != 4:
+        raise ValueError(f"q must be [B, S, H, D], got {tuple(qs)}")
+    B, S, _, D = qs
+    dtype = q.dtype
+    if k is not None:
+        ks = k.shape
+        if len(ks) != 4 or ks[0] != B or ks[1] != S or ks[3] != D or k.dtype is not dtype:
+            raise ValueError(f"k {tuple(ks)} {k.dtype} does not go with q {tuple(qs)} {dtype}")
+    cs = cos.shape
+    if cs != sin.shape or len(cs) not in (2, 3) or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError(f"cos and sin must be fp32 tables of one shape, [L, R/2] or [B, L, R/2]; got "
-                         f"{tuple(cos.shape)} {cos.dtype} and {tuple(sin.shape)} {sin.dtype}")
-    if cos.dim() == 3 and cos.shape[0] not in (1, B):
-        raise ValueError(f"a table of {cos.shape[0]} batch entries does not go with a batch of {B}")
-    if not 1 <= cos.shape[-1] <= D // 2:
-        raise ValueError(f"tables of {cos.shape[-1]} pairs do not go with heads of {D} features")
+                         f"{tuple(cs)} {cos.dtype} and {tuple(sin.shape)} {sin.dtype}")
+    if len(cs) == 3 and cs[0] not in (1, B):
+        raise ValueError(f"a table of {cs[0]} batch entries does not go with a batch of {B}")
+    if not 1 <= cs[-1] <= D // 2:
+        raise ValueError(f"tables of {cs[-1]} pairs do not go with heads of {D} features")
     if positions is None:
-        if cos.shape[-2] < S:
-            raise ValueError(f"a table of {cos.shape[-2]} rows is too short for {S} tokens")
+        if cs[-2] < S:
+            raise ValueError(f"a table of {cs[-2]} rows is too short for {S} tokens")
     else:
         if positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        try:
-            positions = positions.expand(B, S)
-        except RuntimeError:
-            raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to {(B, S)}") from None
-        if cos.shape[-2] < 1:
+        ps = positions.shape
+        if len(ps) != 2 or ps[0] != B or ps[1] != S:
+            try:
+                positions = positions.expand(B, S)
+            except RuntimeError:
+                raise ValueError(f"positions {tuple(ps)} do not broadcast to {(B, S)}") from None
+        if cs[-2] < 1:
             raise ValueError("empty table")
     _lib.dtype_code(q, "q")
-    if layout == "interleaved" and D % 2:
+    if not half and D % 2:
         raise ValueError(f"the interleaved layout needs an even head size, got {D}")
     if D > 1024:
         raise ValueError(f"heads of at most 1024 features, got {D}")
     _lib.require_device(q)
-    _lib.same_device(q, k=k, cos=cos, sin=sin, positions=positions)
-    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
-        raise ValueError("the tables of rotary_embed are constants: cos and sin must not require gradients")
+    _lib.same_device(q, k, cos, sin, positions)
     if cos.stride(-1) != 1 or cos.stride() != sin.stride():
         cos, sin = cos.contiguous(), sin.contiguous()
-    half = int(layout == "half")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, cos, sin, positions, half)
+    if torch.is_grad_enabled():
+        if cos.requires_grad or sin.requires_grad:
+            raise ValueError("the tables of rotary_embed are constants: cos and sin must not require gradients")
+        if q.requires_grad or (k is not None and k.requires_grad):
+            return _Rotary.apply(q, k, cos, sin, positions, half)
     return _rotate(q, k, cos, sin, positions, half, 0)

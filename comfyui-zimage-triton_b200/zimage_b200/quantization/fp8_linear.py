@@ -11,6 +11,8 @@ dx = quantised(dy) W, whose transposed weight has the same 128 x 128 blocks.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -55,18 +57,9 @@ def _quant_rows(x2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     M, K = x2.shape
     q = _empty_rows(M, K, x2.device)
     s = torch.empty(-(-K // BLOCK), M, dtype=torch.float32, device=x2.device)
-    _lib.call_on(x2, "zib_fp8_quant_rows", x2.data_ptr(), _ld(x2), _lib.DTYPES[x2.dtype], q.data_ptr(), _ld16(q),
-                 s.data_ptr(), 1, M, M, K)
+    _lib.call_on(x2.get_device(), "zib_fp8_quant_rows", x2.data_ptr(), _ld(x2), _lib.DTYPES[x2.dtype],
+                 q.data_ptr(), _ld16(q), s.data_ptr(), 1, M, M, K)
     return q, s
-
-
-def _gemm(q, sx, sx_m, sx_k, w, sw, sw_n, sw_k, bias, dtype) -> torch.Tensor:
-    M, K = q.shape
-    N = w.shape[0]
-    y = torch.empty(M, N, dtype=dtype, device=q.device)
-    _lib.call_on(q, "zib_fp8_block_gemm", q.data_ptr(), _ld16(q), sx.data_ptr(), sx_m, sx_k, w.data_ptr(), _ld16(w),
-                 sw.data_ptr(), sw_n, sw_k, _lib.ptr(bias), y.data_ptr(), N, _lib.DTYPES[dtype], M, N, K)
-    return y
 
 
 def fp8_block_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -99,8 +92,8 @@ def fp8_block_quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tens
     N, K = w.shape
     q = _empty_rows(N, K, w.device)
     s = torch.empty(-(-N // BLOCK), -(-K // BLOCK), dtype=torch.float32, device=w.device)
-    _lib.call_on(w, "zib_fp8_quant_blocks", w.data_ptr(), _ld(w), _lib.DTYPES[w.dtype], q.data_ptr(), _ld16(q),
-                 s.data_ptr(), s.stride(0), 1, N, K)
+    _lib.call_on(w.get_device(), "zib_fp8_quant_blocks", w.data_ptr(), _ld(w), _lib.DTYPES[w.dtype],
+                 q.data_ptr(), _ld16(q), s.data_ptr(), s.stride(0), 1, N, K)
     return q, s
 
 
@@ -113,19 +106,22 @@ def fp8_block_transpose(w_q: torch.Tensor) -> torch.Tensor:
         w_q = w_q.contiguous()
     N, K = w_q.shape
     t = _empty_rows(K, N, w_q.device)
-    _lib.call_on(w_q, "zib_fp8_transpose", w_q.data_ptr(), _ld(w_q), t.data_ptr(), _ld16(t), N, K)
+    _lib.call_on(w_q.get_device(), "zib_fp8_transpose", w_q.data_ptr(), _ld(w_q), t.data_ptr(), _ld16(t), N, K)
     return t
 
 
-def _check_weight(K: int, w_q, w_scale, bias, dtype) -> None:
-    if w_q.dim() != 2 or w_q.dtype != E4M3 or w_q.shape[1] != K or w_q.shape[0] < 1:
-        raise ValueError(f"w_q must be e4m3 [N, {K}], got {w_q.dtype} {tuple(w_q.shape)}")
-    N = w_q.shape[0]
-    blocks = (-(-N // BLOCK), -(-K // BLOCK))
-    if w_scale.shape != blocks or w_scale.dtype != torch.float32:
-        raise ValueError(f"w_scale must be fp32 {blocks}, got {w_scale.dtype} {tuple(w_scale.shape)}")
-    if bias is not None and (bias.shape != (N,) or bias.dtype != dtype):
+def _check_weight(K: int, w_q, w_scale, bias, dtype) -> int:
+    """Refuses what does not go together; returns N."""
+    shape = w_q.shape
+    if len(shape) != 2 or w_q.dtype is not E4M3 or shape[1] != K or shape[0] < 1:
+        raise ValueError(f"w_q must be e4m3 [N, {K}], got {w_q.dtype} {tuple(shape)}")
+    N = shape[0]
+    if w_scale.shape != (-(-N // BLOCK), -(-K // BLOCK)) or w_scale.dtype is not torch.float32:
+        raise ValueError(f"w_scale must be fp32 {(-(-N // BLOCK), -(-K // BLOCK))}, got {w_scale.dtype} "
+                         f"{tuple(w_scale.shape)}")
+    if bias is not None and (bias.shape != (N,) or bias.dtype is not dtype):
         raise ValueError(f"bias must be {dtype} ({N},), got {bias.dtype} {tuple(bias.shape)}")
+    return N
 
 
 def fp8_block_matmul(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
@@ -143,41 +139,68 @@ def fp8_block_matmul(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor
         raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
     _check_weight(K, w_q, w_scale, bias, out_dtype)
     _lib.require_device(x_q)
-    _lib.same_device(x_q, x_scale=x_scale, w_q=w_q, w_scale=w_scale, bias=bias)
+    _lib.same_device(x_q, x_scale, w_q, w_scale, bias)
     sx = x_scale.reshape(-1, x_scale.shape[-1])
-    y = _gemm(_aligned(x_q.reshape(-1, K)), sx, sx.stride(0), sx.stride(1), _aligned(w_q), w_scale,
-              w_scale.stride(0), w_scale.stride(1), None if bias is None else bias.contiguous(), out_dtype)
-    return y.view(*x_q.shape[:-1], w_q.shape[0])
+    q, w = _aligned(x_q.reshape(-1, K)), _aligned(w_q)
+    bias = None if bias is None else bias.contiguous()
+    M, N = q.shape[0], w.shape[0]
+    y = torch.empty(*x_q.shape[:-1], N, dtype=out_dtype, device=q.device)
+    _lib.call_on(q.get_device(), "zib_fp8_block_gemm", q.data_ptr(), _ld16(q), sx.data_ptr(), sx.stride(0),
+                 sx.stride(1), w.data_ptr(), _ld16(w), w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1),
+                 _lib.ptr(bias), y.data_ptr(), N, _lib.DTYPES[out_dtype], M, N, K)
+    return y
 
 
-def _linear(x2, w_q, w_scale, bias):
-    q, s = _quant_rows(x2)
-    return _gemm(q, s, 1, s.stride(0), w_q, w_scale, w_scale.stride(0), w_scale.stride(1), bias, x2.dtype)
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(M: int, K: int) -> int:
+    return _lib.load().zib_fp8_block_linear_scratch(M, K)
+
+
+def _linear(x, w, sw, sw_n, sw_k, bias, shape):
+    """x [..., K] (rows as ``_rows`` leaves them) through w [N, K]: a fresh tensor of ``shape``."""
+    N, K = w.shape
+    M = x.numel() // K
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    n = _scratch_bytes(M, K)
+    scratch = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _lib.call_on(x.get_device(), "zib_fp8_block_linear", x.data_ptr(),
+                 K if x.is_contiguous() else x.stride(0), _lib.DTYPES[x.dtype], w.data_ptr(), _ld16(w), sw.data_ptr(), sw_n, sw_k,
+                 None if bias is None else bias.data_ptr(), y.data_ptr(), N,
+                 None if n == 0 else scratch.data_ptr(), n, M, N, K)
+    return y
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x2, bias, w_q, w_scale, w_q_t):
+    def forward(ctx, x, bias, w_q, w_scale, w_q_t, shape):
         ctx.save_for_backward(w_q, w_scale, w_q_t)
-        return _linear(x2, w_q, w_scale, bias)
+        ctx.shape = x.shape
+        return _linear(x, w_q, w_scale, w_scale.stride(0), w_scale.stride(1), bias, shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         w_q, w_scale, w_q_t = ctx.saved_tensors
         N = w_q.shape[0]
-        dy = _rows(dy, N)
+        dy = _lead_rows(dy, N)
         dx = db = None
         if ctx.needs_input_grad[0]:
             wt = _aligned(w_q_t) if w_q_t is not None else fp8_block_transpose(w_q)
-            q, s = _quant_rows(dy)
-            dx = _gemm(q, s, 1, s.stride(0), wt, w_scale, w_scale.stride(1), w_scale.stride(0), None, dy.dtype)
+            dx = _linear(dy, wt, w_scale, w_scale.stride(1), w_scale.stride(0), None, ctx.shape)
         if ctx.needs_input_grad[1]:
             db = torch.empty(N, dtype=dy.dtype, device=dy.device)
             ws = torch.empty(64 * N, dtype=torch.float32, device=dy.device)
-            _lib.call_on(dy, "zib_col_sum", dy.data_ptr(), _ld(dy), _lib.DTYPES[dy.dtype], db.data_ptr(),
-                         ws.data_ptr(), ws.numel() * 4, dy.shape[0], N)
-        return dx, db, None, None, None
+            _lib.call_on(dy.get_device(), "zib_col_sum", dy.data_ptr(),
+                         N if dy.is_contiguous() else dy.stride(0), _lib.DTYPES[dy.dtype], db.data_ptr(), ws.data_ptr(), ws.numel() * 4, dy.numel() // N, N)
+        return dx, db, None, None, None, None
+
+
+def _lead_rows(x: torch.Tensor, K: int) -> torch.Tensor:
+    """x [..., K] itself where its rows are a fixed step apart (contiguous, or a matrix with contiguous
+    columns), else a contiguous copy."""
+    if x.is_contiguous() or (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= K):
+        return x
+    return x.contiguous()
 
 
 def fp8_block_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
@@ -194,20 +217,18 @@ def fp8_block_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, 
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be [..., K] with K >= 1, got {tuple(x.shape)}")
     K = x.shape[-1]
-    _check_weight(K, w_q, w_scale, bias, dtype)
-    N = w_q.shape[0]
+    N = _check_weight(K, w_q, w_scale, bias, dtype)
     if w_q_t is not None and (w_q_t.shape != (K, N) or w_q_t.dtype != E4M3):
         raise ValueError(f"w_q_t must be e4m3 ({K}, {N}), got {w_q_t.dtype} {tuple(w_q_t.shape)}")
     _lib.require_device(x)
-    _lib.same_device(x, w_q=w_q, w_scale=w_scale, bias=bias, w_q_t=w_q_t)
+    _lib.same_device(x, w_q, w_scale, bias, w_q_t)
     grad = torch.is_grad_enabled()
     if grad and (w_scale.requires_grad or w_q.requires_grad):
         raise ValueError("the quantised weight of fp8_block_linear is a constant and must not require gradients")
-    x2, w = _rows(x, K), _aligned(w_q)
+    w = _aligned(w_q)
+    shape = (*x.shape[:-1], N)
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     if grad and (x.requires_grad or (bias is not None and bias.requires_grad)):
-        y = _Linear.apply(x2, bias, w, w_scale, w_q_t)
-    else:
-        y = _linear(x2, w, w_scale, bias)
-    return y.view(*x.shape[:-1], N)
+        return _Linear.apply(_lead_rows(x, K), bias, w, w_scale, w_q_t, shape)
+    return _linear(_lead_rows(x, K), w, w_scale, w_scale.stride(0), w_scale.stride(1), bias, shape)

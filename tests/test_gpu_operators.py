@@ -221,6 +221,36 @@ def test_product_sums_are_kept_in_32_bits(cuda, M):
     assert bool((y == want).all()), float((y - want).abs().max())
 
 
+@pytest.mark.parametrize("M", [1, 8, 9, 16, 17, 300])
+def test_linear_sums_are_kept_in_32_bits(cuda, M):
+    """The same through the linear, whose few-token form sums on other instructions: values that the
+    quantiser holds exactly (448 gives a block the scale 1)."""
+    K, N = 1024, 256
+    x = torch.full((M, K), 2.0 ** -6, device="cuda")
+    x[:, ::128], x[:, 1::128] = 448.0, -448.0
+    x[:, 3], x[:, 260] = 256.0, -256.0
+    y = fp8_block_linear(x, torch.ones(N, K, device="cuda").to(torch.float8_e4m3fn), torch.ones(2, 8, device="cuda"))
+    assert bool((y == (K - 18) * 2.0 ** -6).all()), float((y - (K - 18) * 2.0 ** -6).abs().max())
+
+
+@pytest.mark.parametrize("M", [1, 5, 40])
+def test_linear_of_one_row_dimensions(cuda, M):
+    """Views whose dimensions of one element carry strides of their own."""
+    g = _gen(3)
+    wq, ws = fp8_block_quantize_weight(_randn(g, 130, 256))
+    x = _randn(g, 1, M, 256).to(torch.bfloat16)
+    want = fp8_block_linear(x[0], wq, ws)
+    assert torch.equal(fp8_block_linear(x.transpose(0, 1), wq, ws)[:, 0], want)
+    xs = x.transpose(0, 1).detach().requires_grad_()
+    d = _randn(g, 1, M, 130).to(torch.bfloat16)
+    (dx,) = torch.autograd.grad(fp8_block_linear(xs, wq, ws), (xs,), d.transpose(0, 1))
+    x0 = x[0].detach().requires_grad_()
+    (d0,) = torch.autograd.grad(fp8_block_linear(x0, wq, ws), (x0,), d[0])
+    assert torch.equal(dx[:, 0], d0)
+    wide = _randn(g, M, 300).to(torch.bfloat16)[:, 8:264]
+    assert torch.equal(fp8_block_linear(wide, wq, ws), fp8_block_linear(wide.contiguous(), wq, ws))
+
+
 @pytest.mark.parametrize("M,at", [(4, (2, 300)), (150, (149, 0)), (600, (300, 639))])
 def test_linear_non_finite_rows_stay_apart(cuda, M, at):
     K, N = 640, 256
