@@ -2,39 +2,142 @@
 // quantisers, transposed weights, and the column sums of a bias gradient.
 #include "fp8_quant.cuh"
 
+#include <type_traits>
+
 namespace zib {
 namespace fp8 {
 
-// Activation rows.  Bound by memory (3 bytes per 16-bit element): a warp takes 8 rows of two blocks,
-// 16 lanes x 8 values to a block, with all its loads in flight before the first is used; the 8 rows
-// give each block one whole 32-byte sector of the scales, which lie row after row.
-constexpr int kRowsPerWarp = 8;
+// 8 values as they lie in memory: whole 16-byte pieces where VEC (K % 8 == 0: all eight or none)
+template <typename T>
+struct Raw {
+  Pack<T, 16 / sizeof(T)> v[sizeof(T) / 2];
+};
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quant_rows_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
-                                                         int64_t ldq, float* __restrict__ s, int64_t s_m, int64_t s_k,
-                                                         int64_t M, int64_t K) {
-  const int lane = threadIdx.x & 31;
-  const int64_t pairs = (K + 2 * kBlock - 1) / (2 * kBlock);
-  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t m0 = id / pairs * kRowsPerWarp;
-  if (m0 >= M) return;
-  const int64_t b = 2 * (id % pairs) + (lane >> 4), k = b * kBlock + (lane & 15) * 8;
-  float v[kRowsPerWarp][8];
+__device__ __forceinline__ Raw<T> load_raw(const T* __restrict__ row, int64_t k, int64_t K) {
+  constexpr int E = 16 / sizeof(T);
+  Raw<T> r{};
 #pragma unroll
-  for (int r = 0; r < kRowsPerWarp; ++r) load8<T, VEC>(x + (m0 + r) * ldx, k, m0 + r < M ? K : 0, v[r]);
-  float mine = 0.0f;  // lane r of each half warp keeps the scale of row r
+  for (int h = 0; h < 8 / E; ++h) {
+    if constexpr (VEC) {
+      if (k < K) r.v[h] = *reinterpret_cast<const Pack<T, E>*>(row + k + h * E);
+    } else {
 #pragma unroll
-  for (int r = 0; r < kRowsPerWarp; ++r) {
-    uint32_t a = amax8(v[r]);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
-    const float sc = block_scale(a);
-    if ((lane & 15) == r) mine = sc;
-    store8<VEC>(q + (m0 + r) * ldq, k, m0 + r < M ? K : 0, v[r], inverse_scale(sc));
+      for (int j = 0; j < E; ++j)
+        if (k + h * E + j < K) r.v[h].v[j] = row[k + h * E + j];
+    }
   }
-  const int r = lane & 15;
-  if (r < kRowsPerWarp && m0 + r < M && b * kBlock < K) s[(m0 + r) * s_m + b * s_k] = mine;
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T>& r, float (&v)[8]) {
+  constexpr int E = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = to_f32(r.v[j / E].v[j % E]);
+}
+
+// The largest magnitude of 8 lanes' 16 values each, as fp32 bits.  Magnitudes order as their bits, so
+// the 16-bit types compare two at a time without unpacking.
+template <typename T>
+__device__ __forceinline__ uint32_t block_amax(const Raw<T>& lo, const Raw<T>& hi) {
+  if constexpr (sizeof(T) == 2) {
+    auto max2 = [](uint32_t a, uint32_t b) {
+      uint32_t m;
+      asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+      return m;
+    };
+    const uint4 u = *reinterpret_cast<const uint4*>(&lo), w = *reinterpret_cast<const uint4*>(&hi);
+    uint32_t m = max2(max2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), max2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+    m = max2(m, max2(max2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), max2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = max2(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const uint16_t a = (uint16_t)max(m >> 16, m & 0xFFFFu);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&a)));
+  } else {
+    float f[8], h[8];
+    widen(lo, f);
+    widen(hi, h);
+    uint32_t a = max(amax8(f), amax8(h));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+    return a;
+  }
+}
+
+// Activation rows.  Bound by memory (3 bytes per 16-bit element).  A CTA takes kRows rows of four blocks
+// (512 columns), a warp kRows / 8 of them, two rows in flight; 8 lanes x 16 values to a block (8 of
+// either half of it, so that accesses stay side by side): what is done once per block and lane, its
+// maximum over lanes and its scale, counts half as much as with 16 lanes.
+// SUM: the CTA leaves the sums of its columns in part[.][K] (a bias gradient: the rows need not be read
+// again for it).
+constexpr int kRows = 64;
+constexpr int kQuad = 4 * kBlock;
+
+template <typename T, bool VEC, bool SUM>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && !SUM ? 4 : 3) quant_rows_kernel(
+    const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s, int64_t s_m,
+    int64_t s_k, float* __restrict__ part, int64_t M, int64_t K, int quads) {
+  constexpr int U = 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t group = blockIdx.x / quads;
+  const int64_t b = 4 * (int64_t)(blockIdx.x - group * quads) + (lane >> 3);
+  const int64_t k = b * kBlock + (lane & 7) * 8;
+  const int64_t m0 = group * kRows + warp * (kRows / 8);
+  const int rows = M - m0 < kRows / 8 ? (int)(M - m0) : kRows / 8;
+  const T* xr = x + m0 * ldx;
+  uint8_t* qr = q + m0 * ldq;
+  float* sr = s + m0 * s_m + b * s_k;
+  float sum[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) sum[j] = 0.0f;
+#pragma unroll 1
+  for (int m = 0; m < rows; m += U) {
+    Raw<T> lo[U], hi[U];
+#pragma unroll
+    for (int r = 0; r < U; ++r) {
+      const int64_t Kr = m + r < rows ? K : 0;
+      lo[r] = load_raw<T, VEC>(xr + r * ldx, k, Kr);
+      hi[r] = load_raw<T, VEC>(xr + r * ldx, k + 64, Kr);
+    }
+#pragma unroll
+    for (int r = 0; r < U; ++r) {
+      const float sc = block_scale(block_amax(lo[r], hi[r])), inv = inverse_scale(sc);
+      const int64_t Kr = m + r < rows ? K : 0;
+      float f[8];
+      widen(lo[r], f);
+      if constexpr (SUM)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += f[j];
+      store8<VEC>(qr + r * ldq, k, Kr, f, inv);
+      widen(hi[r], f);
+      if constexpr (SUM)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[8 + j] += f[j];
+      store8<VEC>(qr + r * ldq, k + 64, Kr, f, inv);
+      if ((lane & 7) == 0 && b * kBlock < Kr) sr[r * s_m] = sc;
+    }
+    xr += U * ldx;
+    qr += U * ldq;
+    sr += U * s_m;
+  }
+  if constexpr (SUM) {
+    __shared__ float red[8][kQuad];
+    const int c = (lane >> 3) * kBlock + (lane & 7) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      red[warp][c + j] = sum[j];
+      red[warp][c + 64 + j] = sum[8 + j];
+    }
+    __syncthreads();
+    const int64_t k0 = 4 * (int64_t)(blockIdx.x - group * quads) * kBlock;
+    for (int i = threadIdx.x; i < kQuad && k0 + i < K; i += 256) {
+      float v = red[0][i];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) v += red[w][i];
+      part[group * K + k0 + i] = v;
+    }
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product may start and wait
 }
 
@@ -79,29 +182,46 @@ __global__ void __launch_bounds__(256) transpose_kernel(const uint8_t* __restric
   }
 }
 
-// column sums of x [M, N] in fp32 (a bias gradient): partial sums of row slabs, then their sums
+// column sums of x [M, N] (a bias gradient): fp32 sums of slabs of rows ...
 template <typename T>
 __global__ void __launch_bounds__(256) col_sum_part_kernel(const T* __restrict__ x, int64_t ldx,
                                                            float* __restrict__ part, int64_t M, int64_t N,
                                                            int64_t slab) {
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (n >= N) return;
-  const int64_t m1 = ((int64_t)blockIdx.y + 1) * slab < M ? ((int64_t)blockIdx.y + 1) * slab : M;
+  const int64_t m0 = (int64_t)blockIdx.y * slab, m1 = m0 + slab < M ? m0 + slab : M;
   float s = 0.0f;
-  for (int64_t m = (int64_t)blockIdx.y * slab; m < m1; ++m) s += to_f32(x[m * ldx + n]);
+#pragma unroll 8
+  for (int64_t m = m0; m < m1; ++m) s += to_f32(x[m * ldx + n]);
   part[blockIdx.y * N + n] = s;
 }
+// ... and their sums: 32 columns per CTA, 8 threads to a column
 template <typename T>
 __global__ void __launch_bounds__(256) col_sum_kernel(const float* __restrict__ part, T* __restrict__ y, int64_t N,
-                                                      int slabs) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+                                                      int64_t slabs) {
+  __shared__ double red[8][32];
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + c;
   double s = 0.0;
-  for (int i = 0; i < slabs; ++i) s += part[i * N + n];
-  y[n] = from_f32<T>((float)s);
+  if (n < N)
+    for (int64_t i = r; i < slabs; i += 8) s += part[i * N + n];
+  red[r][c] = s;
+  __syncthreads();
+  if (r == 0 && n < N) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][c];
+    y[n] = from_f32<T>((float)s);
+  }
 }
 
 constexpr int kMaxSlabs = 64;
+
+static void col_sum(const float* part, void* y, int dtype, int64_t N, int64_t slabs, cudaStream_t st) {
+  const unsigned g = (unsigned)ceil_div(N, 32);
+  if (dtype == ZIB_BF16) col_sum_kernel<<<g, 256, 0, st>>>(part, (__nv_bfloat16*)y, N, slabs);
+  else if (dtype == ZIB_F16) col_sum_kernel<<<g, 256, 0, st>>>(part, (__half*)y, N, slabs);
+  else col_sum_kernel<<<g, 256, 0, st>>>(part, (float*)y, N, slabs);
+}
 
 // eight values per access: columns, strides and addresses of input and output allow it
 static bool whole_vectors(const void* x, int64_t ldx, int size, const void* q, int64_t ldq, int64_t rows, int64_t K) {
@@ -114,20 +234,27 @@ static bool whole_vectors(const void* x, int64_t ldx, int size, const void* q, i
 
 using namespace zib;
 
+int64_t zib::fp8_sum_rows(int64_t M) { return ceil_div(M, fp8::kRows); }
+
 int zib::fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m, int64_t s_k,
-                        int64_t M, int64_t K, cudaStream_t st, const char* what) {
-  const int64_t grid = ceil_div(ceil_div(M, fp8::kRowsPerWarp) * ceil_div(K, 2 * fp8::kBlock), 8);
+                        float* part, int64_t M, int64_t K, cudaStream_t st, const char* what) {
+  const int64_t quads = ceil_div(K, fp8::kQuad), grid = ceil_div(M, fp8::kRows) * quads;
   ZIB_HOST_CHECK(grid <= 0x7FFFFFFF, ZIB_ERR_TOO_LARGE, "%s: M=%lld K=%lld", what, (long long)M, (long long)K);
   const bool vec = fp8::whole_vectors(x, ldx, dtype_bytes(dtype), q, ldq, M, K);
-  auto go = [&](auto kernel, auto* xt) {
-    kernel<<<(unsigned)grid, 256, 0, st>>>(xt, ldx, (uint8_t*)q, ldq, s, s_m, s_k, M, K);
+  auto go = [&](auto* xt) {
+    using T = std::remove_cv_t<std::remove_pointer_t<decltype(xt)>>;
+    auto* kernel = part ? (vec ? fp8::quant_rows_kernel<T, true, true> : fp8::quant_rows_kernel<T, false, true>)
+                        : (vec ? fp8::quant_rows_kernel<T, true, false> : fp8::quant_rows_kernel<T, false, false>);
+    kernel<<<(unsigned)grid, 256, 0, st>>>(xt, ldx, (uint8_t*)q, ldq, s, s_m, s_k, part, M, K, (int)quads);
   };
-  using B = __nv_bfloat16;
-  using H = __half;
-  if (dtype == ZIB_BF16) go(vec ? fp8::quant_rows_kernel<B, true> : fp8::quant_rows_kernel<B, false>, (const B*)x);
-  else if (dtype == ZIB_F16) go(vec ? fp8::quant_rows_kernel<H, true> : fp8::quant_rows_kernel<H, false>, (const H*)x);
-  else go(vec ? fp8::quant_rows_kernel<float, true> : fp8::quant_rows_kernel<float, false>, (const float*)x);
+  if (dtype == ZIB_BF16) go((const __nv_bfloat16*)x);
+  else if (dtype == ZIB_F16) go((const __half*)x);
+  else go((const float*)x);
   return zib_check_launch(what);
+}
+
+void zib::fp8_sum_finish(const float* part, void* sum, int dtype, int64_t M, int64_t K, cudaStream_t st) {
+  fp8::col_sum(part, sum, dtype, K, fp8_sum_rows(M), st);
 }
 
 extern "C" int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m,
@@ -138,7 +265,7 @@ extern "C" int zib_fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q
                  (long long)M, (long long)K);
   if (M == 0) return ZIB_OK;
   ZIB_HOST_CHECK(x && q && s, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
-  return fp8_quant_rows(x, ldx, dtype, q, ldq, s, s_m, s_k, M, K, (cudaStream_t)stream, what);
+  return fp8_quant_rows(x, ldx, dtype, q, ldq, s, s_m, s_k, nullptr, M, K, (cudaStream_t)stream, what);
 }
 
 extern "C" int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void* q, int64_t ldq, float* s, int64_t s_n,
@@ -187,17 +314,13 @@ extern "C" int zib_col_sum(const void* x, int64_t ldx, int dtype, void* y, float
                  "%s: workspace of %lld bytes needed", what, (long long)(fp8::kMaxSlabs * N * sizeof(float)));
   const int64_t slab = ceil_div(M > 0 ? M : 1, fp8::kMaxSlabs);
   const int slabs = (int)ceil_div(M, slab);
-  const dim3 g((unsigned)ceil_div(N, 256), (unsigned)(slabs > 0 ? slabs : 1));
+  const dim3 g((unsigned)ceil_div(N, 256), (unsigned)slabs);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == ZIB_BF16) {
-    if (slabs) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const __nv_bfloat16*)x, ldx, workspace, M, N, slab);
-    fp8::col_sum_kernel<<<g.x, 256, 0, st>>>(workspace, (__nv_bfloat16*)y, N, slabs);
-  } else if (dtype == ZIB_F16) {
-    if (slabs) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const __half*)x, ldx, workspace, M, N, slab);
-    fp8::col_sum_kernel<<<g.x, 256, 0, st>>>(workspace, (__half*)y, N, slabs);
-  } else {
-    if (slabs) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const float*)x, ldx, workspace, M, N, slab);
-    fp8::col_sum_kernel<<<g.x, 256, 0, st>>>(workspace, (float*)y, N, slabs);
+  if (slabs > 0) {
+    if (dtype == ZIB_BF16) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const __nv_bfloat16*)x, ldx, workspace, M, N, slab);
+    else if (dtype == ZIB_F16) fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const __half*)x, ldx, workspace, M, N, slab);
+    else fp8::col_sum_part_kernel<<<g, 256, 0, st>>>((const float*)x, ldx, workspace, M, N, slab);
   }
+  fp8::col_sum(workspace, y, dtype, N, slabs, st);
   return zib_check_launch(what);
 }

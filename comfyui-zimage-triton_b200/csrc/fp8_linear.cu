@@ -229,19 +229,28 @@ static bool is_fused(int64_t M, int64_t kb) { return M <= kFusedTokens && fused_
 
 using namespace zib;
 
-static int64_t scratch_bytes(int64_t M, int64_t K) {
+// scratch: quantised rows, their scales, and where the column sums are wanted their parts
+struct Scratch {
+  int64_t scales, part, bytes;
+};
+
+static Scratch scratch_of(int64_t M, int64_t K, bool sum) {
   const int64_t kb = ceil_div(K, fp8::kBlock);
-  if (fp8::is_fused(M, kb)) return 0;
-  return ceil_div(M * ceil_div(K, 16) * 16, 128) * 128 + kb * M * 4;
+  Scratch s{};
+  if (!sum && fp8::is_fused(M, kb)) return s;
+  s.scales = ceil_div(M * ceil_div(K, 16) * 16, 128) * 128;
+  s.part = s.scales + ceil_div(kb * M * 4, 128) * 128;
+  s.bytes = s.part + (sum ? fp8_sum_rows(M) * K * 4 : 0);
+  return s;
 }
 
-extern "C" int64_t zib_fp8_block_linear_scratch(int64_t M, int64_t K) {
-  return M < 1 || K < 1 || K >= (1ll << 31) ? 0 : scratch_bytes(M, K);
+extern "C" int64_t zib_fp8_block_linear_scratch(int64_t M, int64_t K, int with_sum) {
+  return M < 1 || K < 1 || K >= (1ll << 31) ? 0 : scratch_of(M, K, with_sum != 0).bytes;
 }
 
 extern "C" int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_t ldw, const float* sw,
-                                    int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, void* scratch,
-                                    int64_t nscratch, int64_t M, int64_t N, int64_t K, void* stream) {
+                                    int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, void* sum,
+                                    void* scratch, int64_t nscratch, int64_t M, int64_t N, int64_t K, void* stream) {
   const char* what = "zib_fp8_block_linear";
   ZIB_HOST_CHECK(known_dtype(dtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype %d", what, dtype);
   ZIB_HOST_CHECK(M >= 0 && N >= 1 && K >= 1 && ldx >= K && ldw >= K && ldy >= N, ZIB_ERR_INVALID_ARG,
@@ -249,22 +258,27 @@ extern "C" int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const
   ZIB_HOST_CHECK(M < (1ll << 31) - 512 && N < (1ll << 31) - 512 && K < (1ll << 31) - 512, ZIB_ERR_TOO_LARGE,
                  "%s: M=%lld N=%lld K=%lld", what, (long long)M, (long long)N, (long long)K);
   ZIB_HOST_CHECK(ldw % 16 == 0 && (uintptr_t)w % 16 == 0, ZIB_ERR_ALIGNMENT, "%s: w needs 16-byte aligned rows", what);
-  if (M == 0) return ZIB_OK;
-  ZIB_HOST_CHECK(x && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
   cudaStream_t st = (cudaStream_t)stream;
+  if (M == 0) {
+    if (sum) fp8_sum_finish(nullptr, sum, dtype, 0, K, st);
+    return sum ? zib_check_launch(what) : ZIB_OK;
+  }
+  ZIB_HOST_CHECK(x && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
   const int64_t kb = ceil_div(K, fp8::kBlock), ldq = ceil_div(K, 16) * 16;
-  const bool fused = fp8::is_fused(M, kb);
+  const Scratch sc = scratch_of(M, K, sum != nullptr);
   float* s = nullptr;
-  if (!fused) {
-    const int64_t need = scratch_bytes(M, K);
-    ZIB_HOST_CHECK(scratch && nscratch >= need && (uintptr_t)scratch % 128 == 0, ZIB_ERR_INVALID_ARG,
-                   "%s: scratch of %lld bytes, 128-byte aligned, needed", what, (long long)need);
-    s = (float*)((uint8_t*)scratch + ceil_div(M * ldq, 128) * 128);
-    const int rc = fp8_quant_rows(x, ldx, dtype, scratch, ldq, s, 1, M, M, K, st, what);
+  if (sc.bytes) {
+    ZIB_HOST_CHECK(scratch && nscratch >= sc.bytes && (uintptr_t)scratch % 128 == 0, ZIB_ERR_INVALID_ARG,
+                   "%s: scratch of %lld bytes, 128-byte aligned, needed", what, (long long)sc.bytes);
+    s = (float*)((uint8_t*)scratch + sc.scales);
+    float* part = sum ? (float*)((uint8_t*)scratch + sc.part) : nullptr;
+    const int rc = fp8_quant_rows(x, ldx, dtype, scratch, ldq, s, 1, M, part, M, K, st, what);
     if (rc) return rc;
+    if (sum) fp8_sum_finish(part, sum, dtype, M, K, st);
   }
   if (M > fp8::kMaxTokens)
     return fp8_gemm(scratch, ldq, s, 1, M, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, st, what);
+  const bool fused = sc.bytes == 0;
   const int size = dtype_bytes(dtype);
   fp8::SmallParams p{};
   p.x = fused ? x : scratch; p.ldx = fused ? ldx : ldq; p.sx = s;

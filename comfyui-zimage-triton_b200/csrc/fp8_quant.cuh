@@ -78,9 +78,12 @@ __device__ __forceinline__ void store8(uint8_t* __restrict__ row, int64_t k, int
 
 }  // namespace fp8
 
-// rows of x [M, K] as e4m3 q and scales s (fp8_block.cu)
+// fp8_block.cu: rows of x [M, K] as e4m3 q and scales s.  part (may be null): the sums of x's columns
+// over slabs of rows, fp8_sum_rows(M) rows of K floats, which fp8_sum_finish adds up.
 int fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m, int64_t s_k,
-                   int64_t M, int64_t K, cudaStream_t st, const char* what);
+                   float* part, int64_t M, int64_t K, cudaStream_t st, const char* what);
+int64_t fp8_sum_rows(int64_t M);
+void fp8_sum_finish(const float* part, void* sum, int dtype, int64_t M, int64_t K, cudaStream_t st);
 // the product on tensor cores (fp8_gemm.cu)
 int fp8_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k, const void* w, int64_t ldw,
              const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, int dtype, int64_t M,

@@ -152,21 +152,24 @@ def fp8_block_matmul(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor
 
 
 @functools.lru_cache(maxsize=4096)
-def _scratch_bytes(M: int, K: int) -> int:
-    return _lib.load().zib_fp8_block_linear_scratch(M, K)
+def _scratch_bytes(M: int, K: int, with_sum: int) -> int:
+    return _lib.load().zib_fp8_block_linear_scratch(M, K, with_sum)
 
 
-def _linear(x, w, sw, sw_n, sw_k, bias, shape):
-    """x [..., K] (rows as ``_rows`` leaves them) through w [N, K]: a fresh tensor of ``shape``."""
+def _linear(x, w, sw, sw_n, sw_k, bias, shape, col_sum=None):
+    """x [..., K] (rows as ``_lead_rows`` leaves them) through w [N, K]: a fresh tensor of ``shape``;
+    the sums of x's columns into ``col_sum``."""
     N, K = w.shape
     M = x.numel() // K
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    n = _scratch_bytes(M, K)
-    scratch = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _lib.call_on(x.get_device(), "zib_fp8_block_linear", x.data_ptr(),
-                 K if x.is_contiguous() else x.stride(0), _lib.DTYPES[x.dtype], w.data_ptr(), _ld16(w), sw.data_ptr(), sw_n, sw_k,
+    device = x.device
+    y = torch.empty(shape, dtype=x.dtype, device=device)
+    n = _scratch_bytes(M, K, col_sum is not None)
+    scratch = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    _lib.call_on(x.get_device(), "zib_fp8_block_linear", x.data_ptr(), K if x.is_contiguous() else x.stride(0),
+                 _lib.DTYPES[x.dtype], w.data_ptr(), _ld16(w), sw.data_ptr(), sw_n, sw_k,
                  None if bias is None else bias.data_ptr(), y.data_ptr(), N,
-                 None if n == 0 else scratch.data_ptr(), n, M, N, K)
+                 None if col_sum is None else col_sum.data_ptr(), None if scratch is None else scratch.data_ptr(), n,
+                 M, N, K)
     return y
 
 
@@ -184,14 +187,15 @@ class _Linear(torch.autograd.Function):
         N = w_q.shape[0]
         dy = _lead_rows(dy, N)
         dx = db = None
-        if ctx.needs_input_grad[0]:
-            wt = _aligned(w_q_t) if w_q_t is not None else fp8_block_transpose(w_q)
-            dx = _linear(dy, wt, w_scale, w_scale.stride(1), w_scale.stride(0), None, ctx.shape)
         if ctx.needs_input_grad[1]:
             db = torch.empty(N, dtype=dy.dtype, device=dy.device)
+        if ctx.needs_input_grad[0]:  # the pass that quantises dy adds up its columns too
+            wt = _aligned(w_q_t) if w_q_t is not None else fp8_block_transpose(w_q)
+            dx = _linear(dy, wt, w_scale, w_scale.stride(1), w_scale.stride(0), None, ctx.shape, db)
+        elif db is not None:
             ws = torch.empty(64 * N, dtype=torch.float32, device=dy.device)
-            _lib.call_on(dy.get_device(), "zib_col_sum", dy.data_ptr(),
-                         N if dy.is_contiguous() else dy.stride(0), _lib.DTYPES[dy.dtype], db.data_ptr(), ws.data_ptr(), ws.numel() * 4, dy.numel() // N, N)
+            _lib.call_on(dy.get_device(), "zib_col_sum", dy.data_ptr(), N if dy.is_contiguous() else dy.stride(0),
+                         _lib.DTYPES[dy.dtype], db.data_ptr(), ws.data_ptr(), ws.numel() * 4, dy.numel() // N, N)
         return dx, db, None, None, None, None
 
 

@@ -342,13 +342,15 @@ ZIB_API int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int6
                        int64_t K, void* stream);
 
 /* zib_fp8_quant_rows and zib_fp8_block_gemm in one call: y = x W^T (+ bias), x and y
- * and bias of `dtype`.  scratch: zib_fp8_block_linear_scratch(M, K) bytes, 128-byte
- * aligned, for the quantised rows; 0 for one or two rows, which run as one launch. */
-ZIB_API int64_t zib_fp8_block_linear_scratch(int64_t M, int64_t K);
+ * and bias of `dtype`.  sum (may be NULL): the sums of x's columns, [K] of dtype, from
+ * the same pass over x (the bias gradient where x is dy).  scratch:
+ * zib_fp8_block_linear_scratch(M, K, sum != NULL) bytes, 128-byte aligned; 0 bytes for
+ * one or two rows without sums, which run as one launch. */
+ZIB_API int64_t zib_fp8_block_linear_scratch(int64_t M, int64_t K, int with_sum);
 ZIB_API int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_t ldw,
                          const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y,
-                         int64_t ldy, void* scratch, int64_t nscratch, int64_t M, int64_t N,
-                         int64_t K, void* stream);
+                         int64_t ldy, void* sum, void* scratch, int64_t nscratch, int64_t M,
+                         int64_t N, int64_t K, void* stream);
 
 /* wt[k,n] = w[n,k] of 8-bit values: the weight of the gradient towards the
  * activations (its scales are the same blocks, transposed). */

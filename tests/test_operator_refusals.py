@@ -121,13 +121,15 @@ def test_c_entries_validate_on_the_host():
     assert lib.zib_fp8_block_gemm(16, 1 << 31, 16, 1, 1, 16, 1 << 31, 16, 1, 1, None, 16, 8, 0, 4, 8, 1 << 31, None) \
         == _lib.ZIB_ERR_TOO_LARGE
     assert lib.zib_fp8_block_gemm(None, 128, None, 1, 1, None, 128, None, 1, 1, None, None, 8, 0, 0, 8, 128, None) == 0
-    assert lib.zib_fp8_block_linear(16, 64, 0, 16, 128, 16, 1, 1, None, 16, 8, None, 0, 4, 8, 128, None) == INV
-    assert lib.zib_fp8_block_linear(16, 128, 0, 16, 120, 16, 1, 1, None, 16, 8, None, 0, 4, 8, 120, None) == \
+    assert lib.zib_fp8_block_linear(16, 64, 0, 16, 128, 16, 1, 1, None, 16, 8, None, None, 0, 4, 8, 128, None) == INV
+    assert lib.zib_fp8_block_linear(16, 128, 0, 16, 120, 16, 1, 1, None, 16, 8, None, None, 0, 4, 8, 120, None) == \
         _lib.ZIB_ERR_ALIGNMENT
-    assert lib.zib_fp8_block_linear(16, 128, 0, 16, 128, 16, 1, 1, None, 16, 8, 128, 64, 40, 8, 128, None) == INV
-    assert lib.zib_fp8_block_linear(None, 128, 0, None, 128, None, 1, 1, None, None, 8, None, 0, 0, 8, 128, None) == 0
-    assert lib.zib_fp8_block_linear_scratch(0, 128) == 0
-    assert lib.zib_fp8_block_linear_scratch(40, 130) == 40 * 144 + 2 * 40 * 4
+    assert lib.zib_fp8_block_linear(16, 128, 0, 16, 128, 16, 1, 1, None, 16, 8, None, 128, 64, 40, 8, 128, None) == INV
+    assert lib.zib_fp8_block_linear(None, 128, 0, None, 128, None, 1, 1, None, None, 8, None, None, 0, 0, 8, 128, None) == 0
+    assert lib.zib_fp8_block_linear_scratch(0, 128, 0) == 0
+    assert lib.zib_fp8_block_linear_scratch(1, 128, 0) == 0
+    assert lib.zib_fp8_block_linear_scratch(40, 130, 0) >= 40 * 144 + 2 * 40 * 4
+    assert lib.zib_fp8_block_linear_scratch(40, 130, 1) >= 40 * 144 + 2 * 40 * 4 + 130 * 4
     assert lib.zib_fp8_transpose(None, 8, None, 8, 8, 8, None) == INV
     assert lib.zib_col_sum(16, 8, 0, 16, 16, 4, 4, 8, None) == INV
     rot = [16, 0, 0, 0, 16, 1, None, 0, 0, 0, None, 0]
