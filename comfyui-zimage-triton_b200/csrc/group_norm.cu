@@ -26,9 +26,8 @@
 // Arithmetic is on packed pairs (f32x2): at 12 elements per clock and SM, the rate of HBM, single
 // operations left the SMs short of issue slots (79 us instead of TBD for the statistics of
 // [1, 1048576, 128]).
-#include "rot_pack.cuh"
+#include "zib_pairs.cuh"
 #include "zib_tcgen05.cuh"
-#include "zib_types.cuh"
 
 namespace zib {
 namespace gn {
@@ -95,46 +94,7 @@ __device__ __forceinline__ float2 ld_cluster(const float2* p, uint32_t rank) {
 __device__ __forceinline__ void allow_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// --- packed pairs ------------------------------------------------------------------
-
 using px::f2;
-
-__device__ __forceinline__ f2 dup(float v) { return px::mk(v, v); }
-
-template <int VEC>
-constexpr int kPairs = VEC < 2 ? 1 : VEC / 2;
-
-// VEC elements as fp32 pairs (a single one with 0 beside it)
-__device__ __forceinline__ f2 pair_of(const __nv_bfloat16* v) {
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(v);
-  return px::mk(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-__device__ __forceinline__ f2 pair_of(const __half* v) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(v));
-  return px::mk(f.x, f.y);
-}
-__device__ __forceinline__ f2 pair_of(const float* v) { return px::mk(v[0], v[1]); }
-
-template <typename T, int VEC>
-__device__ __forceinline__ void unpack(const Pack<T, VEC>& t, f2 (&o)[kPairs<VEC>]) {
-  if constexpr (VEC == 1) o[0] = px::mk(to_f32(t.v[0]), 0.0f);
-  else
-#pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) o[i] = pair_of(t.v + 2 * i);
-}
-
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> pack(const f2 (&o)[kPairs<VEC>]) {
-  Pack<T, VEC> t;
-#pragma unroll
-  for (int i = 0; i < kPairs<VEC>; ++i) {
-    float lo, hi;
-    px::split(o[i], lo, hi);
-    t.v[2 * i] = from_f32<T>(lo);
-    if constexpr (VEC > 1) t.v[2 * i + 1] = from_f32<T>(hi);
-  }
-  return t;
-}
 
 // --- activation ------------------------------------------------------------------
 

@@ -15,7 +15,7 @@
 // per thread at the price of registers (four heads in flight, 25 to 37% occupancy) measured slower,
 // 97 instead of TBD us for [2, 4608, 30 + 30, 128].
 #include "zib_async.cuh"
-#include "zib_types.cuh"
+#include "zib_pairs.cuh"
 
 ZIB_DEFINE_ERROR_READER(zib_err_read_clear_rotary)
 
@@ -46,6 +46,68 @@ struct Params {
   float sign;
 };
 
+// the tensors that are read are not written by the launch: loads may pass stores
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_vec(const T* p) {
+  Pack<T, VEC> r;
+  if constexpr (sizeof(r) == 16) *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
+  else if constexpr (sizeof(r) == 8) *reinterpret_cast<uint2*>(&r) = __ldg(reinterpret_cast<const uint2*>(p));
+  else if constexpr (sizeof(r) == 4) *reinterpret_cast<uint32_t*>(&r) = __ldg(reinterpret_cast<const uint32_t*>(p));
+  else *reinterpret_cast<uint16_t*>(&r) = __ldg(reinterpret_cast<const uint16_t*>(p));
+  return r;
+}
+
+// The cos and sin of one unit: per pair of neighbouring features (interleaved) or of pairs (half).
+template <int VEC, bool HALF>
+struct Angles {
+  // interleaved, pair j: c = (cos, cos), s = (-sin, sin): (a, b) c + (b, a) s
+  // half, pairs 2j and 2j + 1: c = (cos, cos'), s = (sin, sin')
+  static constexpr int N = VEC < 2 ? 1 : VEC / 2;
+  f2 c[N], s[N];
+  __device__ __forceinline__ void set(int i, float cv, float sv) {  // pair i of the unit
+    if constexpr (HALF) {
+      float c0, c1, s0, s1;
+      px::split(c[i / 2], c0, c1);
+      px::split(s[i / 2], s0, s1);
+      if (i & 1) c1 = cv, s1 = sv;
+      else c0 = cv, s0 = sv;
+      c[i / 2] = px::mk(c0, c1);
+      s[i / 2] = px::mk(s0, s1);
+    } else {
+      c[i] = px::mk(cv, cv);
+      s[i] = px::mk(-sv, sv);
+    }
+  }
+};
+
+__device__ __forceinline__ f2 negate(f2 v) { return v ^ 0x8000000080000000ull; }
+__device__ __forceinline__ f2 swap(f2 v) {
+  float a, b;
+  px::split(v, a, b);
+  return px::mk(b, a);
+}
+
+// one head's unit in a (and d: its second vector); each output is one product and one multiply-add
+template <typename T, int VEC, bool HALF>
+__device__ __forceinline__ void turn(const Angles<VEC, HALF>& w, Pack<T, VEC>& a, Pack<T, VEC>& d) {
+  f2 u[kPairs<VEC>], v[kPairs<VEC>];
+  unpack<T, VEC>(a, u);
+  if constexpr (HALF) {
+    unpack<T, VEC>(d, v);
+#pragma unroll
+    for (int j = 0; j < kPairs<VEC>; ++j) {
+      const f2 r = px::fma(u[j], w.c[j], negate(px::mul(v[j], w.s[j])));
+      v[j] = px::fma(v[j], w.c[j], px::mul(u[j], w.s[j]));
+      u[j] = r;
+    }
+    d = pack<T, VEC>(v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPairs<VEC>; ++j) u[j] = px::fma(u[j], w.c[j], px::mul(swap(u[j]), w.s[j]));
+  }
+  a = pack<T, VEC>(u);
+}
+
 // VEC: elements per access.  The interleaved layout turns VEC / 2 pairs per unit, the half layout VEC.
 // threadIdx: (unit, head lane, token lane); blockIdx: (tokens of a batch entry, batch entry).
 template <typename T, int VEC, bool HALF>
@@ -65,73 +127,54 @@ __global__ void __launch_bounds__(512, 3) rotary_kernel(const Params p) {
   const int at = rot ? u * VEC : p.R + (u - p.rot_units) * VEC;
   const int second = rot ? p.R >> 1 : (p.units - p.rot_units) * VEC;
   const bool two = HALF && at + second < p.D;
-  const T* xq = reinterpret_cast<const T*>(p.q.x) + b * p.q.sb + s * p.q.ss + at;
-  const T* xk = reinterpret_cast<const T*>(p.k.x) + b * p.k.sb + s * p.k.ss + at;
-  T* oq = reinterpret_cast<T*>(p.q.out) + (b * p.S + s) * p.q.H * p.D + at;
-  T* ok = reinterpret_cast<T*>(p.k.out) + (b * p.S + s) * p.k.H * p.D + at;
-  float c[NP], sn[NP];
+  Angles<VEC, HALF> w;
   if (rot) {
     if (l < 0 || l >= p.L) {
       // a position outside the table: the rotated features read NaN and the host learns of it
       atomicExch(&g_zib_err_word, (int)ZIB_ERR_INVALID_ARG);
+      const float nan = __uint_as_float(0x7FC00000u);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) c[i] = sn[i] = __uint_as_float(0x7FC00000u);
+      for (int i = 0; i < NP; ++i) w.set(i, nan, nan);
     } else {
       constexpr int FN = NP >= 4 ? 4 : NP;
       using F = Pack<float, FN>;
       const float* cp = p.cos + b * p.cs_b + l * p.cs_l + u * NP;
       const float* sp = p.sin + b * p.cs_b + l * p.cs_l + u * NP;
-      if (p.table_vec) {
 #pragma unroll
-        for (int i = 0; i < NP; i += FN) {
-          const F fc = *reinterpret_cast<const F*>(cp + i), fs = *reinterpret_cast<const F*>(sp + i);
+      for (int i = 0; i < NP; i += FN) {
+        F c, t;
+        if (p.table_vec) {
+          c = *reinterpret_cast<const F*>(cp + i);
+          t = *reinterpret_cast<const F*>(sp + i);
+        } else {
 #pragma unroll
           for (int j = 0; j < FN; ++j) {
-            c[i + j] = fc.v[j];
-            sn[i + j] = fs.v[j];
+            c.v[j] = cp[i + j];
+            t.v[j] = sp[i + j];
           }
         }
-      } else {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          c[i] = cp[i];
-          sn[i] = sp[i];
-        }
+        for (int j = 0; j < FN; ++j) w.set(i + j, c.v[j], p.sign * t.v[j]);
       }
-#pragma unroll
-      for (int i = 0; i < NP; ++i) sn[i] *= p.sign;
     }
   }
-  const int heads = p.q.H + p.k.H;
-  constexpr int U = HALF ? 1 : 2;  // heads in flight
-  for (int h0 = threadIdx.y; h0 < heads; h0 += U * blockDim.y) {
-    V a[U], d[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int h = h0 + i * blockDim.y;
-      if (h >= heads) break;
-      const T* x = h < p.q.H ? xq + h * p.q.sh : xk + (h - p.q.H) * p.k.sh;
-      a[i] = *reinterpret_cast<const V*>(x);
-      if constexpr (HALF) if (two) d[i] = *reinterpret_cast<const V*>(x + second);
+  // this thread's heads, of the queries and then of the keys, one count
+  int h = threadIdx.y;
+#pragma unroll 1
+  for (int t = 0; t < 2; ++t) {
+    const Heads& hd = t ? p.k : p.q;
+    const T* x = reinterpret_cast<const T*>(hd.x) + b * hd.sb + s * hd.ss + h * hd.sh + at;
+    T* o = reinterpret_cast<T*>(hd.out) + ((b * p.S + s) * hd.H + h) * p.D + at;
+    const int64_t xstep = blockDim.y * hd.sh, ostep = (int64_t)blockDim.y * p.D;
+#pragma unroll 2
+    for (; h < hd.H; h += blockDim.y, x += xstep, o += ostep) {
+      V a = load_vec<T, VEC>(x), d = a;
+      if constexpr (HALF) if (two) d = load_vec<T, VEC>(x + second);
+      if (rot) turn<T, VEC, HALF>(w, a, d);
+      *reinterpret_cast<V*>(o) = a;
+      if constexpr (HALF) if (two) *reinterpret_cast<V*>(o + second) = d;
     }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int h = h0 + i * blockDim.y;
-      if (h >= heads) break;
-      T* o = h < p.q.H ? oq + (int64_t)h * p.D : ok + (int64_t)(h - p.q.H) * p.D;
-      if (rot) {
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          T& ta = HALF ? a[i].v[j] : a[i].v[2 * j];
-          T& tb = HALF ? d[i].v[j] : a[i].v[2 * j + 1];
-          const float fa = to_f32(ta), fb = to_f32(tb);
-          ta = from_f32<T>(fmaf(fa, c[j], -(fb * sn[j])));
-          tb = from_f32<T>(fmaf(fb, c[j], fa * sn[j]));
-        }
-      }
-      *reinterpret_cast<V*>(o) = a[i];
-      if constexpr (HALF) if (two) *reinterpret_cast<V*>(o + second) = d[i];
-    }
+    h -= hd.H;
   }
 }
 

@@ -101,21 +101,26 @@ def _rotate(q, k, cos, sin, positions, half: int, inverse: int):
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, half):
+    def forward(ctx, q, k, cos, sin, positions, half, inverse):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.half = half
-        return _rotate(q, k, cos, sin, positions, half, 0)
+        ctx.conf = half, inverse
+        ctx.set_materialize_grads(False)
+        return _rotate(q, k, cos, sin, positions, half, inverse)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        cos, sin, positions = ctx.saved_tensors
-        dq = dq if ctx.needs_input_grad[0] else None
-        dk = dk if ctx.needs_input_grad[1] else None
-        if dq is None and dk is None:
-            return None, None, None, None, None, None
-        gq, gk = _rotate(dq, dk, cos, sin, positions, ctx.half, 1)
-        return gq, gk, None, None, None, None
+        if not ctx.needs_input_grad[0]:
+            dq = None
+        if not ctx.needs_input_grad[1]:
+            dk = None
+        gq = gk = None
+        if dq is not None or dk is not None:
+            cos, sin, positions = ctx.saved_tensors
+            half, inverse = ctx.conf
+            # the transposed map of a rotation is the rotation back, itself differentiable
+            run = _Rotary.apply if torch.is_grad_enabled() else _rotate
+            gq, gk = run(dq, dk, cos, sin, positions, half, 1 - inverse)
+        return gq, gk, None, None, None, None, None
 
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
@@ -176,5 +181,5 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin
         if cos.requires_grad or sin.requires_grad:
             raise ValueError("the tables of rotary_embed are constants: cos and sin must not require gradients")
         if q.requires_grad or (k is not None and k.requires_grad):
-            return _Rotary.apply(q, k, cos, sin, positions, half)
+            return _Rotary.apply(q, k, cos, sin, positions, half, 0)
     return _rotate(q, k, cos, sin, positions, half, 0)

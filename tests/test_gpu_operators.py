@@ -409,6 +409,26 @@ def test_rotary_gradient_only_of_keys_and_of_expanded_outputs(cuda):
     check(dk, ref, 2 * U32 * mag)
 
 
+def test_second_derivatives(cuda):
+    """A rotation's gradient is a rotation and differentiable again; the others refuse."""
+    g = _gen(6)
+    q = _randn(g, 1, 5, 2, 32).requires_grad_()
+    k = _randn(g, 1, 5, 1, 32).requires_grad_()
+    d = _randn(g, 1, 5, 2, 32).requires_grad_()
+    e = _randn(g, 1, 5, 2, 32)
+    cos, sin = table(5, 16)
+    o, _ = rotary_embed(q, k, cos, sin, layout="half")
+    (gq,) = torch.autograd.grad(o, (q,), d, create_graph=True)
+    (gd,) = torch.autograd.grad(gq, (d,), e)
+    ref, mag = ref_rotary(e, cos[None], sin[None], "half")
+    check(gd, ref, 2 * U32 * mag)
+    x = _randn(g, 4, 9, 32).requires_grad_()
+    wq, ws = fp8_block_quantize_weight(_randn(g, 16, 32))
+    for y in (group_norm_act(x, 4), fp8_block_linear(x, wq, ws)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), (x,), create_graph=True)
+
+
 def test_rotary_shared_key_gradient_through_expanded_heads(cuda):
     """A key head shared by four query heads (expanded view): its gradient is the sum over them."""
     g = _gen(4)
