@@ -148,6 +148,25 @@ struct Slab {
 
 // --- forward statistics --------------------------------------------------------------
 
+// Sums by group, several threads to a group (as many as the CTA has, a power of two up to 32):
+// part(g, first, step) is a thread's share, done(g, sum) gets the sum in one thread of the group.
+// part is also called for g >= G, where it returns 0.
+template <typename Part, typename Done>
+__device__ __forceinline__ void by_group(int G, Part part, Done done) {
+  int n = 32;
+  while (n > 1 && n * G > (int)blockDim.x) n >>= 1;
+  const int per_pass = (int)blockDim.x / n, lane = (int)threadIdx.x % n;
+  for (int g0 = 0; g0 < G; g0 += per_pass) {
+    const int g = g0 + (int)threadIdx.x / n;
+    double2 d = part(g, lane, n);
+    for (int o = n >> 1; o > 0; o >>= 1) {
+      d.x += __shfl_xor_sync(0xFFFFFFFFu, d.x, o);
+      d.y += __shfl_xor_sync(0xFFFFFFFFu, d.y, o);
+    }
+    if (lane == 0 && g < G) done(g, d);
+  }
+}
+
 // The sums of this CTA's pixels by group into sm[0 .. G) (sum x, sum x^2); scratch behind them.  GV
 // consecutive channels of a thread share a group; RUN pixels are in flight at a time.
 template <typename T, int VEC, int GV>
@@ -169,18 +188,7 @@ __device__ __forceinline__ void slab_stats(const Params& p, const Slab& s, doubl
       }
       const T* xv = x + (int64_t)v * VEC;
       const int64_t p0 = s.p0 + s.r, step = p.rows * p.xsp;
-      if (p0 < s.p1) {
-        const V t = *reinterpret_cast<const V*>(xv + p0 * p.xsp);
-#pragma unroll
-        for (int a = 0; a < NA; ++a) {
-#pragma unroll
-          for (int j = 0; j < GV; ++j) piv[a] += to_f32(t.v[a * GV + j]);
-          piv[a] *= 1.0f / GV;
-        }
-      }
       f2 pv[NP];
-#pragma unroll
-      for (int i = 0; i < NP; ++i) pv[i] = VEC == 1 ? px::mk(piv[0], 0.0f) : px::mk(piv[2 * i / GV], piv[(2 * i + 1) / GV % NA]);
       const int n = s.p1 > p0 ? (int)((s.p1 - p0 + p.rows - 1) / p.rows) : 0;  // this thread's pixels
       const T* at = xv + p0 * p.xsp;
       for (int i = 0; i < n; i += RUN, at += RUN * step) {
@@ -188,6 +196,17 @@ __device__ __forceinline__ void slab_stats(const Params& p, const Slab& s, doubl
 #pragma unroll
         for (int k = 0; k < RUN; ++k)
           if (i + k < n) t[k] = *reinterpret_cast<const V*>(at + k * step);
+        if (i == 0) {
+#pragma unroll
+          for (int a = 0; a < NA; ++a) {
+#pragma unroll
+            for (int j = 0; j < GV; ++j) piv[a] += to_f32(t[0].v[a * GV + j]);
+            piv[a] *= 1.0f / GV;
+          }
+#pragma unroll
+          for (int j = 0; j < NP; ++j)
+            pv[j] = VEC == 1 ? px::mk(piv[0], 0.0f) : px::mk(piv[2 * j / GV], piv[(2 * j + 1) / GV % NA]);
+        }
         f2 u[NP], w[NP];
 #pragma unroll
         for (int j = 0; j < NP; ++j) u[j] = w[j] = 0ull;
@@ -230,18 +249,17 @@ __device__ __forceinline__ void slab_stats(const Params& p, const Slab& s, doubl
   }
   if (scratch == sm) return;
   __syncthreads();
-  // a warp per group: its columns of every thread row, in a fixed order
-  for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
+  // the group's columns of every thread row, in a fixed order
+  by_group(p.G, [&](int g, int first, int step) {
     double a = 0.0, q = 0.0;
-    for (int k = threadIdx.x & 31; k < cols * p.rows; k += 32) {
-      const double2 d = scratch[(k / cols) * p.V * NA + g * cols + k % cols];
-      a += d.x;
-      q += d.y;
-    }
-    a = warp_sum(a);
-    q = warp_sum(q);
-    if ((threadIdx.x & 31) == 0) sm[g] = make_double2(a, q);
-  }
+    if (g < p.G)
+      for (int k = first; k < cols * p.rows; k += step) {
+        const double2 d = scratch[(k / cols) * p.V * NA + g * cols + k % cols];
+        a += d.x;
+        q += d.y;
+      }
+    return make_double2(a, q);
+  }, [&](int g, double2 d) { sm[g] = d; });
 }
 
 // the cluster's sum of element g of an array that each of its CTAs holds
@@ -267,15 +285,25 @@ __device__ __forceinline__ void finish(const Params& p, double s, double q, floa
   rstd = (float)(1.0 / sqrt(var + (double)p.eps));
 }
 
-// element g of the clusters' sums of batch entry b, added by a warp in a fixed order
-__device__ __forceinline__ double2 sum_clusters(const Params& p, int64_t b, int g) {
+// a thread's share of the clusters' sums of group g of batch entry b
+__device__ __forceinline__ double2 cluster_share(const Params& p, int64_t b, int g, int first, int step) {
   double s = 0.0, q = 0.0;
-  for (int k = threadIdx.x & 31; k < p.clusters; k += 32) {
-    const double2 d = __ldcg(p.gpart + (b * p.clusters + k) * p.G + g);
-    s += d.x;
-    q += d.y;
+  if (g < p.G) {
+    const double2* at = p.gpart + b * p.clusters * p.G + g;
+#pragma unroll 8
+    for (int k = first; k < p.clusters; k += step) {
+      const double2 d = __ldcg(at + (int64_t)k * p.G);
+      s += d.x;
+      q += d.y;
+    }
   }
-  return make_double2(warp_sum(s), warp_sum(q));
+  return make_double2(s, q);
+}
+
+// the same by a whole warp
+__device__ __forceinline__ double2 sum_clusters(const Params& p, int64_t b, int g) {
+  const double2 d = cluster_share(p, b, g, threadIdx.x & 31, 32);
+  return make_double2(warp_sum(d.x), warp_sum(d.y));
 }
 
 // --- outputs -----------------------------------------------------------------------
@@ -388,25 +416,33 @@ __global__ void __launch_bounds__(256) finish_stats_kernel(const Params p) {
   allow_dependents();
 }
 
+// half of a chunk of the first pass: the CTAs that start first take the second halves, read last
+__device__ __forceinline__ Slab second_pass_slab(const Params& p) {
+  const bool tail = (int)blockIdx.x < p.chunks;
+  Slab s(p, tail ? blockIdx.x : blockIdx.x - p.chunks);
+  const int64_t mid = s.p0 + (s.p1 - s.p0) / 2;
+  if (tail) s.p0 = mid;
+  else s.p1 = mid;
+  return s;
+}
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, 4) apply_kernel(const Params p) {
   __shared__ float mean[kDirectGroups], rstd[kDirectGroups];
-  const Slab s(p, blockIdx.x);
+  const Slab s = second_pass_slab(p);
   wait_for_primary();
   if (!p.direct) {
     slab_apply<T, VEC>(p, s, p.mean + s.b * p.G, p.rstd + s.b * p.G);
     return;
   }
-  for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
-    const double2 d = sum_clusters(p, s.b, g);
-    if ((threadIdx.x & 31) == 0) {
-      finish(p, d.x, d.y, mean[g], rstd[g]);
-      if (blockIdx.x == 0) {
-        p.mean[s.b * p.G + g] = mean[g];
-        p.rstd[s.b * p.G + g] = rstd[g];
-      }
-    }
-  }
+  by_group(p.G, [&](int g, int first, int step) { return cluster_share(p, s.b, g, first, step); },
+           [&](int g, double2 d) {
+             finish(p, d.x, d.y, mean[g], rstd[g]);
+             if (blockIdx.x == 0) {
+               p.mean[s.b * p.G + g] = mean[g];
+               p.rstd[s.b * p.G + g] = rstd[g];
+             }
+           });
   __syncthreads();
   slab_apply<T, VEC>(p, s, mean, rstd);
 }
@@ -619,23 +655,21 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, 3) grad_apply_kernel(const Params p) {
   __shared__ float2 coef[kDirectGroups];
   wait_for_primary();
-  if ((int)blockIdx.x >= p.chunks) {
+  if ((int)blockIdx.x >= 2 * p.chunks) {
     if (blockIdx.y == 0) {
       const int warps = (int)blockDim.x >> 5;
-      param_grads(p, ((int)blockIdx.x - p.chunks) * warps, ((int)gridDim.x - p.chunks) * warps);
+      param_grads(p, ((int)blockIdx.x - 2 * p.chunks) * warps, ((int)gridDim.x - 2 * p.chunks) * warps);
     }
     return;
   }
-  const Slab s(p, blockIdx.x);
+  const Slab s = second_pass_slab(p);
   if (!p.direct) {
     slab_grad_apply<T, VEC>(p, s, p.coef + s.b * p.G);
     return;
   }
   const double n = (double)p.P * (double)p.cpg;
-  for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
-    const double2 t = sum_clusters(p, s.b, g);
-    if ((threadIdx.x & 31) == 0) coef[g] = make_float2((float)(t.x / n), (float)(t.y / n));
-  }
+  by_group(p.G, [&](int g, int first, int step) { return cluster_share(p, s.b, g, first, step); },
+           [&](int g, double2 d) { coef[g] = make_float2((float)(d.x / n), (float)(d.y / n)); });
   __syncthreads();
   slab_grad_apply<T, VEC>(p, s, coef);
 }
@@ -647,7 +681,7 @@ static int gcd(int a, int b) {
   return a;
 }
 
-// clusters per batch entry: four CTAs per SM in all, at most one per 8 pixels
+// clusters per batch entry, at most: four CTAs per SM in all, one cluster per 8 pixels and CTA
 static int64_t most_clusters(int64_t B, int64_t P) {
   if (B < 1 || P < 1) return 1;
   int64_t c = (int64_t)sm_count() * 4 / (kCluster * B);
@@ -665,12 +699,39 @@ struct Plan {
   unsigned threads;
 };
 
-static Plan plan(Params& p, int vec, int size) {
+// clusters of `kernel` that run at once on the current device (asked for once per device)
+static int resident_clusters(void (*kernel)(Params), unsigned threads, size_t smem, int (&known)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count() * 2 / kCluster;
+  if (known[dev] == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kCluster * 64);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = kCluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = sm_count() * 2 / kCluster;
+    }
+    known[dev] = n;
+  }
+  return known[dev];
+}
+
+// `resident`: clusters of the first pass that run at once, so that it runs in one wave
+static Plan plan(Params& p, int vec, int size, int resident) {
   p.V = p.C / vec;
   p.vlanes = p.V < kThreads ? p.V : kThreads;
   p.rows = kThreads / p.vlanes;
   const bool fused = p.P * p.C * size <= kFusedBytes;
   int64_t clusters = fused ? 1 : most_clusters(p.B, p.P);
+  if (clusters * p.B > resident) clusters = resident / p.B > 0 ? resident / p.B : 1;
   // at least 16 pixels per thread row, so that runs fill
   const int64_t most = ceil_div(p.P, (int64_t)kCluster * p.rows * 16);
   if (clusters > most) clusters = most;
@@ -722,7 +783,8 @@ static int launch(void (*kernel)(Params), dim3 grid, unsigned threads, size_t sm
 template <typename T, int VEC, int GV>
 static int forward_g(Params& p, cudaStream_t st) {
   const char* what = "zib_group_norm";
-  const Plan pl = plan(p, VEC, sizeof(T));
+  static int known[64];
+  const Plan pl = plan(p, VEC, sizeof(T), resident_clusters(stats_kernel<T, VEC, GV, false>, kThreads, 24 * 1024, known));
   const size_t sums = (size_t)p.rows * p.V * (VEC / GV);
   size_t smem = ((p.cpg / GV * p.rows == 1 ? 0 : (size_t)p.G) + sums) * sizeof(double2);
   const size_t stats = (size_t)p.G * (sizeof(double2) + 2 * sizeof(float));
@@ -733,7 +795,7 @@ static int forward_g(Params& p, cudaStream_t st) {
   int rc = launch(stats_kernel<T, VEC, GV, false>, grid, pl.threads, smem, kCluster, false, p, st, what);
   if (!rc && !p.direct)
     rc = launch(finish_stats_kernel, dim3((unsigned)ceil_div(p.B * p.G, 8)), 256, 0, 0, true, p, st, what);
-  if (!rc) rc = launch(apply_kernel<T, VEC>, grid, pl.threads, 0, 0, true, p, st, what);
+  if (!rc) rc = launch(apply_kernel<T, VEC>, dim3(2 * p.chunks, (unsigned)p.B), pl.threads, 0, 0, true, p, st, what);
   return rc;
 }
 
@@ -749,7 +811,9 @@ static int forward_v(Params& p, cudaStream_t st) {
 template <typename T, int VEC>
 static int backward_v(Params& p, cudaStream_t st) {
   const char* what = "zib_group_norm_backward";
-  const Plan pl = plan(p, VEC, 2 * sizeof(T));  // x and dy
+  static int known[64];
+  const Plan pl = plan(p, VEC, 2 * sizeof(T),  // x and dy
+                       resident_clusters(grad_stats_kernel<T, VEC, false>, kThreads, 24 * 1024, known));
   size_t smem = ((size_t)p.C + (size_t)p.rows * p.vlanes * VEC) * sizeof(float2);
   const size_t sums = ((size_t)2 * p.C + p.G) * sizeof(float2);
   if (smem < sums) smem = sums;
@@ -768,7 +832,7 @@ static int backward_v(Params& p, cudaStream_t st) {
     rc = launch(finish_grad_kernel, dim3((unsigned)ceil_div(p.B * p.G, 8)), 256, 0, 0, true, p, st, what);
   const unsigned extra = params ? (unsigned)ceil_div(p.C, (int64_t)pl.threads / 32) : 0;
   if (!rc)
-    rc = launch(grad_apply_kernel<T, VEC>, dim3(p.chunks + extra, (unsigned)p.B), pl.threads, 0, 0, true, p, st, what);
+    rc = launch(grad_apply_kernel<T, VEC>, dim3(2 * p.chunks + extra, (unsigned)p.B), pl.threads, 0, 0, true, p, st, what);
   return rc;
 }
 

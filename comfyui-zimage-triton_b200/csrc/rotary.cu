@@ -13,7 +13,7 @@
 // unit are read once for a few heads: the fp32 table would otherwise be as many bytes as the data.
 // A thread's chain is long (position, table row, data), so what hides it is many threads: more loads
 // per thread at the price of registers (four heads in flight, 25 to 37% occupancy) measured slower,
-// 97 instead of TBD us for [2, 4608, 30 + 30, 128].
+// 97 instead of 62 us for [2, 4608, 30 + 30, 128].
 #include "zib_async.cuh"
 #include "zib_pairs.cuh"
 
@@ -110,16 +110,17 @@ __device__ __forceinline__ void turn(const Angles<VEC, HALF>& w, Pack<T, VEC>& a
 
 // VEC: elements per access.  The interleaved layout turns VEC / 2 pairs per unit, the half layout VEC.
 // threadIdx: (unit, head lane, token lane); blockIdx: (tokens of a batch entry, batch entry).
-template <typename T, int VEC, bool HALF>
+// ONE: one token lane, so that a token's addresses, position and table row are the block's.
+template <typename T, int VEC, bool HALF, bool ONE>
 __global__ void __launch_bounds__(512, 3) rotary_kernel(const Params p) {
   using V = Pack<T, VEC>;
   constexpr int NP = HALF ? VEC : VEC / 2;  // pairs per unit
   const int u = threadIdx.x;
-  const int64_t s = (int64_t)blockIdx.x * blockDim.z + threadIdx.z, b = blockIdx.y;
-  if (s >= p.S) return;
+  const int64_t s = ONE ? blockIdx.x : (int64_t)blockIdx.x * blockDim.z + threadIdx.z, b = blockIdx.y;
+  if (!ONE && s >= p.S) return;
   const bool rot = u < p.rot_units;
   int64_t l = s;
-  if (p.pos && rot) {
+  if (p.pos) {
     const int64_t i = b * p.ps_b + s * p.ps_s;
     l = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[i] : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[i];
   }
@@ -160,12 +161,10 @@ __global__ void __launch_bounds__(512, 3) rotary_kernel(const Params p) {
   }
   // this thread's heads, of the queries and then of the keys, one count
   int h = threadIdx.y;
-#pragma unroll 1
-  for (int t = 0; t < 2; ++t) {
-    const Heads& hd = t ? p.k : p.q;
-    const T* x = reinterpret_cast<const T*>(hd.x) + b * hd.sb + s * hd.ss + h * hd.sh + at;
-    T* o = reinterpret_cast<T*>(hd.out) + ((b * p.S + s) * hd.H + h) * p.D + at;
-    const int64_t xstep = blockDim.y * hd.sh, ostep = (int64_t)blockDim.y * p.D;
+  auto walk = [&](const Heads& hd) {
+    const T* x = reinterpret_cast<const T*>(hd.x) + (b * hd.sb + s * hd.ss) + (h * hd.sh + at);
+    T* o = reinterpret_cast<T*>(hd.out) + (b * p.S + s) * ((int64_t)hd.H * p.D) + (h * p.D + at);
+    const int64_t xstep = blockDim.y * hd.sh, ostep = blockDim.y * p.D;
 #pragma unroll 2
     for (; h < hd.H; h += blockDim.y, x += xstep, o += ostep) {
       V a = load_vec<T, VEC>(x), d = a;
@@ -175,17 +174,25 @@ __global__ void __launch_bounds__(512, 3) rotary_kernel(const Params p) {
       if constexpr (HALF) if (two) *reinterpret_cast<V*>(o + second) = d;
     }
     h -= hd.H;
-  }
+  };
+  walk(p.q);
+  walk(p.k);
+}
+
+template <typename T, int VEC, bool HALF>
+static void launch_vec(dim3 grid, dim3 threads, const Params& p, cudaStream_t st) {
+  if (threads.z == 1) rotary_kernel<T, VEC, HALF, true><<<grid, threads, 0, st>>>(p);
+  else rotary_kernel<T, VEC, HALF, false><<<grid, threads, 0, st>>>(p);
 }
 
 template <typename T, bool HALF>
 static void launch(int vec, dim3 grid, dim3 threads, const Params& p, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    if (vec == 8) { rotary_kernel<T, 8, HALF><<<grid, threads, 0, st>>>(p); return; }
+    if (vec == 8) { launch_vec<T, 8, HALF>(grid, threads, p, st); return; }
   }
-  if (vec == 4) { rotary_kernel<T, 4, HALF><<<grid, threads, 0, st>>>(p); return; }
-  if (vec == 2) { rotary_kernel<T, 2, HALF><<<grid, threads, 0, st>>>(p); return; }
-  if constexpr (HALF) rotary_kernel<T, 1, HALF><<<grid, threads, 0, st>>>(p);
+  if (vec == 4) { launch_vec<T, 4, HALF>(grid, threads, p, st); return; }
+  if (vec == 2) { launch_vec<T, 2, HALF>(grid, threads, p, st); return; }
+  if constexpr (HALF) launch_vec<T, 1, HALF>(grid, threads, p, st);
 }
 
 // --- tables ------------------------------------------------------------------------
@@ -203,28 +210,56 @@ struct TableParams {
   float* sin;
 };
 
+// cos and sin of an angle in fixed point, 2^-32 turns: its nearest multiple of a quarter turn decides
+// which of them is which and their signs, exactly, in integers; the rest, within an eighth of a turn
+// and rounded once to fp32, goes through the Taylor series of sine (to x^9) and cosine (to x^10), whose
+// next terms are below 2e-9 and 2e-10 there.
+__device__ __forceinline__ void sincos_turns(uint32_t a, float& s, float& c) {
+  const uint32_t quarter = (a + 0x20000000u) >> 30;
+  const float x = (float)(int32_t)(a - (quarter << 30)) * 1.4629180792671596e-09f;  // 2 pi / 2^32
+  const float x2 = x * x;
+  float ps = 2.7557319e-6f;  // 1 / 9!
+  ps = fmaf(ps, x2, -1.9841270e-4f);
+  ps = fmaf(ps, x2, 8.3333333e-3f);
+  ps = fmaf(ps, x2, -1.6666667e-1f);
+  ps = fmaf(ps * x2, x, x);
+  float pc = -2.7557319e-7f;  // -1 / 10!
+  pc = fmaf(pc, x2, 2.4801587e-5f);
+  pc = fmaf(pc, x2, -1.3888889e-3f);
+  pc = fmaf(pc, x2, 4.1666667e-2f);
+  pc = fmaf(pc, x2, -0.5f);
+  pc = fmaf(pc, x2, 1.0f);
+  const float u = quarter & 1 ? pc : ps, v = quarter & 1 ? ps : pc;
+  s = __uint_as_float(__float_as_uint(u) ^ ((quarter & 2) << 30));
+  c = __uint_as_float(__float_as_uint(v) ^ (((quarter + 1) & 2) << 30));
+}
+
 // cos and sin of p f_j, f_j = theta^(-2j/dim) scaled.  The angle is formed in turns, in fixed point of
 // 64 bits: a whole position times a frequency, modulo whole turns, is one wrapping 64-bit product (the
 // frequency is rounded to 2^-64 turns, so a position below 2^31 is off by less than 2^-33 turns; the
-// fp64 frequency behind it by less than 2^-55 turns a position).  The upper 32 bits of the signed rest
-// split into an fp32 value and a correction d for the first-order step cos(x + d) = cos x - d sin x,
-// so each entry is within about 2 ulp.  A thread keeps one frequency and walks over positions, so the
-// fp64 exp is paid once per thread.  Forming the angle in fp64 instead, with its conversions, measured
-// 28 us at 131072 x 64.
+// fp64 frequency behind it by less than 2^-55 turns a position).  A thread keeps J neighbouring
+// frequencies and walks over positions, so the fp64 exp is paid once per thread.
+// 131072 x 64 (68 MB, 10.4 us at HBM's rate): TBD us; angles in fp64 28 us, sincospi of the fixed-point
+// angle 26 us, both short of issue slots.
+template <int J>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) {
-  const int j = blockIdx.y * blockDim.x + threadIdx.x;
-  if (j >= p.half) return;
-  double f = exp(-p.log_theta * (double)j / (double)p.half);
-  if (p.kind == ZIB_ROTARY_LINEAR) f *= p.inv_factor;
-  if (p.kind == ZIB_ROTARY_YARN) {
-    // whole turns over the original length: few turns are interpolated, many are kept
-    const double turns = p.original * f * 0.15915494309189535;
-    const double keep = fmin(1.0, fmax(0.0, (turns - p.beta_slow) / (p.beta_fast - p.beta_slow)));
-    f = (1.0 - keep) * f * p.inv_factor + keep * f;
+  const int j0 = (blockIdx.y * blockDim.x + threadIdx.x) * J;
+  if (j0 >= p.half) return;
+  uint64_t turns[J];
+#pragma unroll
+  for (int i = 0; i < J; ++i) {
+    double f = exp(-p.log_theta * (double)(j0 + i) / (double)p.half);
+    if (p.kind == ZIB_ROTARY_LINEAR) f *= p.inv_factor;
+    if (p.kind == ZIB_ROTARY_YARN) {
+      // whole turns over the original length: few turns are interpolated, many are kept
+      const double over = p.original * f * 0.15915494309189535;
+      const double keep = fmin(1.0, fmax(0.0, (over - p.beta_slow) / (p.beta_fast - p.beta_slow)));
+      f = (1.0 - keep) * f * p.inv_factor + keep * f;
+    }
+    double ft = f * 0.15915494309189535;  // turns per position; whole ones do not matter
+    ft -= floor(ft);
+    turns[i] = (uint64_t)(ft * 18446744073709551616.0);
   }
-  double ft = f * 0.15915494309189535;  // turns per position; whole ones do not matter
-  ft -= floor(ft);
-  const uint64_t step_turns = (uint64_t)(ft * 18446744073709551616.0);
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
 #pragma unroll 4
   for (int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; t < p.T; t += step) {
@@ -232,14 +267,17 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) 
     if (p.pos)
       pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[t * p.ps]
                     : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[t * p.ps];
-    const int32_t a = (int32_t)(((uint64_t)pos * step_turns) >> 32);  // 2^-32 turns, in [-1/2, 1/2)
-    const float hi = (float)a;
-    // the rest of a below hi; a + 128 may round up to 2^31, which a float holds and an int does not
-    const float d = (float)(int32_t)((uint32_t)a - (uint32_t)(int64_t)hi) * 1.4629180792671596e-09f;  // 2 pi / 2^32
-    float s, c;
-    sincospif(hi * 4.656612873077393e-10f, &s, &c);  // 2 / 2^32: angle / pi
-    p.cos[t * p.half + j] = p.mscale * fmaf(-d, s, c);
-    p.sin[t * p.half + j] = p.mscale * fmaf(d, c, s);
+    Pack<float, J> c, s;
+#pragma unroll
+    for (int i = 0; i < J; ++i) {
+      float sv, cv;
+      // the nearest 2^-32 turns of the 64-bit product
+      sincos_turns((uint32_t)(((uint64_t)pos * turns[i] + 0x80000000ull) >> 32), sv, cv);
+      c.v[i] = p.mscale * cv;
+      s.v[i] = p.mscale * sv;
+    }
+    *reinterpret_cast<Pack<float, J>*>(p.cos + t * p.half + j0) = c;
+    *reinterpret_cast<Pack<float, J>*>(p.sin + t * p.half + j0) = s;
   }
 }
 
@@ -292,17 +330,20 @@ extern "C" int zib_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_s
   p.sign = inverse ? -1.0f : 1.0f;
   const int np = half_layout ? vec : vec / 2, fn = np >= 4 ? 4 : np;
   p.table_vec = ((uintptr_t)cos % (4 * fn) == 0 && (uintptr_t)sin % (4 * fn) == 0 && cs_l % fn == 0 && cs_b % fn == 0);
-  // heads per thread: one where the tokens alone do not fill the SMs (latency), else up to four
+  // Heads per thread: one where the tokens alone do not fill the SMs (latency); else as many, up to 16,
+  // as leave about 64 threads to a token, which pays for a token's addresses and table row over more
+  // heads (256 / 128 / 64 / 32 threads a token: 64 / 59 / 59 / 67 us for [2, 4608, 30 + 30, 128]
+  // interleaved, 72 / 64 / 55 / 57 us for [16383, 24 + 6, 128] half, 64 of 128 features).
   const int64_t heads = Hq + Hk;
   int64_t per = 1;
   if (B * S >= 4 * sm_count()) {
-    per = (heads * p.units + 128) / 256;
+    per = (heads * p.units + 32) / 64;
     if (per < 1) per = 1;
-    if (per > 4) per = 4;
+    if (per > 16) per = 16;
   }
   int64_t lanes = ceil_div(heads, per);
   if (lanes * p.units > 512) lanes = 512 / p.units;  // units <= 512: a unit has two features at least
-  int64_t tokens = 256 / (p.units * lanes);
+  int64_t tokens = 128 / (p.units * lanes);
   if (tokens > S) tokens = S;
   if (tokens > 64) tokens = 64;
   if (tokens < 1) tokens = 1;
@@ -352,12 +393,16 @@ extern "C" int zib_rotary_table(const void* positions, int pos64, int64_t ps, in
   p.original = original; p.beta_fast = beta_fast; p.beta_slow = beta_slow;
   p.mscale = scaling == ZIB_ROTARY_YARN ? (float)attention_factor : 1.0f;
   p.cos = cos; p.sin = sin;
-  const int bx = p.half >= 64 ? 64 : 32;
+  const bool two = p.half % 2 == 0 && (uintptr_t)cos % 8 == 0 && (uintptr_t)sin % 8 == 0;
+  const int cols = two ? p.half / 2 : p.half;
+  const int bx = cols > 16 ? 32 : 16;
   dim3 block(bx, 256 / bx);
-  const int64_t gy = ceil_div(p.half, bx);
+  const int64_t gy = ceil_div(cols, bx);
   int64_t gx = ceil_div(T, (int64_t)block.y * 4);
   const int64_t cap = ceil_div((int64_t)sm_count() * 8, gy);
   if (gx > cap) gx = cap;
-  rotary::rotary_table_kernel<<<dim3((unsigned)gx, (unsigned)gy), block, 0, (cudaStream_t)stream>>>(p);
+  const dim3 grid((unsigned)gx, (unsigned)gy);
+  if (two) rotary::rotary_table_kernel<2><<<grid, block, 0, (cudaStream_t)stream>>>(p);
+  else rotary::rotary_table_kernel<1><<<grid, block, 0, (cudaStream_t)stream>>>(p);
   return zib_check_launch(what);
 }
