@@ -308,27 +308,68 @@ __device__ __forceinline__ double2 sum_clusters(const Params& p, int64_t b, int 
 
 // --- outputs -----------------------------------------------------------------------
 
+// N consecutive parameters from element c on, `missing` where there are none.  One branch on the type
+// for all of them, so that the loads go out together (a branch per element, 16 loads one after the
+// other, cost 5 us a launch).
+template <int N, typename T>
+__device__ __forceinline__ void load_typed(const T* p, float (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = to_f32(p[j]);
+}
+template <int N>
+__device__ __forceinline__ void load_params(const void* p, int dtype, int c, float missing, float (&v)[N]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = missing;
+  } else if (dtype == ZIB_F32) {
+    load_typed<N>(reinterpret_cast<const float*>(p) + c, v);
+  } else if (dtype == ZIB_BF16) {
+    load_typed<N>(reinterpret_cast<const __nv_bfloat16*>(p) + c, v);
+  } else {
+    load_typed<N>(reinterpret_cast<const __half*>(p) + c, v);
+  }
+}
+
+// the group of each of VEC channels from c0 on
+template <int VEC>
+__device__ __forceinline__ void groups_of(const Params& p, int c0, int (&g)[VEC]) {
+  g[0] = c0 / p.cpg;
+  int left = p.cpg - (c0 - g[0] * p.cpg);  // channels of that group from c0 on
+#pragma unroll
+  for (int j = 1; j < VEC; ++j) {
+    const bool next = --left == 0;
+    g[j] = g[j - 1] + (next ? 1 : 0);
+    if (next) left = p.cpg;
+  }
+}
+
 // mean, 1 / sqrt(var + eps), weight and bias of VEC channels from channel c0; mean and rstd by group
 template <int VEC>
 struct Affine {
   f2 mu[kPairs<VEC>], r[kPairs<VEC>], w[kPairs<VEC>], b[kPairs<VEC>];
-  __device__ __forceinline__ void load(const Params& p, const float* mean, const float* rstd, int c0) {
+  __device__ __forceinline__ void load_params_of(const Params& p, int c0) {
+    float wv[VEC], bv[VEC];
+    load_params<VEC>(p.w, p.wdtype, c0, 1.0f, wv);
+    load_params<VEC>(p.b, p.wdtype, c0, 0.0f, bv);
 #pragma unroll
     for (int i = 0; i < kPairs<VEC>; ++i) {
-      float m[2] = {0.0f, 0.0f}, q[2] = {0.0f, 0.0f}, v[2] = {0.0f, 0.0f}, a[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int j = 0; j < (VEC == 1 ? 1 : 2); ++j) {
-        const int c = c0 + 2 * i + j, g = c / p.cpg;
-        m[j] = mean[g];
-        q[j] = rstd[g];
-        v[j] = p.w ? load_as_f32(p.w, p.wdtype, c) : 1.0f;
-        a[j] = p.b ? load_as_f32(p.b, p.wdtype, c) : 0.0f;
-      }
-      mu[i] = px::mk(m[0], m[1]);
-      r[i] = px::mk(q[0], q[1]);
-      w[i] = px::mk(v[0], v[1]);
-      b[i] = px::mk(a[0], a[1]);
+      w[i] = px::mk(wv[2 * i], VEC == 1 ? 0.0f : wv[(2 * i + 1) % VEC]);
+      b[i] = px::mk(bv[2 * i], VEC == 1 ? 0.0f : bv[(2 * i + 1) % VEC]);
     }
+  }
+  __device__ __forceinline__ void load_stats_of(const Params& p, const float* mean, const float* rstd, int c0) {
+    int g[VEC];
+    groups_of<VEC>(p, c0, g);
+#pragma unroll
+    for (int i = 0; i < kPairs<VEC>; ++i) {
+      const int h = VEC == 1 ? g[0] : g[(2 * i + 1) % VEC];
+      mu[i] = px::mk(mean[g[2 * i]], VEC == 1 ? 0.0f : mean[h]);
+      r[i] = px::mk(rstd[g[2 * i]], VEC == 1 ? 0.0f : rstd[h]);
+    }
+  }
+  __device__ __forceinline__ void load(const Params& p, const float* mean, const float* rstd, int c0) {
+    load_params_of(p, c0);
+    load_stats_of(p, mean, rstd, c0);
   }
 };
 
@@ -529,9 +570,11 @@ __device__ __forceinline__ void slab_grad_apply(const Params& p, const Slab& s, 
     Affine<VEC> f;
     f.load(p, p.mean + s.b * p.G, p.rstd + s.b * p.G, v * VEC);
     f2 c1[NP], c2[NP];
+    int g[VEC];
+    groups_of<VEC>(p, v * VEC, g);
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const float2 a = coef[(v * VEC + 2 * j) / p.cpg], b = VEC == 1 ? a : coef[(v * VEC + 2 * j + 1) / p.cpg];
+      const float2 a = coef[g[2 * j]], b = coef[VEC == 1 ? g[0] : g[(2 * j + 1) % VEC]];
       c1[j] = px::mk(-a.x, -b.x);
       c2[j] = px::mk(-a.y, -b.y);
     }
