@@ -20,7 +20,7 @@
 // between the two does that once).  Dependent launches start early and wait for the one before them.
 //
 // Sums.  A thread subtracts a value of its own group first (the mean of its first pixel's channels),
-// adds the differences and their squares in fp32 over 8 pixels and joins them in fp64, so a mean that
+// adds the differences and their squares in fp32 over 16 pixels at most and joins them in fp64, so a mean that
 // is large against the spread costs no precision.  All sums have a fixed order (no atomics).
 //
 // Arithmetic is on packed pairs (f32x2): at 12 elements per clock and SM, the rate of HBM, single
@@ -171,7 +171,7 @@ __device__ __forceinline__ void by_group(int G, Part part, Done done) {
 // consecutive channels of a thread share a group; RUN pixels are in flight at a time.
 template <typename T, int VEC, int GV>
 __device__ __forceinline__ void slab_stats(const Params& p, const Slab& s, double2* sm) {
-  constexpr int NA = VEC / GV, NP = kPairs<VEC>, RUN = NA > 2 ? 4 : 8;
+  constexpr int NA = VEC / GV, NP = kPairs<VEC>, RUN = NA > 2 ? 8 : 16;
   using V = Pack<T, VEC>;
   const int cols = p.cpg / GV;  // sums per group and thread row
   // [rows][V * NA]; with one sum per group it is the result
@@ -409,7 +409,7 @@ __device__ __forceinline__ void slab_apply(const Params& p, const Slab& s, const
 
 // FUSED: one cluster per batch entry, outputs included; else the clusters' sums to memory
 template <typename T, int VEC, int GV, bool FUSED>
-__global__ void __launch_bounds__(kThreads, 3) stats_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) stats_kernel(const Params p) {
   extern __shared__ double2 sm[];  // [G], then scratch
   const Slab s(p, blockIdx.x);
   slab_stats<T, VEC, GV>(p, s, sm);
