@@ -26,6 +26,7 @@ from .kernels import (  # noqa: E402
 )
 from .patching import apply_triton_kernels_comfyui  # noqa: E402
 from .quantization import (  # noqa: E402
+    Fp8BlockLinear,
     apply_int8_quantization,
     fp8_block_linear,
     fp8_block_matmul,
@@ -53,6 +54,7 @@ __all__ = [
     "fp8_block_transpose",
     "fp8_block_matmul",
     "fp8_block_linear",
+    "Fp8BlockLinear",
     "rotary_embed",
     "rotary_table",
     "group_norm_act",

@@ -10,6 +10,7 @@ RuntimeError for oversize rows, ``kernels/utils.py:33-37``).
 from __future__ import annotations
 
 import ctypes
+import importlib
 import threading
 from pathlib import Path
 
@@ -88,9 +89,6 @@ SIGNATURES: dict[str, list] = {
 }
 _RESTYPES = {"zib_status_string": ctypes.c_char_p, "zib_last_error": ctypes.c_char_p,
              "zib_group_norm_workspace": ctypes.c_int64, "zib_fp8_block_linear_scratch": ctypes.c_int64}
-
-# zib_dtype codes of the entry points that take several element types
-DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 _lib = None
 _lock = threading.Lock()
@@ -182,52 +180,18 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
-_FN: dict[str, object] = {}  # entry points by name, bound once
+_ops = None
 
 
-def call_on(dev: int, name: str, *args) -> None:
-    """``call`` on CUDA device ``dev``, whichever device is current; its current stream is appended.
-
-    The path of the operators that a latency-bound loop calls: the entry point is bound once and the
-    stream handle read without a Stream object (2 us each through ``torch.cuda.current_stream``).
-    """
-    global LAUNCHES
-    fn = _FN.get(name)
-    if fn is None:
-        fn = _FN[name] = getattr(load(), name)
-    LAUNCHES += 1
-    if dev == _current_device():
-        status = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev))
-    if status != ZIB_OK:
-        check(status, name)
-
-
-def _raw_stream(dev: int) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-_current_device = torch.cuda.current_device
-if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle, without the object around it
-    _raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def dtype_code(t: torch.Tensor, what: str) -> int:
-    """The zib_dtype of ``t``; ValueError for a type the entry points do not take."""
-    code = DTYPES.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{what} must be bfloat16, float16 or float32; got {t.dtype}")
-    return code
-
-
-def same_device(t: torch.Tensor, *others: torch.Tensor | None) -> None:
-    """ValueError unless every given tensor lies on the device of ``t``."""
-    dev = t.device
-    for o in others:
-        if o is not None and o.device != dev:
-            raise ValueError(f"an operand is on {o.device}, expected {dev}")
+def ops():
+    """The torch functions over the library (csrc/torch_ops.cpp), loaded on first use."""
+    global _ops
+    if _ops is None:
+        load()
+        if not LIB_PATH.with_name("_ops.so").exists():
+            raise RuntimeError("_ops.so is not built; run `python comfyui-zimage-triton_b200/csrc/build.py`")
+        _ops = importlib.import_module("._ops", __package__)
+    return _ops
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

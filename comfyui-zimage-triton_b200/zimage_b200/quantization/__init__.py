@@ -2,6 +2,7 @@
 8-bit floating-point products."""
 
 from .fp8_linear import (
+    Fp8BlockLinear,
     fp8_block_linear,
     fp8_block_matmul,
     fp8_block_quantize,
@@ -12,4 +13,4 @@ from .int8_linear import apply_int8_quantization, refresh_int8_weights, restore_
 
 __all__ = ["apply_int8_quantization", "restore_int8_quantization", "refresh_int8_weights",
            "fp8_block_quantize", "fp8_block_quantize_weight", "fp8_block_transpose", "fp8_block_matmul",
-           "fp8_block_linear"]
+           "fp8_block_linear", "Fp8BlockLinear"]
