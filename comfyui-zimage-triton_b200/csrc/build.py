@@ -49,13 +49,14 @@ def build_ops(force: bool = False, verbose: bool = False) -> Path:
         return OPS
     import sysconfig
 
-    import torch
+    import torch  # its C++ runtime is the system's shared one: the system compiler links against that
     from torch.utils import cpp_extension
 
     inc = cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]
     lib = cpp_extension.library_paths("cuda")
+    gxx = next(c for c in ("/usr/bin/g++", shutil.which("g++") or "g++") if Path(c).exists() or c == "g++")
     tmp = OPS.with_suffix(".so.tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc), str(src),
            "-o", str(tmp), *(f"-L{p}" for p in lib), "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_cuda",
            f"-L{PKG}", "-l:libzimage_b200.so", "-Wl,-rpath,$ORIGIN"]

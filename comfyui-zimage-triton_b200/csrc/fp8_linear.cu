@@ -13,7 +13,7 @@
 // first use of the result.
 //
 // 3840 x 11520 (44 MB, 6.8 us at HBM's rate; a plain reduction over as many bytes takes 11 us): one
-// token 14.3 us, eight 13.9 us behind a quantiser of 4.3 us.  Staging the weight in shared memory, one
+// token 13.0 us, eight 13.9 us behind a quantiser of 4.3 us.  Staging the weight in shared memory, one
 // persistent CTA per SM, measured 18 us by one bulk copy per 1024 bytes of a row and 15 us by TMA boxes
 // of 16 x 1024 bytes.
 //
@@ -29,6 +29,7 @@ constexpr int kWarps = 8;
 constexpr int kRing = 4;         // blocks in flight per warp
 constexpr int kMaxTokens = 8;
 constexpr int kFusedTokens = 2;  // tokens that every CTA quantises itself
+constexpr int kFusedSmem = 96 * 1024;  // for them; leaves two CTAs to an SM
 
 struct SmallParams {
   const void* x;  // FUSED: the tokens; else e4m3 rows, 16-byte aligned
@@ -192,8 +193,8 @@ template <typename T, bool FUSED>
 static int launch_small(const SmallParams& p, cudaStream_t st, const char* what) {
   auto* kernel = linear_small_kernel<T, FUSED>;
   const size_t smem = FUSED ? fused_smem(p.kb) : 0;
-  if (smem > 32 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 32 * 1024) {  // the largest size at once: another thread may launch with another one
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFusedSmem);
     ZIB_HOST_CHECK(e == cudaSuccess, ZIB_ERR_LAUNCH, "%s: cudaFuncSetAttribute failed: %s", what,
                    cudaGetErrorString(e));
   }
@@ -221,8 +222,7 @@ static int small(const SmallParams& p, bool fused, cudaStream_t st, const char* 
   return fused ? launch_small<T, true>(p, st, what) : launch_small<T, false>(p, st, what);
 }
 
-// 96 KB of shared memory for the tokens leaves two CTAs to an SM
-static bool is_fused(int64_t M, int64_t kb) { return M <= kFusedTokens && fused_smem(kb) <= 96 * 1024; }
+static bool is_fused(int64_t M, int64_t kb) { return M <= kFusedTokens && fused_smem(kb) <= kFusedSmem; }
 
 }  // namespace fp8
 }  // namespace zib

