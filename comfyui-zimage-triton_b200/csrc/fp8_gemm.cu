@@ -128,6 +128,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
 }
 
+// Launched behind the quantiser that writes q and its scales, the kernel may start before that has
+// ended: set-up overlaps its tail (2 to 3 us of a call on few rows), and what reads them waits here.
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Tile t -> (M-block, N-block): the fast index runs in groups whose rows stay in L2 while the
 // tiles sweep the slow index (the same order as the int8 GEMM's).
 __device__ __forceinline__ void tile_at(const GemmParams& p, int tile, int& mb, int& nb) {
@@ -283,6 +287,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
     if (warp == 0 && lane == 0) {  // ---- TMA producer (both CTAs)
+      wait_for_primary();  // q
       int stage = 0;
       uint32_t phase = 0, pend_mask = 0, pend_parity = 0;
       bool ok = true;
@@ -363,6 +368,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       sx = px_ ? __ldg(px_) : 0.0f;
       sw = pw_ ? __ldg(pw_) : 0.0f;
     };
+    wait_for_primary();  // the scales of q
     if (cluster_id < p.num_tiles) locate(cluster_id);
     for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
       const int row0 = mb * 256 + (int)rank * 128 + quarter * 32, n0 = nb * BN + half * CW;
@@ -446,7 +452,7 @@ constexpr int64_t kGroupBudget = 48ll << 20;  // L2 bytes for the operand that e
 
 template <typename T, int BN>
 static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K,
-                       cudaStream_t st, const char* what) {
+                       bool dependent, cudaStream_t st, const char* what) {
   CUtensorMap ta, tb, ty;
   int rc = make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, K, p.M, ldq, 128u, what);
   if (!rc) rc = make_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, K, p.N, ldw, BN / 2, what);
@@ -478,18 +484,33 @@ static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, 
   p.group = (int)ceil_div(nfast, groups);
   int clusters = sm_count() / 2;
   if (clusters > p.num_tiles) clusters = p.num_tiles;
-  gemm_pair_kernel<T, BN><<<2 * clusters, kThreads, Cfg<BN>::SMEM, st>>>(ta, tb, ty, p);
-  return zib_check_launch(what);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * clusters);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<BN>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = dependent ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_pair_kernel<T, BN>, ta, tb, ty, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    zib_set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
+    return ZIB_ERR_LAUNCH;
+  }
+  return ZIB_OK;
 }
 
 template <typename T>
 static int gemm(const GemmParams& p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K,
-                cudaStream_t st, const char* what) {
+                bool dependent, cudaStream_t st, const char* what) {
   // whole waves of 256 x 256 tiles, or twice as many 256 x 128 ones where those end sooner
   const int64_t pairs = sm_count() / 2, mb = ceil_div(p.M, 256);
   const int64_t wide = ceil_div(mb * ceil_div(p.N, 256), pairs) * 2, slim = ceil_div(mb * ceil_div(p.N, 128), pairs);
-  if (slim < wide) return launch_pair<T, 128>(p, q, ldq, w, ldw, K, st, what);
-  return launch_pair<T, 256>(p, q, ldq, w, ldw, K, st, what);
+  if (slim < wide) return launch_pair<T, 128>(p, q, ldq, w, ldw, K, dependent, st, what);
+  return launch_pair<T, 256>(p, q, ldq, w, ldw, K, dependent, st, what);
 }
 
 }  // namespace fp8
@@ -499,15 +520,15 @@ using namespace zib;
 
 int zib::fp8_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k, const void* w, int64_t ldw,
                   const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, int dtype,
-                  int64_t M, int64_t N, int64_t K, cudaStream_t st, const char* what) {
+                  int64_t M, int64_t N, int64_t K, bool dependent, cudaStream_t st, const char* what) {
   fp8::GemmParams p{};
   p.M = (int)M; p.N = (int)N;
   p.sx = sx; p.sx_m = sx_m; p.sx_k = sx_k;
   p.sw = sw; p.sw_n = sw_n; p.sw_k = sw_k;
   p.bias = bias; p.y = y; p.ldy = ldy;
-  if (dtype == ZIB_BF16) return fp8::gemm<__nv_bfloat16>(p, q, ldq, w, ldw, K, st, what);
-  if (dtype == ZIB_F16) return fp8::gemm<__half>(p, q, ldq, w, ldw, K, st, what);
-  return fp8::gemm<float>(p, q, ldq, w, ldw, K, st, what);
+  if (dtype == ZIB_BF16) return fp8::gemm<__nv_bfloat16>(p, q, ldq, w, ldw, K, dependent, st, what);
+  if (dtype == ZIB_F16) return fp8::gemm<__half>(p, q, ldq, w, ldw, K, dependent, st, what);
+  return fp8::gemm<float>(p, q, ldq, w, ldw, K, dependent, st, what);
 }
 
 extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
@@ -524,6 +545,6 @@ extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, i
                  ZIB_ERR_ALIGNMENT, "%s: q and w need 16-byte aligned rows", what);
   if (M == 0) return ZIB_OK;
   ZIB_HOST_CHECK(q && sx && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
-  return fp8_gemm(q, ldq, sx, sx_m, sx_k, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, (cudaStream_t)stream,
-                  what);
+  return fp8_gemm(q, ldq, sx, sx_m, sx_k, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, false,
+                  (cudaStream_t)stream, what);
 }

@@ -277,7 +277,7 @@ extern "C" int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const
     if (sum) fp8_sum_finish(part, sum, dtype, M, K, st);
   }
   if (M > fp8::kMaxTokens)
-    return fp8_gemm(scratch, ldq, s, 1, M, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, st, what);
+    return fp8_gemm(scratch, ldq, s, 1, M, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, true, st, what);
   const bool fused = sc.bytes == 0;
   const int size = dtype_bytes(dtype);
   fp8::SmallParams p{};
