@@ -286,22 +286,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
-    if (warp == 0 && lane == 0) {  // ---- TMA producer (both CTAs)
+    if (warp == 0) {  // ---- TMA producer (both CTAs): the whole warp waits, one elected thread issues
       wait_for_primary();  // q
       int stage = 0;
       uint32_t phase = 0, pend_mask = 0, pend_parity = 0;
       bool ok = true;
+      const uint32_t full0 = leader ? smem_u32(full_bar) : mapa_rank(smem_u32(full_bar), 0);
       for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
         int mb, nb;
         tile_at(p, t, mb, nb);
+        const int row_a = mb * 256 + (int)rank * 128, row_b = nb * BN + (int)rank * (BN / 2);
         for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
-          const uint32_t fb = smem_u32(&full_bar[stage]);
-          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * C::STAGE);
-          const uint32_t fb_leader = leader ? fb : mapa_rank(fb, 0);
+          if (!warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
           uint8_t* st = smem + stage * C::STAGE;
-          tma_load_2d_pair(st, &map_a, fb_leader, kb * kBlock, mb * 256 + (int)rank * 128);
-          tma_load_2d_pair(st + kABytes, &map_b, fb_leader, kb * kBlock, nb * BN + (int)rank * (BN / 2));
+          if (elect_one()) {
+            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * C::STAGE);
+            tma_load_2d_pair(st, &map_a, full0 + 8 * stage, kb * kBlock, row_a);
+            tma_load_2d_pair(st + kABytes, &map_b, full0 + 8 * stage, kb * kBlock, row_b);
+          }
+          __syncwarp();
           pend_mask |= 1u << stage;
           pend_parity = (pend_parity & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
