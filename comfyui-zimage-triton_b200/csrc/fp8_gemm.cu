@@ -18,11 +18,13 @@
 //              that scale is one value too: one packed multiply-add per two elements and K-block.
 //              The output tile leaves through shared memory and TMA stores that drain while the
 //              next tile is summed.
-// What bounds it at 18432 x 11520 x 3840 (723 us, 2250 TFLOP/s): the way of one accumulator from MMA
-// to registers and back to the MMA, 1740 clocks of which the MMAs themselves take 820 (the same
-// pipeline without the sums between blocks runs at 590-650 us, bound by the operands' way to shared
-// memory).  Measured on that way: release at cluster scope 1805 us, one thread waiting and issuing
-// 840 us, accumulators of 128 columns in two halves of the tile 895 us (the rows of q are read twice).
+// What bounds it at 18432 x 11520 x 3840 (714 us, 2285 TFLOP/s): the way of one accumulator from MMA to
+// registers and back to the MMA, about 1750 clocks with two of them under way, of which the MMAs take
+// 900, the signals between the two CTAs and the warps 600 and the reads 250.  Without the sums
+// between blocks the same pipeline runs at 580 us (2810 TFLOP/s), where the library's product with one
+// scale a tensor is too.  Measured on that way: release at cluster scope 1805 us, one thread waiting
+// and issuing 840 us, accumulators of 128 columns in two halves of the tile 790 us (the rows of q are
+// read twice), tiles of 256 x 128 throughout 1030 us.
 // Every mbarrier wait is bounded; on expiry the CTA records ZIB_ERR_TIMEOUT in a device error word,
 // drains its loads and MMAs, frees TMEM and exits.
 #include "fp8_quant.cuh"
@@ -355,6 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ---- sums over K-blocks and output (both CTAs)
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     uint8_t* xw = xbuf + (warp - 4) * C::XWARP;
+    const uint32_t tempty0 = mapa_rank(smem_u32(tempty_bar), 0);
     const uint32_t t_warp = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * CW);
     int buf = 0;
     uint32_t buf_phase = 0;
@@ -404,7 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // read: the accumulator may be filled again
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_pair(mapa_rank(smem_u32(&tempty_bar[buf]), 0));
+        if (lane == 0) arrive_pair(tempty0 + 8 * buf);
         add_scaled(acc, CW / 2 - 32, r0, s2);
         add_scaled(acc, CW / 2 - 16, r1, s2);
         if (++buf == BUFS) { buf = 0; buf_phase ^= 1u; }
