@@ -67,9 +67,9 @@ __device__ __forceinline__ void store8(uint8_t* __restrict__ row, int64_t k, int
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h + 2] * inv, v[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
     w[h] = lo | (hi << 16);
   }
-  if constexpr (VEC) {
-    if (k < K) *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
-  } else {
+  if (VEC && k + 8 <= K) {
+    *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
+  } else {  // also a ragged row's end: what lies behind it stays
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (k + j < K) row[k + j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));

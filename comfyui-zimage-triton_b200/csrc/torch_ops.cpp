@@ -98,7 +98,14 @@ Tensor aligned(const Tensor& q) {
   const bool rows = q.size(0) <= 1 || (q.stride(0) % 16 == 0 && q.stride(0) >= q.size(1));
   if (cols && rows && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0) return q;
   Tensor t = e4m3_rows(q.size(0), q.size(1), q);
-  t.copy_(q);
+  if (cols) {
+    On on(q);
+    status(zib_fp8_align_rows(ptr(q), q.size(0) <= 1 ? q.size(1) : q.stride(0), ptr(t), ld_of(t), q.size(0), q.size(1),
+                              on.stream),
+           "8-bit operand");
+  } else {
+    t.copy_(q);
+  }
   return t;
 }
 

@@ -75,6 +75,7 @@ SIGNATURES: dict[str, list] = {
     "zib_fp8_block_linear_scratch": [_I64, _I64, _I32],
     "zib_fp8_block_linear": [_VP, _I64, _I32, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _I64, _VP, _VP, _I64, _I64,
                              _I64, _I64, _VP],
+    "zib_fp8_align_rows": [_VP, _I64, _VP, _I64, _I64, _I64, _VP],
     "zib_fp8_transpose": [_VP, _I64, _VP, _I64, _I64, _I64, _VP],
     "zib_col_sum": [_VP, _I64, _I32, _VP, _VP, _I64, _I64, _I64, _VP],
     "zib_rotary": [_VP, _I64, _I64, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _VP, _I64, _I32, _VP, _VP, _I64,

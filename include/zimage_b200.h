@@ -352,6 +352,11 @@ ZIB_API int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const vo
                          int64_t ldy, void* sum, void* scratch, int64_t nscratch, int64_t M,
                          int64_t N, int64_t K, void* stream);
 
+/* Rows of 8-bit values copied to rows on 16-byte boundaries (ldo % 16 == 0), as the
+ * products read them. */
+ZIB_API int zib_fp8_align_rows(const void* w, int64_t ldw, void* out, int64_t ldo, int64_t N, int64_t K,
+                       void* stream);
+
 /* wt[k,n] = w[n,k] of 8-bit values: the weight of the gradient towards the
  * activations (its scales are the same blocks, transposed). */
 ZIB_API int zib_fp8_transpose(const void* w, int64_t ldw, void* wt, int64_t ldt, int64_t N, int64_t K,

@@ -839,3 +839,31 @@ def test_operators_on_another_stream(cuda):
         got = fp8_block_linear(group_norm_act(x, 8), wq, ws)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("K", [1, 7, 8, 13, 129, 1001])
+def test_quantised_rows_leave_what_lies_behind_them(cuda, K):
+    """Rows inside a wider buffer: the kernel stores eights where it can, and nothing past a row's end."""
+    x = torch.randn(9, K, generator=_gen(K), device="cuda", dtype=torch.float32)
+    ld = (K + 7) // 8 * 8 + 16
+    buf = torch.full((9, ld), 0x5A, device="cuda", dtype=torch.uint8)
+    s = torch.zeros((K + 127) // 128, 9, device="cuda")
+    _lib.call("zib_fp8_quant_rows", x.data_ptr(), K, 2, buf.data_ptr(), ld, s.data_ptr(), 1, 9, 9, K,
+              torch.cuda.current_stream().cuda_stream)
+    rq, rs = ref_rows(x)
+    assert same(buf[:, :K].contiguous().view(torch.float8_e4m3fn), rq) and same(s.t(), rs)
+    assert (buf[:, K:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("K,cut", [(1, 3), (15, 1), (129, 2), (1000, 5)])
+def test_weights_at_any_address_and_stride(cuda, K, cut):
+    x = torch.randn(40, K, generator=_gen(3), device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(70, K, generator=_gen(4), device="cuda", dtype=torch.bfloat16)
+    qw, sw = fp8_block_quantize_weight(w)
+    wide = torch.zeros(70, K + 9, device="cuda", dtype=torch.uint8)
+    wide[:, cut:cut + K] = qw.view(torch.uint8)
+    view = wide[:, cut:cut + K].view(torch.float8_e4m3fn)
+    even = torch.zeros(70, (K + 15) // 16 * 16, device="cuda", dtype=torch.uint8)
+    even[:, :K] = qw.view(torch.uint8)
+    even = even.view(torch.float8_e4m3fn)[:, :K]
+    assert torch.equal(fp8_block_linear(x, view, sw), fp8_block_linear(x, even, sw))
