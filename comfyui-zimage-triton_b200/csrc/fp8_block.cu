@@ -40,32 +40,45 @@ __device__ __forceinline__ void widen(const Raw<T>& r, float (&v)[8]) {
   for (int j = 0; j < 8; ++j) v[j] = to_f32(r.v[j / E].v[j % E]);
 }
 
-// The largest magnitude of 8 lanes' 16 values each, as fp32 bits.  Magnitudes order as their bits, so
-// the 16-bit types compare two at a time without unpacking.
+// Largest magnitudes.  They order as their bits, so the 16-bit types are compared two at a time without
+// unpacking (first in either half of the result), fp32 as they are.
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
 template <typename T>
-__device__ __forceinline__ uint32_t block_amax(const Raw<T>& lo, const Raw<T>& hi) {
+__device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) {
+  return sizeof(T) == 2 ? max2(a, b) : max(a, b);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t largest(const Raw<T>& r) {
   if constexpr (sizeof(T) == 2) {
-    auto max2 = [](uint32_t a, uint32_t b) {
-      uint32_t m;
-      asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
-      return m;
-    };
-    const uint4 u = *reinterpret_cast<const uint4*>(&lo), w = *reinterpret_cast<const uint4*>(&hi);
-    uint32_t m = max2(max2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), max2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
-    m = max2(m, max2(max2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), max2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) m = max2(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const uint4 u = *reinterpret_cast<const uint4*>(&r);
+    return max2(max2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), max2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+  } else {
+    float f[8];
+    widen(r, f);
+    return amax8(f);
+  }
+}
+// as fp32 bits
+template <typename T>
+__device__ __forceinline__ uint32_t largest_f32(uint32_t m) {
+  if constexpr (sizeof(T) == 2) {
     const uint16_t a = (uint16_t)max(m >> 16, m & 0xFFFFu);
     return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&a)));
   } else {
-    float f[8], h[8];
-    widen(lo, f);
-    widen(hi, h);
-    uint32_t a = max(amax8(f), amax8(h));
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
-    return a;
+    return m;
   }
+}
+// of 8 lanes' 16 values each
+template <typename T>
+__device__ __forceinline__ uint32_t block_amax(const Raw<T>& lo, const Raw<T>& hi) {
+  uint32_t m = join<T>(largest(lo), largest(hi));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) m = join<T>(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  return largest_f32<T>(m);
 }
 
 // Activation rows.  Bound by memory (3 bytes per 16-bit element).  A CTA takes kRows rows of four blocks
@@ -148,28 +161,34 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && !SUM ? 4 : 3) quant_row
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product may start and wait
 }
 
-// Weights: one CTA per block of 128 x 128, held in registers between its maximum and its values.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quant_blocks_kernel(const T* __restrict__ w, int64_t ldw,
-                                                           uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s,
-                                                           int64_t s_n, int64_t s_k, int64_t N, int64_t K) {
+// Weights: one CTA per block of 128 x 128, held in registers (as loaded) between its maximum and its
+// values.  11520 x 3840 bf16 33 us (4.0 TB/s; 37 with a fourth CTA on an SM, whose registers spill, 40 with
+// the values widened first), fp32 37 us (6.0 TB/s).
+template <typename T, bool VEC, bool VST>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quant_blocks_kernel(
+    const T* __restrict__ w, int64_t ldw, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s, int64_t s_n,
+    int64_t s_k, int64_t N, int64_t K) {
   __shared__ uint32_t red[8];
   const int64_t n0 = (int64_t)blockIdx.y * kBlock + (threadIdx.x >> 4);
   const int64_t k = (int64_t)blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
-  float v[8][8];
-  uint32_t a = 0;
+  Raw<T> v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load8<T, VEC>(w + (n0 + 16 * i) * ldw, k, n0 + 16 * i < N ? K : 0, v[i]);
+  for (int i = 0; i < 8; ++i) v[i] = load_raw<T, VEC>(w + (n0 + 16 * i) * ldw, k, n0 + 16 * i < N ? K : 0);
+  uint32_t a = largest(v[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, amax8(v[i]));
-  a = __reduce_max_sync(0xFFFFFFFFu, a);
+  for (int i = 1; i < 8; ++i) a = join<T>(a, largest(v[i]));
+  a = __reduce_max_sync(0xFFFFFFFFu, largest_f32<T>(a));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) a = max(a, red[i]);
   const float sc = block_scale(a), inv = inverse_scale(sc);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) store8<VEC>(q + (n0 + 16 * i) * ldq, k, n0 + 16 * i < N ? K : 0, v[i], inv);
+  for (int i = 0; i < 8; ++i) {
+    float f[8];
+    widen(v[i], f);
+    store8<VST>(q + (n0 + 16 * i) * ldq, k, n0 + 16 * i < N ? K : 0, f, inv);
+  }
   if (threadIdx.x == 0) s[blockIdx.y * s_n + blockIdx.x * s_k] = sc;
 }
 
@@ -315,15 +334,18 @@ extern "C" int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void*
   ZIB_HOST_CHECK(nb <= 65535, ZIB_ERR_TOO_LARGE, "%s: N=%lld", what, (long long)N);
   cudaStream_t st = (cudaStream_t)stream;
   const dim3 g((unsigned)kb, (unsigned)nb);
-  const bool vec = fp8::vector_loads(w, ldw, dtype_bytes(dtype), N, K) && fp8::vector_stores(q, ldq, N);
-  auto go = [&](auto kernel, auto* wt) {
+  const bool vec = fp8::vector_loads(w, ldw, dtype_bytes(dtype), N, K), vst = fp8::vector_stores(q, ldq, N);
+  auto go = [&](auto* wt) {
+    using T = std::remove_cv_t<std::remove_pointer_t<decltype(wt)>>;
+    using namespace fp8;
+    auto* kernel = !vst  ? quant_blocks_kernel<T, false, false>
+                   : vec ? quant_blocks_kernel<T, true, true>
+                         : quant_blocks_kernel<T, false, true>;
     kernel<<<g, 256, 0, st>>>(wt, ldw, (uint8_t*)q, ldq, s, s_n, s_k, N, K);
   };
-  using B = __nv_bfloat16;
-  using H = __half;
-  if (dtype == ZIB_BF16) go(vec ? fp8::quant_blocks_kernel<B, true> : fp8::quant_blocks_kernel<B, false>, (const B*)w);
-  else if (dtype == ZIB_F16) go(vec ? fp8::quant_blocks_kernel<H, true> : fp8::quant_blocks_kernel<H, false>, (const H*)w);
-  else go(vec ? fp8::quant_blocks_kernel<float, true> : fp8::quant_blocks_kernel<float, false>, (const float*)w);
+  if (dtype == ZIB_BF16) go((const __nv_bfloat16*)w);
+  else if (dtype == ZIB_F16) go((const __half*)w);
+  else go((const float*)w);
   return zib_check_launch(what);
 }
 
