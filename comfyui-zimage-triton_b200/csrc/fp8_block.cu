@@ -81,11 +81,11 @@ __device__ __forceinline__ uint32_t block_amax(const Raw<T>& lo, const Raw<T>& h
   return largest_f32<T>(m);
 }
 
-// Activation rows.  Bound by memory (3 bytes per 16-bit element).  A CTA takes kRows rows of four blocks
-// (512 columns), a warp kRows / 8 of them, two rows in flight; 8 lanes x 16 values to a block (8 of
+// Activation rows.  Bound by memory (3 bytes per 16-bit element).  A CTA takes 8 * wrows rows of four blocks
+// (512 columns), a warp wrows of them, two rows in flight; 8 lanes x 16 values to a block (8 of
 // either half of it, so that accesses stay side by side): what is done once per block and lane, its
-// maximum over lanes and its scale, counts half as much as with 16 lanes.  18432 x 3840 bf16: 43 us
-// (5.0 TB/s, 71% of the issue slots); 16 lanes to a block, 8 rows in flight 72 us.
+// maximum over lanes and its scale, counts half as much as with 16 lanes.  18432 x 3840 bf16: 47 us
+// with its launch (4.5 TB/s, 71% of the issue slots); 16 lanes to a block, 8 rows in flight 72 us.
 // SUM: the CTA leaves the sums of its columns in part[.][K] (a bias gradient: the rows need not be read
 // again for it).
 constexpr int kRows = 64;
@@ -97,14 +97,14 @@ constexpr int kQuad = 4 * kBlock;
 template <typename T, bool VEC, bool VST, bool SUM>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 && !SUM ? 4 : 3) quant_rows_kernel(
     const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s, int64_t s_m,
-    int64_t s_k, float* __restrict__ part, int64_t M, int64_t K, int quads) {
+    int64_t s_k, float* __restrict__ part, int64_t M, int64_t K, int quads, int wrows) {
   constexpr int U = 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t group = blockIdx.x / quads;
   const int64_t b = 4 * (int64_t)(blockIdx.x - group * quads) + (lane >> 3);
   const int64_t k = b * kBlock + (lane & 7) * 8;
-  const int64_t m0 = group * kRows + warp * (kRows / 8);
-  const int rows = M - m0 < kRows / 8 ? (int)(M - m0) : kRows / 8;
+  const int64_t m0 = (group * 8 + warp) * wrows;
+  const int rows = M - m0 < wrows ? (int)(M - m0) : wrows;
   const T* xr = x + m0 * ldx;
   uint8_t* qr = q + m0 * ldq;
   float* sr = s + m0 * s_m + b * s_k;
@@ -288,7 +288,13 @@ int64_t zib::fp8_sum_rows(int64_t M) { return ceil_div(M, fp8::kRows); }
 
 int zib::fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m, int64_t s_k,
                         float* part, int64_t M, int64_t K, cudaStream_t st, const char* what) {
-  const int64_t quads = ceil_div(K, fp8::kQuad), grid = ceil_div(M, fp8::kRows) * quads;
+  const int64_t quads = ceil_div(K, fp8::kQuad);
+  // Rows to a warp.  Two are in flight anyway: more make a chain of loads, which few rows wait for
+  // (3840 columns bf16, 2 / 4 / 8 of them: 8 rows 2.2 / 3.2 / 5.0 us, 1024 5.8 / 6.7 / 8.2, 4608 14.5 / 15.2 / 18.2);
+  // fewer are more CTAs to start (18432 rows 50.0 / 47.4 / 48.6).  Column sums want long slabs.
+  const bool many = ceil_div(M, 32) * quads >= 8 * sm_count();
+  const int wrows = part ? fp8::kRows / 8 : many ? 4 : 2;
+  const int64_t grid = ceil_div(M, 8 * wrows) * quads;
   ZIB_HOST_CHECK(grid <= 0x7FFFFFFF, ZIB_ERR_TOO_LARGE, "%s: M=%lld K=%lld", what, (long long)M, (long long)K);
   const bool vec = fp8::vector_loads(x, ldx, dtype_bytes(dtype), M, K), vst = fp8::vector_stores(q, ldq, M);
   auto go = [&](auto* xt) {
@@ -300,7 +306,7 @@ int zib::fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t 
                         : (!vst  ? quant_rows_kernel<T, false, false, false>
                            : vec ? quant_rows_kernel<T, true, true, false>
                                  : quant_rows_kernel<T, false, true, false>);
-    kernel<<<(unsigned)grid, 256, 0, st>>>(xt, ldx, (uint8_t*)q, ldq, s, s_m, s_k, part, M, K, (int)quads);
+    kernel<<<(unsigned)grid, 256, 0, st>>>(xt, ldx, (uint8_t*)q, ldq, s, s_m, s_k, part, M, K, (int)quads, wrows);
   };
   if (dtype == ZIB_BF16) go((const __nv_bfloat16*)x);
   else if (dtype == ZIB_F16) go((const __half*)x);

@@ -18,13 +18,14 @@
 //              that scale is one value too: one packed multiply-add per two elements and K-block.
 //              The output tile leaves through shared memory and TMA stores that drain while the
 //              next tile is summed.
-// What bounds it at 18432 x 11520 x 3840 (714 us, 2285 TFLOP/s): the way of one accumulator from MMA to
-// registers and back to the MMA, about 1750 clocks with two of them under way, of which the MMAs take
-// 900, the signals between the two CTAs and the warps 600 and the reads 250.  Without the sums
-// between blocks the same pipeline runs at 580 us (2810 TFLOP/s), where the library's product with one
-// scale a tensor is too.  Measured on that way: release at cluster scope 1805 us, one thread waiting
-// and issuing 840 us, accumulators of 128 columns in two halves of the tile 790 us (the rows of q are
-// read twice), tiles of 256 x 128 throughout 1030 us.
+// What bounds it at 18432 x 11520 x 3840 (686 us, 2380 TFLOP/s): the way of one accumulator from the MMAs
+// to registers and back, 565 ns a K-block with two of them under way (the MMAs alone take 270, the
+// operands arrive every 320).  Without the sums between blocks the same pipeline runs at 580 us
+// (2810 TFLOP/s), where the library's product with one scale a tensor is too.  Measured on that way:
+// release at cluster scope 1805 us, one thread waiting and issuing 840 us, accumulators of 128 columns
+// in two halves of the tile 790 us (the rows of q are read twice), tiles of 256 x 128 throughout 1030 us,
+// the next accumulator's loads behind the current sums 800 us.  Tiles of 256 x 128 take 285 ns a K-block,
+// with 2 to 4 accumulators and 3 to 6 stages alike.
 // Every mbarrier wait is bounded; on expiry the CTA records ZIB_ERR_TIMEOUT in a device error word,
 // drains its loads and MMAs, frees TMEM and exits.
 #include "fp8_quant.cuh"

@@ -2,7 +2,7 @@
 //
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} q[m, k] w[n, k]  (+ bias[n]),  q, sx from x
 //
-// For a few tokens the product is a stream over the weight, bound by memory.  A CTA takes 16 weight
+// For few tokens the product is a stream over the weight, bound by memory.  A CTA takes 16 weight
 // rows, its eight warps every eighth block of 128 columns; a warp keeps four blocks (8 KB) in flight,
 // so an SM has 128 KB on the way.  Within a block the products run on mma.sync (m16n8k32, weight rows
 // as its rows, tokens as its columns), whose fresh fp32 sums are scaled into registers block by block;
@@ -13,12 +13,13 @@
 // first use of the result.
 //
 // 3840 x 11520 (44 MB, 6.8 us at HBM's rate; a plain reduction over as many bytes takes 11 us): one
-// token 13.0 us, eight 13.9 us behind a quantiser of 4.3 us.  Staging the weight in shared memory, one
+// token 13.0 us, eight 13.9 us behind a quantiser of 1.9 us.  Staging the weight in shared memory, one
 // persistent CTA per SM, measured 18 us by one bulk copy per 1024 bytes of a row and 15 us by TMA boxes
 // of 16 x 1024 bytes.
 //
-// More than 8 tokens: the rows are quantised to memory and the tcgen05 product reads them there (19 us
-// for 9 to 256 rows of 3840 x 11520; a second group of 8 tokens here: 20 us).
+// More than 8 tokens run in groups of 8 through the same kernel while the weight is so small, or its rows so
+// long, that the tcgen05 product's few tiles would take longer; else the rows are quantised to
+// memory and that product reads them there.
 #include "fp8_quant.cuh"
 
 namespace zib {
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_small_kernel(const Smal
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * kTileN;
+  const int m0 = FUSED ? 0 : blockIdx.y * kMaxTokens, M = min(p.M - m0, kMaxTokens);  // this CTA's tokens
 
   // rows g and g + 8 of the tile
   const bool ok0 = n0 + g < p.N, ok1 = n0 + g + 8 < p.N;
@@ -127,7 +129,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_small_kernel(const Smal
 
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   const float* sw = p.sw + (n0 / kBlock) * p.sw_n;
-  const bool c0 = 2 * t < p.M, c1 = 2 * t + 1 < p.M;  // columns behind the last token stay unused
+  const float* sx = FUSED ? nullptr : p.sx + m0 + 2 * t;
+  const bool c0 = 2 * t < M, c1 = 2 * t + 1 < M;  // columns behind the last token stay unused
   for (int b0 = warp; b0 < p.kb; b0 += kRing * kWarps) {
 #pragma unroll
     for (int i = 0; i < kRing; ++i) {
@@ -144,11 +147,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_small_kernel(const Smal
         sc1 = c1 ? ssx[b * kFusedTokens + 2 * t + 1] : 0.0f;
       } else {
         const int k = b * kBlock + 16 * t;
-        const uint8_t* xr = reinterpret_cast<const uint8_t*>(p.x) + g * p.ldx + k;
-        x0 = load16(xr, g < p.M && k < p.K);
-        x1 = load16(xr + 64, g < p.M && k + 64 < p.K);
-        sc0 = c0 ? __ldg(p.sx + b * p.M + 2 * t) : 0.0f;
-        sc1 = c1 ? __ldg(p.sx + b * p.M + 2 * t + 1) : 0.0f;
+        const uint8_t* xr = reinterpret_cast<const uint8_t*>(p.x) + (m0 + g) * p.ldx + k;
+        x0 = load16(xr, g < M && k < p.K);
+        x1 = load16(xr + 64, g < M && k + 64 < p.K);
+        sc0 = c0 ? __ldg(sx + (int64_t)b * p.M) : 0.0f;
+        sc1 = c1 ? __ldg(sx + (int64_t)b * p.M + 1) : 0.0f;
       }
       uint4 (&v)[4] = w[i];
       const int left = p.K - b * kBlock - 16 * t;  // bytes of a row from this thread's first one on
@@ -175,14 +178,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_small_kernel(const Smal
   *reinterpret_cast<float2*>(&red[warp][g][2 * t]) = make_float2(acc[0], acc[1]);
   *reinterpret_cast<float2*>(&red[warp][g + 8][2 * t]) = make_float2(acc[2], acc[3]);
   __syncthreads();
-  for (int i = threadIdx.x; i < kTileN * p.M; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < kTileN * M; i += kWarps * 32) {
     const int m = i / kTileN, n = i % kTileN;  // a token's 16 outputs side by side
     float v = 0.0f;
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) v += red[k][n][m];
     if (n0 + n < p.N) {
       if (p.bias) v += to_f32(reinterpret_cast<const T*>(p.bias)[n0 + n]);
-      reinterpret_cast<T*>(p.y)[m * p.ldy + n0 + n] = from_f32<T>(v);
+      reinterpret_cast<T*>(p.y)[(m0 + m) * p.ldy + n0 + n] = from_f32<T>(v);
     }
   }
 }
@@ -199,7 +202,7 @@ static int launch_small(const SmallParams& p, cudaStream_t st, const char* what)
                    cudaGetErrorString(e));
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ceil_div(p.N, kTileN));
+  cfg.gridDim = dim3((unsigned)ceil_div(p.N, kTileN), (unsigned)ceil_div(p.M, kMaxTokens));
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -220,6 +223,17 @@ static int launch_small(const SmallParams& p, cudaStream_t st, const char* what)
 template <typename T>
 static int small(const SmallParams& p, bool fused, cudaStream_t st, const char* what) {
   return fused ? launch_small<T, true>(p, st, what) : launch_small<T, false>(p, st, what);
+}
+
+// This kernel or the tcgen05 product.  One group of tokens is a stream over the weight: always here.  With
+// more groups a call takes about 8 us and 1 us per 2400 blocks (16 weight rows x 128 columns x 8
+// tokens; a CTA costs as much as 8 of them) here, and 11 us and 1 us per 3 blocks of K there, as long as
+// its tiles fill one wave.  Quantiser included, here / there: 640 x 4096, 128 tokens 17.3 / 21.2 us, 256
+// tokens 25.1 / 21.5; 128 x 16384, 256 tokens 20.6 / 52.2; 11520 x 3840, 9 tokens 27.1 / 23.6; 768 x
+// 256, 64 tokens 9.7 / 11.5.
+static bool is_small(int64_t M, int64_t N, int64_t kb) {
+  const int64_t ctas = ceil_div(M, kMaxTokens) * ceil_div(N, kTileN);
+  return M <= kMaxTokens || ctas * (kb > 8 ? kb : 8) < 7200 + 800 * kb;
 }
 
 static bool is_fused(int64_t M, int64_t kb) { return M <= kFusedTokens && fused_smem(kb) <= kFusedSmem; }
@@ -276,7 +290,7 @@ extern "C" int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const
     if (rc) return rc;
     if (sum) fp8_sum_finish(part, sum, dtype, M, K, st);
   }
-  if (M > fp8::kMaxTokens)
+  if (!fp8::is_small(M, N, kb))
     return fp8_gemm(scratch, ldq, s, 1, M, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, true, st, what);
   const bool fused = sc.bytes == 0;
   const int size = dtype_bytes(dtype);

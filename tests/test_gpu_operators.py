@@ -867,3 +867,16 @@ def test_weights_at_any_address_and_stride(cuda, K, cut):
     even[:, :K] = qw.view(torch.uint8)
     even = even.view(torch.float8_e4m3fn)[:, :K]
     assert torch.equal(fp8_block_linear(x, view, sw), fp8_block_linear(x, even, sw))
+
+
+@pytest.mark.parametrize("M,K,N", [(20, 2000, 346), (45, 257, 130), (100, 1024, 40), (257, 4096, 48), (600, 300, 17)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_groups_of_tokens(cuda, M, K, N, dtype):
+    """Few weight rows: tokens in groups of 8, the last one ragged."""
+    g = _gen(M + N)
+    x, w = (_randn(g, M, K)).to(dtype), (_randn(g, N, K) / 8).to(dtype)
+    b = _randn(g, N).to(dtype)
+    qw, sw = fp8_block_quantize_weight(w)
+    qx, sx = fp8_block_quantize(x)
+    ref, mag = product_terms(qx, sx, qw, sw)
+    check(fp8_block_linear(x, qw, sw, b), ref + b.double(), product_extra(mag, K, b))
