@@ -84,8 +84,8 @@ __device__ __forceinline__ uint32_t block_amax(const Raw<T>& lo, const Raw<T>& h
 // Activation rows.  Bound by memory (3 bytes per 16-bit element).  A CTA takes 8 * wrows rows of four blocks
 // (512 columns), a warp wrows of them, two rows in flight; 8 lanes x 16 values to a block (8 of
 // either half of it, so that accesses stay side by side): what is done once per block and lane, its
-// maximum over lanes and its scale, counts half as much as with 16 lanes.  18432 x 3840 bf16: 47 us
-// with its launch (4.5 TB/s, 71% of the issue slots); 16 lanes to a block, 8 rows in flight 72 us.
+// maximum over lanes and its scale, counts half as much as with 16 lanes.  18432 x 3840 bf16: 41 us
+// (5.2 TB/s, 71% of the issue slots); 16 lanes to a block, 8 rows in flight 72 us.
 // SUM: the CTA leaves the sums of its columns in part[.][K] (a bias gradient: the rows need not be read
 // again for it).
 constexpr int kRows = 64;
@@ -93,7 +93,7 @@ constexpr int kQuad = 4 * kBlock;
 
 // VEC: 16-byte loads (x has aligned rows of whole eights); VST: 8-byte stores (q has aligned rows, of
 // any length).  Rows of odd lengths come with unaligned x and, from a linear, aligned q: 14951 x 2129 bf16
-// in 42 us.
+// in 35 us.
 template <typename T, bool VEC, bool VST, bool SUM>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 && !SUM ? 4 : 3) quant_rows_kernel(
     const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s, int64_t s_m,
@@ -129,12 +129,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && !SUM ? 4 : 3) quant_row
       if constexpr (SUM)
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += f[j];
-      store8<VST>(qr + r * ldq, k, Kr, f, inv);
+      store8<VST, VEC>(qr + r * ldq, k, Kr, f, inv);
       widen(hi[r], f);
       if constexpr (SUM)
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[8 + j] += f[j];
-      store8<VST>(qr + r * ldq, k + 64, Kr, f, inv);
+      store8<VST, VEC>(qr + r * ldq, k + 64, Kr, f, inv);
       if ((lane & 7) == 0 && b * kBlock < Kr) sr[r * s_m] = sc;
     }
     xr += U * ldx;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quant_blocks_kern
   for (int i = 0; i < 8; ++i) {
     float f[8];
     widen(v[i], f);
-    store8<VST>(q + (n0 + 16 * i) * ldq, k, n0 + 16 * i < N ? K : 0, f, inv);
+    store8<VST, VEC>(q + (n0 + 16 * i) * ldq, k, n0 + 16 * i < N ? K : 0, f, inv);
   }
   if (threadIdx.x == 0) s[blockIdx.y * s_n + blockIdx.x * s_k] = sc;
 }
@@ -288,15 +288,15 @@ int64_t zib::fp8_sum_rows(int64_t M) { return ceil_div(M, fp8::kRows); }
 
 int zib::fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, float* s, int64_t s_m, int64_t s_k,
                         float* part, int64_t M, int64_t K, cudaStream_t st, const char* what) {
+  const bool vec = fp8::vector_loads(x, ldx, dtype_bytes(dtype), M, K), vst = fp8::vector_stores(q, ldq, M);
   const int64_t quads = ceil_div(K, fp8::kQuad);
-  // Rows to a warp.  Two are in flight anyway: more make a chain of loads, which few rows wait for
-  // (3840 columns bf16, 2 / 4 / 8 of them: 8 rows 2.2 / 3.2 / 5.0 us, 1024 5.8 / 6.7 / 8.2, 4608 14.5 / 15.2 / 18.2);
-  // fewer are more CTAs to start (18432 rows 50.0 / 47.4 / 48.6).  Column sums want long slabs.
-  const bool many = ceil_div(M, 32) * quads >= 8 * sm_count();
-  const int wrows = part ? fp8::kRows / 8 : many ? 4 : 2;
+  // Rows to a warp.  Two are in flight anyway: eight make a chain of loads, which few rows wait for and
+  // scalar loads lengthen (2 / 8 rows, bf16: 8 x 3840 1.9 / 3.3 us, 1024 x 3840 4.4 / 6.3, 14951 x 2129
+  // 35 / 41); two are more CTAs to start (18432 x 3840 44 / 41).  Column sums want long slabs.
+  const bool many = vec && ceil_div(M, fp8::kRows) * quads >= 3 * sm_count();
+  const int wrows = part || many ? fp8::kRows / 8 : 2;
   const int64_t grid = ceil_div(M, 8 * wrows) * quads;
   ZIB_HOST_CHECK(grid <= 0x7FFFFFFF, ZIB_ERR_TOO_LARGE, "%s: M=%lld K=%lld", what, (long long)M, (long long)K);
-  const bool vec = fp8::vector_loads(x, ldx, dtype_bytes(dtype), M, K), vst = fp8::vector_stores(q, ldq, M);
   auto go = [&](auto* xt) {
     using T = std::remove_cv_t<std::remove_pointer_t<decltype(xt)>>;
     using namespace fp8;

@@ -57,7 +57,8 @@ __device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
   return a;
 }
 
-template <bool VEC>
+// 8-byte stores where VEC; WHOLE: K % 8 == 0
+template <bool VEC, bool WHOLE = true>
 __device__ __forceinline__ void store8(uint8_t* __restrict__ row, int64_t k, int64_t K, const float (&v)[8],
                                        float inv) {
   uint32_t w[2];
@@ -67,7 +68,9 @@ __device__ __forceinline__ void store8(uint8_t* __restrict__ row, int64_t k, int
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h + 2] * inv, v[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
     w[h] = lo | (hi << 16);
   }
-  if (VEC && k + 8 <= K) {
+  if constexpr (VEC && WHOLE) {
+    if (k < K) *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
+  } else if (VEC && k + 8 <= K) {
     *reinterpret_cast<uint2*>(row + k) = make_uint2(w[0], w[1]);
   } else {  // also a ragged row's end: what lies behind it stays
 #pragma unroll
