@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && !SUM ? 4 : 3) quant_row
 // values.  11520 x 3840 bf16 33 us (4.0 TB/s; 37 with a fourth CTA on an SM, whose registers spill, 40 with
 // the values widened first), fp32 37 us (6.0 TB/s).
 template <typename T, bool VEC, bool VST>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quant_blocks_kernel(
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? (VEC ? 3 : 2) : 1) quant_blocks_kernel(
     const T* __restrict__ w, int64_t ldw, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ s, int64_t s_n,
     int64_t s_k, int64_t N, int64_t K) {
   __shared__ uint32_t red[8];
