@@ -234,13 +234,43 @@ __device__ __forceinline__ void sincos_turns(uint32_t a, float& s, float& c) {
   c = __uint_as_float(__float_as_uint(v) ^ (((quarter + 1) & 2) << 30));
 }
 
+// the same of two angles, on packed pairs
+__device__ __forceinline__ void sincos_turns2(uint32_t a0, uint32_t a1, float m, float (&s)[2], float (&c)[2]) {
+  const uint32_t q[2] = {(a0 + 0x20000000u) >> 30, (a1 + 0x20000000u) >> 30};
+  auto all = [](float v) { return px::mk(v, v); };
+  const px::f2 x = px::mul(px::mk((float)(int32_t)(a0 - (q[0] << 30)), (float)(int32_t)(a1 - (q[1] << 30))),
+                           all(1.4629180792671596e-09f));
+  const px::f2 x2 = px::mul(x, x);
+  px::f2 ps = all(2.7557319e-6f);
+  ps = px::fma(ps, x2, all(-1.9841270e-4f));
+  ps = px::fma(ps, x2, all(8.3333333e-3f));
+  ps = px::fma(ps, x2, all(-1.6666667e-1f));
+  ps = px::fma(px::mul(ps, x2), x, x);
+  px::f2 pc = all(-2.7557319e-7f);
+  pc = px::fma(pc, x2, all(2.4801587e-5f));
+  pc = px::fma(pc, x2, all(-1.3888889e-3f));
+  pc = px::fma(pc, x2, all(4.1666667e-2f));
+  pc = px::fma(pc, x2, all(-0.5f));
+  pc = px::fma(pc, x2, all(1.0f));
+  float sv[2], cv[2];
+  px::split(px::mul(ps, all(m)), sv[0], sv[1]);
+  px::split(px::mul(pc, all(m)), cv[0], cv[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float u = q[i] & 1 ? cv[i] : sv[i], v = q[i] & 1 ? sv[i] : cv[i];
+    s[i] = __uint_as_float(__float_as_uint(u) ^ ((q[i] & 2) << 30));
+    c[i] = __uint_as_float(__float_as_uint(v) ^ (((q[i] + 1) & 2) << 30));
+  }
+}
+
 // cos and sin of p f_j, f_j = theta^(-2j/dim) scaled.  The angle is formed in turns, in fixed point of
 // 64 bits: a whole position times a frequency, modulo whole turns, is one wrapping 64-bit product (the
 // frequency is rounded to 2^-64 turns, so a position below 2^31 is off by less than 2^-33 turns; the
 // fp64 frequency behind it by less than 2^-55 turns a position).  A thread keeps J neighbouring
 // frequencies and walks over positions, so the fp64 exp is paid once per thread.
-// 131072 x 64 (68 MB, 10.4 us at HBM's rate): 20.5 us; angles in fp64 28 us, sincospi of the fixed-point
-// angle 26 us, both short of issue slots.
+// 131072 x 64 (68 MB, 10.4 us at HBM's rate): 20 us launched alone, 14.3 back to back (a fill of as many
+// bytes 10.1; without packed pairs 15.8).  Launched alone, angles in fp64 take 28 us and sincospi of the
+// fixed-point angle 26, both short of issue slots.
 template <int J>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) {
   const int j0 = (blockIdx.y * blockDim.x + threadIdx.x) * J;
@@ -268,13 +298,15 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) 
       pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[t * p.ps]
                     : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[t * p.ps];
     Pack<float, J> c, s;
-#pragma unroll
-    for (int i = 0; i < J; ++i) {
+    // the nearest 2^-32 turns of the 64-bit product
+    auto angle = [&](int i) { return (uint32_t)(((uint64_t)pos * turns[i] + 0x80000000ull) >> 32); };
+    if constexpr (J == 2) {
+      sincos_turns2(angle(0), angle(1), p.mscale, s.v, c.v);
+    } else {
       float sv, cv;
-      // the nearest 2^-32 turns of the 64-bit product
-      sincos_turns((uint32_t)(((uint64_t)pos * turns[i] + 0x80000000ull) >> 32), sv, cv);
-      c.v[i] = p.mscale * cv;
-      s.v[i] = p.mscale * sv;
+      sincos_turns(angle(0), sv, cv);
+      c.v[0] = p.mscale * cv;
+      s.v[0] = p.mscale * sv;
     }
     *reinterpret_cast<Pack<float, J>*>(p.cos + t * p.half + j0) = c;
     *reinterpret_cast<Pack<float, J>*>(p.sin + t * p.half + j0) = s;
@@ -399,7 +431,7 @@ extern "C" int zib_rotary_table(const void* positions, int pos64, int64_t ps, in
   dim3 block(bx, 256 / bx);
   const int64_t gy = ceil_div(cols, bx);
   int64_t gx = ceil_div(T, (int64_t)block.y * 4);
-  const int64_t cap = ceil_div((int64_t)sm_count() * 8, gy);
+  const int64_t cap = ceil_div((int64_t)sm_count() * 6, gy);
   if (gx > cap) gx = cap;
   const dim3 grid((unsigned)gx, (unsigned)gy);
   if (two) rotary::rotary_table_kernel<2><<<grid, block, 0, (cudaStream_t)stream>>>(p);
