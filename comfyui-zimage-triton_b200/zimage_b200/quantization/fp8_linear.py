@@ -90,6 +90,15 @@ class Fp8BlockLinear(torch.nn.Module):
         m.bias = linear.bias
         return m
 
+    def _apply(self, fn, recurse: bool = True):
+        """``.to(dtype)``, ``.half()`` and the like change the bias alone: values and scales keep their types."""
+        kept = {k: t for k, t in self._buffers.items() if t is not None}
+        super()._apply(fn, recurse)
+        for k, t in kept.items():
+            if self._buffers[k].dtype != t.dtype:
+                self._buffers[k] = t.to(self._buffers[k].device)
+        return self
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return fp8_block_linear(x, self.w_q, self.w_scale, self.bias, self.w_q_t)
 

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from zimage_b200 import (GroupNormAct, _lib, fp8_block_linear, fp8_block_matmul, fp8_block_quantize,
+from zimage_b200 import (Fp8BlockLinear, GroupNormAct, _lib, fp8_block_linear, fp8_block_matmul, fp8_block_quantize,
                          fp8_block_quantize_weight, fp8_block_transpose, group_norm_act, rotary_embed, rotary_table)
 
 E4M3 = torch.float8_e4m3fn
@@ -152,3 +152,16 @@ def test_c_entries_validate_on_the_host():
     assert lib.zib_group_norm(*gn, 0, 0, 4, 12, 4, 0, 1e-6, 1, None) == 0
     assert lib.zib_group_norm_workspace(0, 4, 12, 4, 0) == 0
     assert lib.zib_group_norm_workspace(2, 400, 12, 4, 1) > 0
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.float16), lambda m: m.half(), lambda m: m.double(),
+                                  lambda m: torch.nn.Sequential(m).float()[0]])
+def test_fp8_block_linear_keeps_its_weight_through_casts(cast):
+    m = Fp8BlockLinear(130, 70, transposed=True)
+    m.w_q.view(torch.uint8).random_(0, 100)
+    q, s = m.w_q.clone(), m.w_scale.clone()
+    want = cast(torch.nn.Linear(1, 1)).bias.dtype
+    m = cast(m)
+    assert m.bias.dtype == want
+    assert m.w_q.dtype == m.w_q_t.dtype == torch.float8_e4m3fn and m.w_scale.dtype == torch.float32
+    assert torch.equal(m.w_q.view(torch.uint8), q.view(torch.uint8)) and torch.equal(m.w_scale, s)
