@@ -880,3 +880,33 @@ def test_linear_groups_of_tokens(cuda, M, K, N, dtype):
     qx, sx = fp8_block_quantize(x)
     ref, mag = product_terms(qx, sx, qw, sw)
     check(fp8_block_linear(x, qw, sw, b), ref + b.double(), product_extra(mag, K, b))
+
+
+@pytest.mark.parametrize("M,K,N", [(600, 1024, 1300), (70, 512, 257), (5, 300, 200)])
+def test_linear_captured_with_its_gradients(cuda, M, K, N):
+    """Each of the linear's kernels in a captured forward and backward pass, replayed on other inputs."""
+    g = _gen(M)
+    wq, ws = fp8_block_quantize_weight(_randn(g, N, K) / 16)
+    b = _randn(g, N).to(torch.bfloat16)
+    ins = [(_randn(g, M, K).to(torch.bfloat16), _randn(g, M, N).to(torch.bfloat16)) for _ in range(3)]
+
+    def step(x, d):
+        x, c = x.detach().requires_grad_(), b.detach().requires_grad_()
+        y = fp8_block_linear(x, wq, ws, c)
+        return (y.detach(), *torch.autograd.grad(y, (x, c), d))
+
+    want = [step(*i) for i in ins]
+    x, d = ins[0][0].clone(), ins[0][1].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, d)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, d)
+    for i in (1, 2, 0):
+        x.copy_(ins[i][0])
+        d.copy_(ins[i][1])
+        graph.replay()
+        assert all(torch.equal(a, e) for a, e in zip(out, want[i]))
