@@ -1,4 +1,5 @@
-// Block-scaled 8-bit product on 5th-generation tensor cores (tcgen05, kind::f8f6f4) for sm_100a.
+// Block-scaled 8-bit product on 5th-generation tensor cores (tcgen05) for sm_100a: for any scales by sums in
+// registers (kind::f8f6f4), and for powers of two by the tensor cores' own scales (kind::mxf8f6f4, below).
 //
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} q[m, k] w[n, k]  (+ bias[n])
 //
@@ -18,7 +19,7 @@
 //              that scale is one value too: one packed multiply-add per two elements and K-block.
 //              The output tile leaves through shared memory and TMA stores that drain while the
 //              next tile is summed.
-// What bounds it at 18432 x 11520 x 3840 (686 us, 2380 TFLOP/s): the way of one accumulator from the MMAs
+// What bounds the sums in registers at 18432 x 11520 x 3840 (686 us, 2380 TFLOP/s): the way of one accumulator from the MMAs
 // to registers and back, 565 ns a K-block with two of them under way (the MMAs alone take 270, the
 // operands arrive every 320).  Without the sums between blocks the same pipeline runs at 580 us
 // (2810 TFLOP/s), where the library's product with one scale a tensor is too.  Measured on that way:
@@ -74,6 +75,7 @@ struct GemmParams {
   void* y;
   int64_t ldy;
   int tma_store;  // y's rows are 16-byte aligned
+  int where;      // 0: any scales; 1: only where the weight's are not powers of two
 };
 
 // one tcgen05.mma of K = 32; acc is a constant after unrolling
@@ -236,6 +238,20 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, const CUtensorMa
   }
 }
 
+// every scale of the weight is a normal power of two (all CTAs find the same; the weight's scales are
+// not written by the launch before)
+__device__ __forceinline__ bool powers_of_two(const GemmParams& p) {
+  const int rows = (p.N + kBlock - 1) / kBlock, n = rows * p.num_kb;
+  bool ok = true;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int r = i / p.num_kb, k = i - r * p.num_kb;
+    const uint32_t b = __float_as_uint(__ldg(p.sw + r * p.sw_n + k * p.sw_k));
+    ok &= ((b & 0x7FFFFFu) == 0) & (b - 1 < 0x7F7FFFFFu);
+  }
+  return __syncthreads_and(ok) != 0;
+}
+
 template <typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -258,6 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
   const int cluster_id = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  if (p.where && powers_of_two(p)) return;  // the whole grid
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -437,6 +454,266 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                  : "memory");
 }
 
+// --- scales that the tensor cores apply -----------------------------------------------
+
+// Where the weight's scales are powers of two as the activations' are, both are exponents: the tensor
+// cores multiply them in (tcgen05.mma kind::mxf8f6f4, a scale of 8 exponent bits for each row and 32
+// columns; a block of 128 has the same one four times), and the sum over all K-blocks stays in one
+// accumulator.
+//
+// Tiles of 256 x 192 by pairs of CTAs: two accumulators of 192 columns leave 128 of TMEM's 512 for the
+// scales of the stages in flight (16 each).
+//   warp 0     TMA producer, as above
+//   warp 1     MMA issuer
+//   warps 4-7  output: TMEM to registers, through shared memory to TMA stores, while the next tile is summed
+//   warps 8-11 scales: every stage's 128 exponents of rows (4 columns) and 192 of weight rows (6 columns,
+//              each of 32 equal ones) to TMEM, once per lane quarter
+// 18432 x 11520 x 3840: 608 us (2680 TFLOP/s; 695 for the sums in registers, timed in turns), 4608 x 3840 x
+// 10240: 133 us (174).  Bound by the operands' way from L2 (28 KB an SM and K-block) and, with one
+// K-block's scales on their way at a time, by those: 779 us; two 614, four 609, six 608, ten 619, six over
+// the ends of tiles (more instructions per K-block) 640; without any loads of scales 579.
+// A weight with another scale anywhere is left to the kernel above, launched behind this one, which
+// otherwise ends at once.
+struct Mx {
+  static constexpr int BN = 192;
+  static constexpr int STAGES = 6;
+  static constexpr int STAGE = kABytes + BN / 2 * kBlock;
+  static constexpr int AHEAD = 6;  // K-blocks whose scales are on their way
+  static constexpr int XWARP = 8192;
+  static constexpr int SCALES = 2 * BN;  // first TMEM column of the scales
+  static constexpr int SMEM = STAGES * STAGE + 4 * XWARP + 256 + 1024;
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+  static_assert(SCALES + 16 * STAGES <= kTmemCols, "TMEM columns");
+  // D = f32, A = B = e4m3, both K-major, scales of 8 exponent bits, the first byte of their words
+  static constexpr uint32_t IDESC = ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(256 >> 7) << 27);
+};
+
+__device__ __forceinline__ void umma_mx_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t sa, uint32_t sb, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(Mx::IDESC), "r"(sa), "r"(sb), "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+// the exponent of a power of two (255: NaN), four times
+__device__ __forceinline__ uint32_t exponents(float s) {
+  return ((__float_as_uint(s) >> 23) & 0xFFu) * 0x01010101u;
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_mx_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_y, const GemmParams p) {
+  constexpr int STAGES = Mx::STAGES, BN = Mx::BN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* xbuf = smem + STAGES * Mx::STAGE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xbuf + 4 * Mx::XWARP);
+  uint64_t* full_bar = bars;                 // leader's is used
+  uint64_t* empty_bar = bars + STAGES;       // both
+  uint64_t* tfull_bar = bars + 2 * STAGES;   // both
+  uint64_t* tempty_bar = tfull_bar + 2;      // leader's is used
+  uint64_t* mma_done_bar = tempty_bar + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(mma_done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  static_assert((2 * STAGES + 5) * 8 + 8 <= 256, "barrier area");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int cluster_id = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  if (!powers_of_two(p)) {  // the whole grid; the launch behind this one counts on the quantiser's end
+    wait_for_primary();
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1 + 2 * 4);  // the operands, the scale warps of both CTAs
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 2 * 4);  // output warps of both CTAs
+    }
+    mbar_init(mma_done_bar, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before any cross-CTA signal
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  bool ok = true;
+  wait_for_primary();  // q and its scales
+
+  if (warp == 0) {  // ---- TMA producer (both CTAs): the whole warp waits, one elected thread issues
+    int stage = 0;
+    uint32_t phase = 0;
+    const uint32_t full0 = leader ? smem_u32(full_bar) : mapa_rank(smem_u32(full_bar), 0);
+    for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
+      int mb, nb;
+      tile_at(p, t, mb, nb);
+      const int row_a = mb * 256 + (int)rank * 128, row_b = nb * BN + (int)rank * (BN / 2);
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        if (!warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+        uint8_t* st = smem + stage * Mx::STAGE;
+        if (elect_one()) {
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Mx::STAGE);
+          tma_load_2d_pair(st, &map_a, full0 + 8 * stage, kb * kBlock, row_a);
+          tma_load_2d_pair(st + kABytes, &map_b, full0 + 8 * stage, kb * kBlock, row_b);
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    if (leader) {  // ---- MMA issuer: the whole warp waits, one elected thread issues
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      const uint32_t base = smem_u32(smem);
+      for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
+        if (!warp_wait(&tempty_bar[buf], buf_phase ^ 1u, abort_flag)) { ok = false; break; }
+        const uint32_t d = tmem_base + (uint32_t)(buf * BN);
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!warp_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t adesc = sdesc_sw128(base + stage * Mx::STAGE);
+          const uint64_t bdesc = sdesc_sw128(base + stage * Mx::STAGE + kABytes);
+          const uint32_t sc = tmem_base + (uint32_t)(Mx::SCALES + 16 * stage);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kBlock / 32; ++k)
+              umma_mx_pair(d, adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), sc, sc + 4u, kb + k != 0);
+            umma_commit_pair(&empty_bar[stage], (uint16_t)3);  // frees the stage in both CTAs
+            if (kb + 1 == p.num_kb) umma_commit_pair(&tfull_bar[buf], (uint16_t)3);
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
+      }
+      if (elect_one()) {
+        umma_commit_pair(mma_done_bar, (uint16_t)1);
+        mbar_drain_wait(mma_done_bar, 0);
+      }
+    }
+  } else if (warp >= 8) {  // ---- scales (both CTAs)
+    const int quarter = warp & 3;
+    const uint32_t full0 = mapa_rank(smem_u32(full_bar), 0);
+    const uint32_t t_warp = tmem_base + ((uint32_t)(quarter * 32) << 16) + Mx::SCALES;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
+      int mb, nb;
+      tile_at(p, t, mb, nb);
+      const int row0 = mb * 256 + (int)rank * 128 + lane, n = nb * BN + lane * 32;  // lanes 0 .. 5: a column each
+      const float* pa[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) pa[c] = row0 + 32 * c < p.M ? p.sx + (row0 + 32 * c) * p.sx_m : nullptr;
+      const float* pb = lane < BN / 32 && n < p.N ? p.sw + (n / kBlock) * p.sw_n : nullptr;
+      float a[Mx::AHEAD][4], b[Mx::AHEAD];  // of the coming K-blocks
+      auto load = [&](int r, int kb) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) a[r][c] = pa[c] && kb < p.num_kb ? __ldg(pa[c] + kb * p.sx_k) : 1.0f;
+        b[r] = pb && kb < p.num_kb ? __ldg(pb + kb * p.sw_k) : 1.0f;
+      };
+#pragma unroll
+      for (int r = 0; r < Mx::AHEAD; ++r) load(r, r);
+      for (int kb0 = 0; kb0 < p.num_kb && ok; kb0 += Mx::AHEAD) {
+#pragma unroll
+        for (int r = 0; r < Mx::AHEAD; ++r) {
+          if (kb0 + r >= p.num_kb) break;
+          uint32_t va[4], b0[4], b1[4];
+          const uint32_t e = exponents(b[r]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            va[c] = exponents(a[r][c]);
+            b0[c] = __shfl_sync(0xFFFFFFFFu, e, c);
+            b1[c] = __shfl_sync(0xFFFFFFFFu, e, 4 + c);
+          }
+          load(r, kb0 + r + Mx::AHEAD);
+          if (!warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t at = t_warp + (uint32_t)(16 * stage);
+          tmem_st4(at, va);
+          tmem_st4(at + 4u, b0);
+          tmem_st4(at + 8u, b1);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_pair(full0 + 8 * stage);
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp >= 4) {  // ---- output (both CTAs)
+    const int quarter = warp & 3;
+    uint8_t* xw = xbuf + (warp - 4) * Mx::XWARP;
+    const uint32_t tempty0 = mapa_rank(smem_u32(tempty_bar), 0);
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
+      int mb, nb;
+      tile_at(p, t, mb, nb);
+      const int row0 = mb * 256 + (int)rank * 128 + quarter * 32, n0 = nb * BN;
+      if (!warp_wait(&tfull_bar[buf], buf_phase, abort_flag)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t ta = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
+#pragma unroll 1
+      for (int c = 0; c < BN / 64; ++c) {
+        uint32_t r0[32], r1[32];
+        tmem_ld32(ta + 64u * c, r0);
+        tmem_ld32(ta + 64u * c + 32u, r1);
+        wait_ld(r0);
+        after_wait(r1);
+        if (c + 1 == BN / 64) {  // read: the accumulator may be filled again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_pair(tempty0 + 8 * buf);
+        }
+        px::f2 v[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[j] = px::mk(__uint_as_float(r0[2 * j]), __uint_as_float(r0[2 * j + 1]));
+          v[16 + j] = px::mk(__uint_as_float(r1[2 * j]), __uint_as_float(r1[2 * j + 1]));
+        }
+        store_tile<T, 64>(p, &map_y, v, xw, row0, n0 + 64 * c, lane);
+      }
+      if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
+    }
+    if (p.tma_store && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+
+  // An aborted CTA gives copies still in flight (the peer's loads complete on the leader's
+  // barrier) a bounded grace period before the CTAs leave.
+  if (__syncthreads_or(ok ? 0 : 1)) {
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 2000000ull) {
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs are done with TMEM and with each other's barriers
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols)
+                 : "memory");
+}
+
 // --- host ------------------------------------------------------------------------
 
 // [rows, cols] row-major with row stride ld_bytes, boxes of 128 bytes x box_rows, 128-byte swizzle
@@ -457,7 +734,8 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, int size, const 
 
 constexpr int64_t kGroupBudget = 48ll << 20;  // L2 bytes for the operand that every wave re-reads
 
-template <typename T, int BN>
+// MX: the tensor cores apply the scales (BN = Mx::BN), or the launch does nothing where they cannot
+template <typename T, int BN, bool MX = false>
 static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K,
                        bool dependent, cudaStream_t st, const char* what) {
   CUtensorMap ta, tb, ty;
@@ -469,12 +747,15 @@ static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, 
     rc = make_map(&ty, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T),
                   p.y, p.N, p.M, p.ldy * (int64_t)sizeof(T), 32u, what);
   if (rc) return rc;
+  void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, GemmParams);
+  int smem;
+  if constexpr (MX) kernel = gemm_mx_kernel<T>, smem = Mx::SMEM;
+  else kernel = gemm_pair_kernel<T, BN>, smem = Cfg<BN>::SMEM;
   static bool set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_pair_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               Cfg<BN>::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     ZIB_HOST_CHECK(e == cudaSuccess, ZIB_ERR_LAUNCH, "%s: cudaFuncSetAttribute failed: %s", what,
                    cudaGetErrorString(e));
     set[dev] = true;
@@ -494,14 +775,14 @@ static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, 
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * clusters);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<BN>::SMEM;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = dependent ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_pair_kernel<T, BN>, ta, tb, ty, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ta, tb, ty, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
     zib_set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
@@ -511,11 +792,23 @@ static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, 
 }
 
 template <typename T>
-static int gemm(const GemmParams& p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K,
-                bool dependent, cudaStream_t st, const char* what) {
+static int gemm(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K, bool dependent,
+                cudaStream_t st, const char* what) {
+  const bool exponents = dependent;  // the scales of q come from the quantiser: powers of two
   // whole waves of 256 x 256 tiles, or twice as many 256 x 128 ones where those end sooner
-  const int64_t pairs = sm_count() / 2, mb = ceil_div(p.M, 256);
+  const int64_t pairs = sm_count() / 2, mb = ceil_div(p.M, 256), kb = ceil_div(K, kBlock);
   const int64_t wide = ceil_div(mb * ceil_div(p.N, 256), pairs) * 2, slim = ceil_div(mb * ceil_div(p.N, 128), pairs);
+  if (exponents) {
+    // the tensor cores apply the scales where that and the second launch, which then ends at once, are
+    // sooner: 0.34 us a wave and K-block and 3 us for the launch, against 0.50 or 0.29 (wide, slim)
+    const int64_t mx = ceil_div(mb * ceil_div(p.N, Mx::BN), pairs);
+    if (300 + 34 * mx * kb < (slim < wide ? 29 * slim : 25 * wide) * kb) {
+      const int rc = launch_pair<T, Mx::BN, true>(p, q, ldq, w, ldw, K, dependent, st, what);
+      if (rc) return rc;
+      p.where = 1;
+      dependent = false;
+    }
+  }
   if (slim < wide) return launch_pair<T, 128>(p, q, ldq, w, ldw, K, dependent, st, what);
   return launch_pair<T, 256>(p, q, ldq, w, ldw, K, dependent, st, what);
 }

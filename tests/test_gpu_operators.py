@@ -882,7 +882,7 @@ def test_linear_groups_of_tokens(cuda, M, K, N, dtype):
     check(fp8_block_linear(x, qw, sw, b), ref + b.double(), product_extra(mag, K, b))
 
 
-@pytest.mark.parametrize("M,K,N", [(600, 1024, 1300), (70, 512, 257), (5, 300, 200)])
+@pytest.mark.parametrize("M,K,N", [(600, 4096, 3840), (600, 1024, 1300), (70, 512, 257), (5, 300, 200)])
 def test_linear_captured_with_its_gradients(cuda, M, K, N):
     """Each of the linear's kernels in a captured forward and backward pass, replayed on other inputs."""
     g = _gen(M)
@@ -910,3 +910,87 @@ def test_linear_captured_with_its_gradients(cuda, M, K, N):
         d.copy_(ins[i][1])
         graph.replay()
         assert all(torch.equal(a, e) for a, e in zip(out, want[i]))
+
+
+# enough tiles and K-blocks that the tensor cores apply the scales where all are powers of two
+MANY_BLOCKS = [(600, 4096, 3840), (1030, 6000, 2001)]
+
+
+def _varied(g, M, K, spread=12):
+    """Values whose 128-blocks differ in size by powers of two."""
+    e = torch.randint(-spread, spread + 1, (M, -(-K // 128)), generator=g, device="cuda").float()
+    return _randn(g, M, K) * torch.exp2(e).repeat_interleave(128, 1)[:, :K]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", MANY_BLOCKS)
+def test_linear_of_many_blocks(cuda, dtype, M, K, N):
+    g = _gen(K)
+    x = _varied(g, M, K, 3).to(dtype)
+    w = _varied(g, N, K, 3) / 64
+    bias = _randn(g, N).to(dtype) if N % 2 else None
+    wq, ws = fp8_block_quantize_weight(w)
+    qx, sx = ref_rows(x)
+    ref, mag = product_terms(qx, sx, wq, ws)
+    check(fp8_block_linear(x, wq, ws, bias), ref if bias is None else ref + bias.double(), product_extra(mag, K, bias))
+    # one scale that is no power of two, of another sign, zero
+    for bad in (0.7, -1.0, 0.0):
+        other = ws.clone()
+        other[-1, -1] = bad
+        ref, mag = product_terms(qx, sx, wq, other)
+        check(fp8_block_linear(x, wq, other), ref, product_extra(mag, K))
+    assert _lib.device_error_read_clear() == 0
+
+
+def test_linear_of_many_blocks_sums_in_32_bits(cuda):
+    M, K, N = 600, 4096, 3840
+    x = torch.full((M, K), 2.0 ** -6, device="cuda")
+    x[:, ::128], x[:, 1::128] = 448.0, -448.0
+    x[:, 3], x[:, 260] = 256.0, -256.0
+    y = fp8_block_linear(x, torch.ones(N, K, device="cuda").to(torch.float8_e4m3fn), torch.ones(30, 32, device="cuda"))
+    assert bool((y == (K - 66) * 2.0 ** -6).all()), float((y - (K - 66) * 2.0 ** -6).abs().max())
+
+
+@pytest.mark.parametrize("ex,ew", [(-110, 100), (100, -110), (-60, -60), (60, 60), (-110, 0), (0, 100)])
+def test_linear_of_many_blocks_far_exponents(cuda, ex, ew):
+    M, K, N = 600, 4096, 3840
+    g = _gen(5)
+    x, w = _randn(g, M, K), _randn(g, N, K)
+    wq, ws = fp8_block_quantize_weight(w)
+    qx, sx = ref_rows(x)
+    ref, mag = product_terms(qx, sx, wq, ws)
+    y = fp8_block_linear(x * 2.0 ** ex, wq, ws * 2.0 ** ew)
+    # Compared as they are.  With 60 and 60 an output is 2^120 times a sum whose partial sums, in fp32 like it, reach
+    # 2^8 = 2^128 / 2^120 where fp32 ends: no partial sum is larger than the sum of magnitudes, so an infinity
+    # is right where that times 2^120 is at least 2^128, and nowhere else.
+    f = 2.0 ** (ex + ew)
+    over = torch.isinf(y) & (mag * f >= 2.0 ** 128)
+    check(torch.where(over, torch.zeros_like(y), y), torch.where(over, torch.zeros_like(ref), ref * f),
+          product_extra(mag, K) * f)
+
+
+def test_linear_of_many_blocks_non_finite(cuda):
+    M, K, N = 600, 4096, 3840
+    g = _gen(6)
+    x, w = _randn(g, M, K).to(torch.bfloat16), _randn(g, N, K)
+    x[17, 300], x[599, 4095] = math.inf, math.nan
+    wq, ws = fp8_block_quantize_weight(w)
+    bad = torch.isnan(fp8_block_linear(x, wq, ws))
+    assert bool(bad[17].all()) and bool(bad[599].all()) and int(bad.sum()) == 2 * N
+    w[200, 5] = math.inf
+    wq, ws = fp8_block_quantize_weight(w)
+    bad = torch.isnan(fp8_block_linear(x, wq, ws))
+    assert bool(bad[:, 128:256].all()) and int(bad.sum()) == 2 * N + 128 * (M - 2)
+
+
+def test_linear_of_many_blocks_gradients(cuda):
+    M, K, N = 640, 4096, 3840
+    g = _gen(7)
+    x = _randn(g, M, K).to(torch.bfloat16).requires_grad_()
+    b = _randn(g, N).to(torch.bfloat16).requires_grad_()
+    wq, ws = fp8_block_quantize_weight(_varied(g, N, K, 3) / 64)
+    dy = _varied(g, M, N, 3).to(torch.bfloat16)
+    dx, db = torch.autograd.grad(fp8_block_linear(x, wq, ws, b), (x, b), dy)
+    ref, mag = product_terms(*ref_rows(dy), wq.t(), ws.t())
+    check(dx, ref, product_extra(mag, N))
+    check(db, dy.double().sum(0), (M + 2) * U32 * dy.double().abs().sum(0))
