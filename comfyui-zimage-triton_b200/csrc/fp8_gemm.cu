@@ -221,16 +221,28 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, const CUtensorMa
       }
     } else {
       __syncwarp();
-      for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
-        T* dst = reinterpret_cast<T*>(p.y) + (int64_t)(row0 + r) * p.ldy;
+      // rows that start on any element: single elements, a few rows' reads under way at a time (18226 x 4071 x
+      // 640: 100 us, 190 one after the other, 166 in pairs where a row's parity allows)
+      constexpr int RUN = 4;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32 && row0 + r0 < p.M; r0 += RUN) {
 #pragma unroll
         for (int b = 0; b < PER; ++b) {
-          const int col = n0 + (b0 + b) * BOXC;
-          for (int e = lane; e < BOXC && col + e < p.N; e += 32) {
-            const int at = e * (int)sizeof(T);
-            dst[col + e] = *reinterpret_cast<const T*>(xw + b * 4096 + r * 128 + (((at >> 4) ^ (r & 7)) << 4) +
-                                                       (at & 15));
-          }
+          const int col = n0 + (b0 + b) * BOXC + lane;
+          T v[RUN][BOXC / 32];
+#pragma unroll
+          for (int i = 0; i < RUN; ++i)
+#pragma unroll
+            for (int e = 0; e < BOXC / 32; ++e) {
+              const int r = r0 + i, at = (lane + 32 * e) * (int)sizeof(T);
+              v[i][e] = *reinterpret_cast<const T*>(xw + b * 4096 + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+            }
+          T* dst = reinterpret_cast<T*>(p.y) + (int64_t)(row0 + r0) * p.ldy + col;
+#pragma unroll
+          for (int i = 0; i < RUN; ++i)
+#pragma unroll
+            for (int e = 0; e < BOXC / 32; ++e)
+              if (row0 + r0 + i < p.M && col + 32 * e < p.N) dst[i * p.ldy + 32 * e] = v[i][e];
         }
       }
       __syncwarp();
