@@ -172,9 +172,10 @@ __device__ __forceinline__ void add_scaled(px::f2 (&acc)[N2], int at, const uint
 
 // This thread's CW columns of row `row` to y, through the warp's staging boxes (32 rows x 128 bytes,
 // 16-byte chunk c of row r at c ^ (r & 7): the TMA's 128-byte swizzle).
-template <typename T, int CW>
+template <typename T, int CW, bool SB = false>
 __device__ __forceinline__ void store_tile(const GemmParams& p, const CUtensorMap* map_y, px::f2 (&acc)[CW / 2],
-                                           uint8_t* xw, int row0, int n0, int lane) {
+                                           uint8_t* xw, int row0, int n0, int lane,
+                                           const float* sbias = nullptr) {
   constexpr int BOXC = 128 / sizeof(T);            // columns per box
   constexpr int BOXES = CW / BOXC;                 // boxes of this warp's part
   constexpr int PER = BOXES < 2 ? BOXES : 2;       // staged at a time
@@ -194,11 +195,23 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, const CUtensorMa
         float v[EC];
 #pragma unroll
         for (int j = 0; j < EC; j += 2) px::split(acc[(col + c * EC + j) / 2], v[j], v[j + 1]);
-        if (p.bias) {
+        if constexpr (SB) {  // the bias of these columns in shared memory
 #pragma unroll
-          for (int j = 0; j < EC; ++j) {
-            const int n = n0 + col + c * EC + j;
-            if (n < p.N) v[j] += to_f32(reinterpret_cast<const T*>(p.bias)[n]);
+          for (int j = 0; j < EC; j += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(sbias + col + c * EC + j);
+            v[j] += t.x, v[j + 1] += t.y, v[j + 2] += t.z, v[j + 3] += t.w;
+          }
+        } else if (p.bias) {
+          const int n = n0 + col + c * EC;
+          const T* from = reinterpret_cast<const T*>(p.bias) + n;
+          if (reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && n + EC <= p.N) {
+            const Pack<T, EC> t = *reinterpret_cast<const Pack<T, EC>*>(from);
+#pragma unroll
+            for (int j = 0; j < EC; ++j) v[j] += to_f32(t.v[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < EC; ++j)
+              if (n + j < p.N) v[j] += to_f32(from[j]);
           }
         }
         uint4 o;
@@ -493,7 +506,8 @@ struct Mx {
   static constexpr int AHEAD = 6;  // K-blocks whose scales are on their way
   static constexpr int XWARP = 8192;
   static constexpr int SCALES = 2 * BN;  // first TMEM column of the scales
-  static constexpr int SMEM = STAGES * STAGE + 4 * XWARP + 256 + 1024;
+  static constexpr int BIAS = BN * 4;  // bytes of a warp's copy of a tile's bias
+  static constexpr int SMEM = STAGES * STAGE + 4 * (XWARP + BIAS) + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory per CTA");
   static_assert(SCALES + 16 * STAGES <= kTmemCols, "TMEM columns");
   // D = f32, A = B = e4m3, both K-major, scales of 8 exponent bits, the first byte of their words
@@ -525,7 +539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* xbuf = smem + STAGES * Mx::STAGE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xbuf + 4 * Mx::XWARP);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xbuf + 4 * (Mx::XWARP + Mx::BIAS));
   uint64_t* full_bar = bars;                 // leader's is used
   uint64_t* empty_bar = bars + STAGES;       // both
   uint64_t* tfull_bar = bars + 2 * STAGES;   // both
@@ -675,6 +689,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp >= 4) {  // ---- output (both CTAs)
     const int quarter = warp & 3;
     uint8_t* xw = xbuf + (warp - 4) * Mx::XWARP;
+    float* sbias = reinterpret_cast<float*>(xbuf + 4 * Mx::XWARP + (warp - 4) * Mx::BIAS);
     const uint32_t tempty0 = mapa_rank(smem_u32(tempty_bar), 0);
     int buf = 0;
     uint32_t buf_phase = 0;
@@ -682,6 +697,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int mb, nb;
       tile_at(p, t, mb, nb);
       const int row0 = mb * 256 + (int)rank * 128 + quarter * 32, n0 = nb * BN;
+      __syncwarp();
+#pragma unroll
+      for (int c = lane; c < BN; c += 32)
+        sbias[c] = p.bias && n0 + c < p.N ? to_f32(reinterpret_cast<const T*>(p.bias)[n0 + c]) : 0.0f;
+      __syncwarp();
       if (!warp_wait(&tfull_bar[buf], buf_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
       const uint32_t ta = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
@@ -703,7 +723,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           v[j] = px::mk(__uint_as_float(r0[2 * j]), __uint_as_float(r0[2 * j + 1]));
           v[16 + j] = px::mk(__uint_as_float(r1[2 * j]), __uint_as_float(r1[2 * j + 1]));
         }
-        store_tile<T, 64>(p, &map_y, v, xw, row0, n0 + 64 * c, lane);
+        store_tile<T, 64, true>(p, &map_y, v, xw, row0, n0 + 64 * c, lane, sbias + 64 * c);
       }
       if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
     }
