@@ -54,7 +54,9 @@ struct Cfg {
   static constexpr int STAGE = kABytes + BN / 2 * kBlock;
   static constexpr int STAGES = BN == 256 ? 5 : 6;
   static constexpr int XWARP = 8192;  // output staging per warp: two boxes of 32 rows x 128 bytes
-  static constexpr int SMEM = STAGES * STAGE + kEpiWarps * XWARP + 256 + 1024;
+  // bytes of a warp's copy of its bias; tiles of 256 columns leave no room for one
+  static constexpr int BIAS = BN == 128 ? BN / 2 * 4 : 0;
+  static constexpr int SMEM = STAGES * STAGE + kEpiWarps * (XWARP + BIAS) + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
@@ -195,7 +197,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, const CUtensorMa
         float v[EC];
 #pragma unroll
         for (int j = 0; j < EC; j += 2) px::split(acc[(col + c * EC + j) / 2], v[j], v[j + 1]);
-        if constexpr (SB) {  // the bias of these columns in shared memory
+        if (SB && p.bias) {  // the bias of these columns is in shared memory
 #pragma unroll
           for (int j = 0; j < EC; j += 4) {
             const float4 t = *reinterpret_cast<const float4*>(sbias + col + c * EC + j);
@@ -286,7 +288,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* xbuf = smem + STAGES * C::STAGE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xbuf + kEpiWarps * C::XWARP);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xbuf + kEpiWarps * (C::XWARP + C::BIAS));
   uint64_t* full_bar = bars;                       // leader's is used
   uint64_t* empty_bar = bars + STAGES;             // both
   uint64_t* tfull_bar = bars + 2 * STAGES;         // both
@@ -400,6 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ---- sums over K-blocks and output (both CTAs)
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     uint8_t* xw = xbuf + (warp - 4) * C::XWARP;
+    float* sbias = reinterpret_cast<float*>(xbuf + kEpiWarps * C::XWARP + (warp - 4) * C::BIAS);
     const uint32_t tempty0 = mapa_rank(smem_u32(tempty_bar), 0);
     const uint32_t t_warp = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * CW);
     int buf = 0;
@@ -421,6 +424,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (cluster_id < p.num_tiles) locate(cluster_id);
     for (int t = cluster_id; t < p.num_tiles && ok; t += nclusters) {
       const int row0 = mb * 256 + (int)rank * 128 + quarter * 32, n0 = nb * BN + half * CW;
+      if (C::BIAS > 0 && p.bias) {
+        __syncwarp();
+#pragma unroll
+        for (int c = lane; c < CW; c += 32)
+          sbias[c] = n0 + c < p.N ? to_f32(reinterpret_cast<const T*>(p.bias)[n0 + c]) : 0.0f;
+        __syncwarp();
+      }
       px::f2 acc[CW / 2];
 #pragma unroll
       for (int j = 0; j < CW / 2; ++j) acc[j] = 0ull;
@@ -457,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (t + nclusters < p.num_tiles) locate(t + nclusters);
-      store_tile<T, CW>(p, &map_y, acc, xw, row0, n0, lane);
+      store_tile<T, CW, (C::BIAS > 0)>(p, &map_y, acc, xw, row0, n0, lane, sbias);
     }
     if (!ok) aborted = true;
     if (p.tma_store && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -697,11 +707,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int mb, nb;
       tile_at(p, t, mb, nb);
       const int row0 = mb * 256 + (int)rank * 128 + quarter * 32, n0 = nb * BN;
-      __syncwarp();
+      if (p.bias) {
+        __syncwarp();
 #pragma unroll
-      for (int c = lane; c < BN; c += 32)
-        sbias[c] = p.bias && n0 + c < p.N ? to_f32(reinterpret_cast<const T*>(p.bias)[n0 + c]) : 0.0f;
-      __syncwarp();
+        for (int c = lane; c < BN; c += 32)
+          sbias[c] = n0 + c < p.N ? to_f32(reinterpret_cast<const T*>(p.bias)[n0 + c]) : 0.0f;
+        __syncwarp();
+      }
       if (!warp_wait(&tfull_bar[buf], buf_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
       const uint32_t ta = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
