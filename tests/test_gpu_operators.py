@@ -994,3 +994,17 @@ def test_linear_of_many_blocks_gradients(cuda):
     ref, mag = product_terms(*ref_rows(dy), wq.t(), ws.t())
     check(dx, ref, product_extra(mag, N))
     check(db, dy.double().sum(0), (M + 2) * U32 * dy.double().abs().sum(0))
+
+
+def test_gradients_of_dual_gradients_are_refused(cuda):
+    """Forward over reverse: a tangent of the upstream gradient would be lost."""
+    fw = torch.autograd.forward_ad
+    g = _gen(91)
+    wq, ws = fp8_block_quantize_weight(_randn(g, 32, 64))
+    cos, sin = table(4, 32)
+    x = _randn(g, 1, 4, 2, 64).requires_grad_()
+    for y in (fp8_block_linear(x, wq, ws), group_norm_act(x, 4), rotary_embed(x, None, cos, sin)[0]):
+        with fw.dual_level():
+            d = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad(y, (x,), d)

@@ -165,3 +165,23 @@ def test_fp8_block_linear_keeps_its_weight_through_casts(cast):
     assert m.bias.dtype == want
     assert m.w_q.dtype == m.w_q_t.dtype == torch.float8_e4m3fn and m.w_scale.dtype == torch.float32
     assert torch.equal(m.w_q.view(torch.uint8), q.view(torch.uint8)) and torch.equal(m.w_scale, s)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor that requires no gradient: the output would have no tangent, and nothing would say so."""
+    fw = torch.autograd.forward_ad
+    x, c = torch.ones(1, 2, 2, 8), torch.ones(2, 4)
+    w, s = torch.zeros(4, 8).to(E4M3), torch.ones(1, 1)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: fp8_block_linear(dual(x), w, s), lambda: fp8_block_linear(x, w, s, dual(torch.zeros(4))),
+                     lambda: fp8_block_linear(x, w, dual(s)), lambda: rotary_embed(dual(x), None, c, c),
+                     lambda: rotary_embed(x, dual(x), c, c), lambda: rotary_embed(x, None, c, dual(c)),
+                     lambda: group_norm_act(dual(x), 2), lambda: group_norm_act(x, 2, dual(torch.ones(8))),
+                     lambda: group_norm_act(x, 2, None, dual(torch.ones(8)))):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+            with fw._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):
+                call()
