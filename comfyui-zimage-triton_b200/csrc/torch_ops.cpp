@@ -8,11 +8,13 @@
 //
 // ValueError: operands that do not go together, wrong types, tensors that are not on an sm_100 GPU.
 // RuntimeError: sizes beyond the supported ones, failed launches, a second or a forward-mode derivative
-// that does not exist.
+// that does not exist, calls under a tracer.
 #include <torch/extension.h>
 
 #include <ATen/TensorUtils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -67,6 +69,15 @@ void same_device(const Tensor& t, const Tensor& o) {
 }
 void same_device(const Tensor& t, const OptTensor& o) {
   if (o) same_device(t, *o);
+}
+
+// A tracer records torch's own operations alone: of a call here the allocation of its output and not the
+// kernel, so the replay would return memory that nothing has written.
+void not_traced(const char* what) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !(Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY)),
+              what, " cannot be traced (torch.jit.trace, make_fx): its kernels are not in the trace");
 }
 
 // A dual tensor need not require a gradient, so autograd does not see it: the kernel's output would
@@ -134,6 +145,7 @@ Tensor rows_of(const Tensor& x, int64_t K, int64_t& ld) {
 }
 
 std::tuple<Tensor, Tensor> fp8_block_quantize(const Tensor& x) {
+  not_traced("fp8_block_quantize");
   const int dt = dtype_of(x, "x");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must be [..., K] with K >= 1, got ", x.sizes());
   require_device(x);
@@ -153,6 +165,7 @@ std::tuple<Tensor, Tensor> fp8_block_quantize(const Tensor& x) {
 }
 
 std::tuple<Tensor, Tensor> fp8_block_quantize_weight(const Tensor& w) {
+  not_traced("fp8_block_quantize_weight");
   const int dt = dtype_of(w, "w");
   TORCH_CHECK_VALUE(w.dim() == 2 && w.numel() > 0, "w must be a non-empty [N, K], got ", w.sizes());
   require_device(w);
@@ -168,6 +181,7 @@ std::tuple<Tensor, Tensor> fp8_block_quantize_weight(const Tensor& w) {
 }
 
 Tensor fp8_block_transpose(const Tensor& w_q) {
+  not_traced("fp8_block_transpose");
   TORCH_CHECK_VALUE(w_q.dim() == 2 && w_q.scalar_type() == kE4M3 && w_q.numel() > 0,
                     "w_q must be a non-empty e4m3 [N, K], got ", w_q.scalar_type(), " ", w_q.sizes());
   require_device(w_q);
@@ -195,6 +209,7 @@ int64_t check_weight(int64_t K, const Tensor& w_q, const Tensor& w_scale, const 
 
 Tensor fp8_block_matmul(const Tensor& x_q, const Tensor& x_scale, const Tensor& w_q, const Tensor& w_scale,
                         const OptTensor& bias, at::ScalarType out) {
+  not_traced("fp8_block_matmul");
   TORCH_CHECK_VALUE(x_q.dim() >= 1 && x_q.scalar_type() == kE4M3 && x_q.size(-1) >= 1,
                     "x_q must be e4m3 [..., K], got ", x_q.scalar_type(), " ", x_q.sizes());
   const int64_t K = x_q.size(-1), M = x_q.numel() / K, kb = ceil_div(K, kBlock);
@@ -279,6 +294,7 @@ struct Linear : torch::autograd::Function<Linear> {
 
 Tensor fp8_block_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scale, const OptTensor& bias_,
                         const OptTensor& w_q_t) {
+  not_traced("fp8_block_linear");
   no_tangent("fp8_block_linear", x, w_scale, bias_);
   dtype_of(x, "x");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must be [..., K] with K >= 1, got ", x.sizes());
@@ -383,6 +399,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 
 std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, const Tensor& cos_, const Tensor& sin_,
                                            const OptTensor& positions_, bool half) {
+  not_traced("rotary_embed");
   no_tangent("rotary_embed", q, k, cos_, sin_);
   TORCH_CHECK_VALUE(q.dim() == 4, "q must be [B, S, H, D], got ", q.sizes());
   const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
@@ -437,6 +454,7 @@ std::tuple<Tensor, OptTensor> rotary_embed(const Tensor& q, const OptTensor& k, 
 std::tuple<Tensor, Tensor> rotary_table(const OptTensor& positions, int64_t T, at::Device device, int64_t dim,
                                         double theta, int scaling, double factor, double original, double beta_fast,
                                         double beta_slow, double attention_factor) {
+  not_traced("rotary_table");
   if (positions) {
     TORCH_CHECK_VALUE(positions->dim() == 1 && (positions->scalar_type() == at::kInt ||
                                                 positions->scalar_type() == at::kLong),
@@ -537,6 +555,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 constexpr int64_t kMaxChannels = 8192;
 
 Tensor group_norm_act(const Tensor& x, int64_t G, const OptTensor& w_, const OptTensor& b_, double eps, int64_t act) {
+  not_traced("group_norm_act");
   no_tangent("group_norm_act", x, w_, b_);
   TORCH_CHECK_VALUE(x.dim() >= 2, "x must be [B, ..., C], got ", x.sizes());
   const int64_t C = x.size(-1);

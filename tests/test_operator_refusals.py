@@ -185,3 +185,21 @@ def test_forward_mode_derivatives_are_refused():
                 call()
             with fw._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):
                 call()
+
+
+def test_tracing_is_refused():
+    """A trace would hold the allocation of the output without the kernel that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, c = torch.ones(1, 2, 2, 8), torch.ones(2, 4)
+    w, s = torch.zeros(4, 8).to(E4M3), torch.ones(1, 1)
+    xq, xs = torch.zeros(3, 8).to(E4M3), torch.ones(3, 1)
+    for call in (lambda t: fp8_block_quantize(t), lambda t: fp8_block_quantize_weight(t[0, 0]),
+                 lambda t: fp8_block_transpose(w), lambda t: fp8_block_matmul(xq, xs, w, s),
+                 lambda t: fp8_block_linear(t, w, s), lambda t: rotary_embed(t, None, c, c)[0],
+                 lambda t: rotary_table(torch.arange(4), 8), lambda t: rotary_table(4, 8),
+                 lambda t: group_norm_act(t, 2), Fp8BlockLinear(8, 4), GroupNormAct(2, 8)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (x,))
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(call)(x)
