@@ -333,11 +333,12 @@ std::tuple<Tensor, Tensor> rotate(const Tensor& q, const Tensor& k, const Tensor
     if (!t.defined()) continue;
     Side& s = side[i];
     s.x = t;
-    // features side by side; interleaved, a pair is one access
+    // features side by side; interleaved, a pair is one access (a copy even of a contiguous tensor that
+    // starts between two pairs)
     if ((t.stride(3) != 1 && D != 1) ||
         (!half && (((t.stride(0) | t.stride(1) | t.stride(2)) & 1) ||
                    reinterpret_cast<uintptr_t>(t.data_ptr()) % (2 * esize))))
-      s.x = t.contiguous();
+      s.x = t.clone(at::MemoryFormat::Contiguous);
     s.out = at::empty(t.sizes(), t.options());
     s.sb = s.x.stride(0), s.ss = s.x.stride(1), s.sh = s.x.stride(2), s.H = t.size(2);
   }

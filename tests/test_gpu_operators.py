@@ -1008,3 +1008,32 @@ def test_gradients_of_dual_gradients_are_refused(cuda):
             d = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
             with pytest.raises(RuntimeError, match="no forward-mode derivative"):
                 torch.autograd.grad(y, (x,), d)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_rotary_contiguous_tensors_at_odd_offsets(cuda, layout, dtype, off):
+    """Queries, keys and upstream gradients that are contiguous but start on any element."""
+    B, S, H, D = 2, 5, 3, 32
+    g = _gen(off)
+
+    def at_offset(h):
+        buf = _randn(g, B * S * h * D + off).to(dtype)[off:].view(B, S, h, D)
+        assert buf.is_contiguous() and buf.data_ptr() % 16 == off * buf.element_size() % 16
+        return buf
+
+    q, k, dq, dk = (at_offset(h) for h in (H, 1, H, 1))
+    cos, sin = table(S, 10)
+    q.requires_grad_(), k.requires_grad_()
+    outs = rotary_embed(q, k, cos, sin, layout=layout)
+    grads = torch.autograd.grad(outs, (q, k), (dq, dk))
+    c2, s2 = cos.expand(B, -1, -1), sin.expand(B, -1, -1)
+    for x, o, d, gr in zip((q, k), outs, (dq, dk), grads):
+        ref, mag = ref_rotary(x.detach(), c2, s2, layout)
+        check(o.detach(), ref, 2 * U32 * mag)
+        ref, mag = ref_rotary(d, c2, -s2, layout)
+        check(gr, ref, 2 * U32 * mag)
+    # in the mixed case one of the two alone is copied
+    a, b = rotary_embed(q.detach(), k.detach().clone(), cos, sin, layout=layout)
+    assert torch.equal(a, outs[0]) and torch.equal(b, outs[1])
