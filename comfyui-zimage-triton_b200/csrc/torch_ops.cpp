@@ -115,11 +115,15 @@ Tensor e4m3_rows(int64_t rows, int64_t cols, const Tensor& like) {
 }
 int64_t ld_of(const Tensor& t) { return t.size(0) <= 1 ? round_up(t.size(1), 16) : t.stride(0); }
 
-// 8-bit [R, C] with contiguous columns and 16-byte aligned rows: q itself, or a copy
+// 8-bit [R, C] with contiguous columns and 16-byte aligned rows: q itself, or a copy.  The products for few
+// tokens read whole 16-byte pieces, so the last row's last one has to lie within the storage too.
 Tensor aligned(const Tensor& q) {
-  const bool cols = q.stride(1) == 1 || q.size(1) == 1;
-  const bool rows = q.size(0) <= 1 || (q.stride(0) % 16 == 0 && q.stride(0) >= q.size(1));
-  if (cols && rows && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0) return q;
+  const int64_t R = q.size(0), C = q.size(1);
+  const bool cols = q.stride(1) == 1 || C == 1;
+  const bool rows = R <= 1 || (q.stride(0) % 16 == 0 && q.stride(0) >= C);
+  const bool inside = C % 16 == 0 || R == 0 ||
+                      q.storage_offset() + (R - 1) * q.stride(0) + round_up(C, 16) <= (int64_t)q.storage().nbytes();
+  if (cols && rows && inside && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0) return q;
   Tensor t = e4m3_rows(q.size(0), q.size(1), q);
   if (cols) {
     On on(q);

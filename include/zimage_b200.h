@@ -345,7 +345,9 @@ ZIB_API int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int6
  * and bias of `dtype`.  sum (may be NULL): the sums of x's columns, [K] of dtype, from
  * the same pass over x (the bias gradient where x is dy).  scratch:
  * zib_fp8_block_linear_scratch(M, K, sum != NULL) bytes, 128-byte aligned; 0 bytes for
- * one or two rows without sums, which run as one launch. */
+ * one or two rows without sums, which run as one launch.  The rows of w are read in
+ * whole 16-byte pieces: also its last row's memory has to reach the next multiple of 16
+ * bytes (what lies behind a row's end does not matter). */
 ZIB_API int64_t zib_fp8_block_linear_scratch(int64_t M, int64_t K, int with_sum);
 ZIB_API int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const void* w, int64_t ldw,
                          const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y,

@@ -1037,3 +1037,25 @@ def test_rotary_contiguous_tensors_at_odd_offsets(cuda, layout, dtype, off):
     # in the mixed case one of the two alone is copied
     a, b = rotary_embed(q.detach(), k.detach().clone(), cos, sin, layout=layout)
     assert torch.equal(a, outs[0]) and torch.equal(b, outs[1])
+
+
+@pytest.mark.parametrize("M", [1, 3, 40])
+@pytest.mark.parametrize("N,K", [(1, 17), (1, 8), (1, 250), (5, 100), (40, 1000)])
+def test_weight_rows_that_end_with_their_storage(cuda, M, N, K):
+    """A one-row weight, and padded rows whose last one has nothing behind it."""
+    g = _gen(N + K)
+    ld = (K + 15) // 16 * 16
+    w = torch.empty((N - 1) * ld + K, dtype=torch.float8_e4m3fn, device="cuda").as_strided((N, K), (ld, 1))
+    wq, ws = fp8_block_quantize_weight(_randn(g, N, K))
+    w.copy_(wq)
+    assert w.untyped_storage().nbytes() == (N - 1) * ld + K
+    x = _randn(g, M, K).to(torch.bfloat16).requires_grad_()
+    y = fp8_block_linear(x, w, ws)
+    ref, mag = product_terms(*ref_rows(x.detach()), wq, ws)
+    check(y.detach(), ref, product_extra(mag, K))
+    d = _randn(g, M, N).to(torch.bfloat16)
+    (dx,) = torch.autograd.grad(y, (x,), d)
+    ref, mag = product_terms(*ref_rows(d), wq.t(), ws.t())
+    check(dx, ref, product_extra(mag, N))
+    assert torch.equal(fp8_block_matmul(*fp8_block_quantize(x.detach()), w, ws),
+                       fp8_block_matmul(*fp8_block_quantize(x.detach()), wq, ws))
