@@ -62,10 +62,19 @@ def fp8_block_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, 
     return _lib.ops().fp8_block_linear(x, w_q, w_scale, bias, w_q_t)
 
 
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """t [R, C] of 8-bit values with rows on 16-byte boundaries, as the products read them: itself or a copy."""
+    if t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] and (t.stride(1) == 1 or t.shape[1] == 1):
+        return t
+    return t.new_zeros(t.shape[0], -(-t.shape[1] // 16) * 16)[:, :t.shape[1]].copy_(t)
+
+
 class Fp8BlockLinear(torch.nn.Module):
     """A frozen linear layer on a block-quantised weight, differentiable in its input and bias.
 
     ``transposed=True`` keeps the weight laid out for the input's gradient too (another byte a weight).
+    The weight's rows start on 16-byte boundaries, also after loading, casts and moves between devices, so
+    that no call copies it; where a width is no multiple of 16 its buffers are views of padded rows.
     """
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, transposed: bool = False,
@@ -74,10 +83,10 @@ class Fp8BlockLinear(torch.nn.Module):
         self.in_features, self.out_features = in_features, out_features
         blocks = (-(-out_features // BLOCK), -(-in_features // BLOCK))
         kw = dict(device=device)
-        self.register_buffer("w_q", torch.zeros(out_features, in_features, dtype=torch.float8_e4m3fn, **kw))
+        zeros = lambda *shape: _aligned_rows(torch.zeros(*shape, dtype=torch.float8_e4m3fn, **kw))  # noqa: E731
+        self.register_buffer("w_q", zeros(out_features, in_features))
         self.register_buffer("w_scale", torch.ones(blocks, dtype=torch.float32, **kw))
-        self.register_buffer("w_q_t", torch.zeros(in_features, out_features, dtype=torch.float8_e4m3fn, **kw)
-                             if transposed else None)
+        self.register_buffer("w_q_t", zeros(in_features, out_features) if transposed else None)
         self.bias = torch.nn.Parameter(torch.zeros(out_features, dtype=dtype, **kw)) if bias else None
 
     @classmethod
@@ -97,7 +106,17 @@ class Fp8BlockLinear(torch.nn.Module):
         for k, t in kept.items():
             if self._buffers[k].dtype != t.dtype:
                 self._buffers[k] = t.to(self._buffers[k].device)
+        self._lay_out()  # a move packs padded rows
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._lay_out()  # assign=True takes the loaded tensors as they are
+
+    def _lay_out(self):
+        for k in ("w_q", "w_q_t"):
+            if self._buffers[k] is not None:
+                self._buffers[k] = _aligned_rows(self._buffers[k])
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return fp8_block_linear(x, self.w_q, self.w_scale, self.bias, self.w_q_t)

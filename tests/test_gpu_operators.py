@@ -1059,3 +1059,19 @@ def test_weight_rows_that_end_with_their_storage(cuda, M, N, K):
     check(dx, ref, product_extra(mag, N))
     assert torch.equal(fp8_block_matmul(*fp8_block_quantize(x.detach()), w, ws),
                        fp8_block_matmul(*fp8_block_quantize(x.detach()), wq, ws))
+
+
+@pytest.mark.parametrize("K,N", [(300, 200), (129, 70), (64, 1)])
+def test_fp8_block_linear_module_moved_and_loaded(cuda, K, N):
+    """To the host and back, and into a layer of the constructor's: the same results from aligned rows."""
+    g = _gen(K)
+    lin = torch.nn.Linear(K, N, device="cuda", dtype=torch.bfloat16)
+    m = Fp8BlockLinear.from_linear(lin, transposed=True)
+    x = _randn(g, 7, K).to(torch.bfloat16).requires_grad_()
+    y = m(x)
+    (dx,) = torch.autograd.grad(y.sum(), (x,))
+    other = Fp8BlockLinear(K, N, transposed=True, device="cuda")
+    other.load_state_dict(m.state_dict())
+    for n in (other, m.cpu().cuda()):
+        assert all(t.stride(0) % 16 == 0 and t.stride(1) == 1 for t in (n.w_q, n.w_q_t))
+        assert torch.equal(n(x), y) and torch.equal(torch.autograd.grad(n(x).sum(), (x,))[0], dx)

@@ -1,4 +1,5 @@
-"""What the block-scaled 8-bit products, rotary positions and group normalisation refuse, before any launch."""
+"""The operators' host side: what the block-scaled 8-bit products, rotary positions and group normalisation refuse
+before any launch, and how the linear layer keeps its weight."""
 
 import math
 
@@ -203,3 +204,40 @@ def test_tracing_is_refused():
             torch.jit.trace(call, (x,))
         with pytest.raises(RuntimeError, match="cannot be traced"):
             make_fx(call)(x)
+
+
+@pytest.mark.parametrize("K,N", [(130, 70), (64, 33), (17, 1), (1, 17), (128, 256)])
+def test_fp8_block_linear_keeps_its_rows_aligned(K, N):
+    """Through the constructor, loading (copied and assigned), casts, moves, copies and files."""
+    import copy
+    import io
+
+    def check(m):
+        for t in (m.w_q, m.w_q_t):
+            assert t.dtype == E4M3 and t.stride(0) % 16 == 0 and t.stride(1) == 1
+            assert t.device.type == "meta" or t.data_ptr() % 16 == 0
+        return m
+
+    dense = {"w_q": torch.randint(0, 100, (N, K), dtype=torch.uint8).view(E4M3), "w_scale": torch.rand(-(-N // 128), -(-K // 128)),
+             "bias": torch.zeros(N, dtype=torch.bfloat16)}
+    dense["w_q_t"] = dense["w_q"].t().contiguous()
+    check(Fp8BlockLinear(K, N, transposed=True, device="meta"))
+    new = lambda: check(Fp8BlockLinear(K, N, transposed=True))  # noqa: E731
+    made = []
+    for assign in (False, True):
+        m = new()
+        m.load_state_dict(dense, assign=assign)
+        made.append(check(m))
+    m = Fp8BlockLinear(K, N, transposed=True, device="meta").to_empty(device="cpu")
+    check(m).load_state_dict(made[0].state_dict())
+    buf = io.BytesIO()
+    torch.save(m.state_dict(), buf)
+    buf.seek(0)
+    n = new()
+    n.load_state_dict(torch.load(buf, weights_only=True), assign=True)
+    made += [m, n, copy.deepcopy(m), copy.deepcopy(m).half(), torch.nn.Sequential(copy.deepcopy(m)).to(torch.float32)[0]]
+    for m in made:
+        check(m)
+        for t, k in ((m.w_q, "w_q"), (m.w_q_t, "w_q_t")):
+            assert torch.equal(t.contiguous().view(torch.uint8), dense[k].view(torch.uint8))
+    check(copy.deepcopy(made[0]).to("meta"))
