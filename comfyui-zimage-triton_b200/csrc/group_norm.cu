@@ -134,11 +134,15 @@ __device__ __forceinline__ f2 slope(f2 z, int act) {
 
 // --- a thread's share of a CTA's pixels -------------------------------------------
 
+// Batch entries lie along y and z of the grid (batch_grid): any number of them, the last z's surplus
+// without work (whole clusters, which leave before their first barrier).
+__device__ __forceinline__ int64_t batch_entry() { return (int64_t)blockIdx.z * gridDim.y + blockIdx.y; }
+
 struct Slab {
   int64_t b, p0, p1;  // batch entry, pixels [p0, p1)
   int vl, r;          // column lane, pixel row
   __device__ __forceinline__ Slab(const Params& p, int chunk) {
-    b = blockIdx.y;
+    b = batch_entry();
     vl = threadIdx.x % p.vlanes;
     r = threadIdx.x / p.vlanes;
     p0 = chunk * p.chunk;
@@ -413,6 +417,7 @@ template <typename T, int VEC, int GV, bool FUSED>
 __global__ void __launch_bounds__(kThreads, 2) stats_kernel(const Params p) {
   extern __shared__ double2 sm[];  // [G], then scratch
   const Slab s(p, blockIdx.x);
+  if (s.b >= p.B) return;
   slab_stats<T, VEC, GV>(p, s, sm);
   cluster_barrier();
   if constexpr (FUSED) {
@@ -473,6 +478,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads, 4) apply_kernel(const Params p) {
   __shared__ float mean[kDirectGroups], rstd[kDirectGroups];
   const Slab s = second_pass_slab(p);
+  if (s.b >= p.B) return;
   wait_for_primary();
   if (!p.direct) {
     slab_apply<T, VEC>(p, s, p.mean + s.b * p.G, p.rstd + s.b * p.G);
@@ -626,6 +632,7 @@ __global__ void __launch_bounds__(kThreads, 3) grad_stats_kernel(const Params p)
   extern __shared__ double2 sm[];
   float2* ae = reinterpret_cast<float2*>(sm);  // [C] of this CTA, [C] scratch or the cluster's sums
   const Slab s(p, blockIdx.x);
+  if (s.b >= p.B) return;
   const int rank = (int)tc::cluster_rank();
   const int64_t cl = s.b * p.clusters + blockIdx.x / kCluster;
   slab_grad_stats<T, VEC>(p, s, ae);
@@ -703,13 +710,14 @@ __global__ void __launch_bounds__(kThreads, 3) grad_apply_kernel(const Params p)
   __shared__ float2 coef[kDirectGroups];
   wait_for_primary();
   if ((int)blockIdx.x >= p.chunks) {
-    if (blockIdx.y == 0) {
+    if (batch_entry() == 0) {
       const int warps = (int)blockDim.x >> 5;
       param_grads(p, ((int)blockIdx.x - p.chunks) * warps, ((int)gridDim.x - p.chunks) * warps);
     }
     return;
   }
   const Slab s(p, blockIdx.x);
+  if (s.b >= p.B) return;
   if (!p.direct) {
     slab_grad_apply<T, VEC>(p, s, p.coef + s.b * p.G);
     return;
@@ -740,6 +748,12 @@ static int64_t most_clusters(int64_t B, int64_t P) {
 // One cluster per batch entry is enough up to this many bytes of x: 8 CTAs read 32 KB each in about
 // the time of the second launch that they save.
 constexpr int64_t kFusedBytes = 256 * 1024;
+
+// x CTAs for each of B batch entries
+static dim3 batch_grid(unsigned x, int64_t B) {
+  const int64_t z = ceil_div(B, 65535);
+  return dim3(x, (unsigned)ceil_div(B, z), (unsigned)z);
+}
 
 struct Plan {
   bool fused;
@@ -838,12 +852,12 @@ static int forward_g(Params& p, cudaStream_t st) {
   const size_t stats = (size_t)p.G * (sizeof(double2) + 2 * sizeof(float));
   if (smem < stats) smem = stats;
   ZIB_HOST_CHECK(smem <= kMaxSmem, ZIB_ERR_TOO_LARGE, "%s: %d channels", what, p.C);
-  const dim3 grid(p.chunks, (unsigned)p.B);
+  const dim3 grid = batch_grid(p.chunks, p.B);
   if (pl.fused) return launch(stats_kernel<T, VEC, GV, true>, grid, pl.threads, smem, kCluster, false, p, st, what);
   int rc = launch(stats_kernel<T, VEC, GV, false>, grid, pl.threads, smem, kCluster, false, p, st, what);
   if (!rc && !p.direct)
     rc = launch(finish_stats_kernel, dim3((unsigned)ceil_div(p.B * p.G, 8)), 256, 0, 0, true, p, st, what);
-  if (!rc) rc = launch(apply_kernel<T, VEC>, dim3(2 * p.chunks, (unsigned)p.B), pl.threads, 0, 0, true, p, st, what);
+  if (!rc) rc = launch(apply_kernel<T, VEC>, batch_grid(2 * p.chunks, p.B), pl.threads, 0, 0, true, p, st, what);
   return rc;
 }
 
@@ -865,7 +879,7 @@ static int backward_v(Params& p, cudaStream_t st) {
   size_t smem = ((size_t)p.C + (size_t)p.rows * p.vlanes * VEC) * sizeof(float2);
   const size_t sums = ((size_t)2 * p.C + p.G) * sizeof(float2);
   if (smem < sums) smem = sums;
-  const dim3 grid(p.chunks, (unsigned)p.B);
+  const dim3 grid = batch_grid(p.chunks, p.B);
   const bool params = p.dw || p.db;
   int rc;
   if (pl.fused || !p.out) {
@@ -880,7 +894,7 @@ static int backward_v(Params& p, cudaStream_t st) {
     rc = launch(finish_grad_kernel, dim3((unsigned)ceil_div(p.B * p.G, 8)), 256, 0, 0, true, p, st, what);
   const unsigned extra = params ? (unsigned)ceil_div(p.C, (int64_t)pl.threads / 32) : 0;
   if (!rc)
-    rc = launch(grad_apply_kernel<T, VEC>, dim3(p.chunks + extra, (unsigned)p.B), pl.threads, 0, 0, true, p, st, what);
+    rc = launch(grad_apply_kernel<T, VEC>, batch_grid(p.chunks + extra, p.B), pl.threads, 0, 0, true, p, st, what);
   return rc;
 }
 
@@ -888,8 +902,8 @@ static int check(const Params& p, int64_t C, int64_t G, int dtype, const char* w
   ZIB_HOST_CHECK(known_dtype(dtype) && known_dtype(p.wdtype), ZIB_ERR_INVALID_ARG, "%s: unknown dtype", what);
   ZIB_HOST_CHECK(p.B >= 0 && p.P >= 0 && C >= 1 && G >= 1 && C % G == 0, ZIB_ERR_INVALID_ARG,
                  "%s: %lld channels in %lld groups", what, (long long)C, (long long)G);
-  ZIB_HOST_CHECK(C <= kMaxChannels && p.B <= 65535, ZIB_ERR_TOO_LARGE,
-                 "%s: at most %d channels and 65535 batch entries", what, kMaxChannels);
+  ZIB_HOST_CHECK(C <= kMaxChannels && p.B < (1ll << 31), ZIB_ERR_TOO_LARGE,
+                 "%s: at most %d channels and 2^31 - 1 batch entries", what, kMaxChannels);
   ZIB_HOST_CHECK(p.act == ZIB_ACT_NONE || p.act == ZIB_ACT_SILU, ZIB_ERR_INVALID_ARG, "%s: unknown activation %d",
                  what, p.act);
   ZIB_HOST_CHECK(p.eps >= 0.0f, ZIB_ERR_INVALID_ARG, "%s: eps must not be negative", what);

@@ -13,7 +13,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
                    bias: torch.Tensor | None = None, eps: float = 1e-6, activation: str = "silu") -> torch.Tensor:
     """act((x - mean) / sqrt(var + eps) * weight + bias) over groups of the last dimension.
 
-    x [B, ..., C] (bf16, fp16, fp32; channels last, any strides of the others); the mean and the
+    x [B, ..., C] (bf16, fp16, fp32; channels last, C <= 8192, any strides of the others); the mean and the
     variance of a batch entry's group run over its C / num_groups channels and every position
     between.  A convolution's [B, C, H, W] tensor in channels-last memory format is passed as
     ``x.permute(0, 2, 3, 1)`` without a copy.  weight, bias: [C] of one type (bf16, fp16, fp32),

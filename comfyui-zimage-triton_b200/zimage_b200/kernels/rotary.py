@@ -64,7 +64,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin
                  positions: torch.Tensor | None = None, layout: str = "interleaved"):
     """(q, k) with the first 2 * cos.shape[-1] features of every head turned; new contiguous tensors.
 
-    q [B, S, H, D], k [B, S, Hk, D] or None, of one type (bf16, fp16, fp32), any strides.
+    q [B, S, H, D], k [B, S, Hk, D] or None, of one type (bf16, fp16, fp32), any strides; B <= 65535,
+    D <= 1024.
     cos, sin: fp32 [L, R/2], or [B or 1, L, R/2]; row ``positions[b, s]`` turns token (b, s)
     (int32 or int64, broadcastable to [B, S]), row s where ``positions`` is None.  ``layout``:
     "interleaved" pairs features (2j, 2j+1), "half" pairs (j, j + R/2).  Features from R on pass

@@ -406,7 +406,7 @@ ZIB_API int64_t zib_group_norm_workspace(int64_t B, int64_t P, int64_t C, int64_
  * stride xsb and pixel stride xsp, channels contiguous; y: contiguous [B,P,C];
  * w, b: [C] of wdtype, each may be NULL; mean, rstd: fp32 [B,G] outputs.
  * y = act((x - mean) * rstd * w + b), statistics per batch entry over the
- * P * C/G values of a group. */
+ * P * C/G values of a group.  C <= 8192. */
 ZIB_API int zib_group_norm(const void* x, int64_t xsb, int64_t xsp, void* y, const void* w, const void* b,
                    int wdtype, float* mean, float* rstd, void* workspace, int64_t workspace_bytes,
                    int64_t B, int64_t P, int64_t C, int64_t G, int dtype, float eps, int act,

@@ -1075,3 +1075,40 @@ def test_fp8_block_linear_module_moved_and_loaded(cuda, K, N):
     for n in (other, m.cpu().cuda()):
         assert all(t.stride(0) % 16 == 0 and t.stride(1) == 1 for t in (n.w_q, n.w_q_t))
         assert torch.equal(n(x), y) and torch.equal(torch.autograd.grad(n(x).sum(), (x,))[0], dx)
+
+
+@pytest.mark.parametrize("B", [65535, 65536, 70001, 131072])
+def test_group_norm_of_many_batch_entries(cuda, B):
+    """A matrix [rows, C]: its rows are the batch entries."""
+    g = _gen(B)
+    C, G = 64, 4
+    x, dy = _randn(g, B, C).to(torch.bfloat16).requires_grad_(), _randn(g, B, C).to(torch.bfloat16)
+    w, b = (1 + 0.2 * _randn(g, C)).requires_grad_(), (0.2 * _randn(g, C)).requires_grad_()
+    y = group_norm_act(x, G, w, b)
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    ref = ref_group_norm(x.detach()[:, None], G, w.detach(), b.detach(), 1e-6, "silu", dy[:, None])
+    check(y.detach()[:, None], *ref[0])
+    check(got[0][:, None], *ref[1])
+    for a, r in zip(got[1:], ref[2:]):
+        check(a, *r)
+
+
+@pytest.mark.parametrize("G", [4, 128])
+def test_group_norm_of_many_batch_entries_in_two_passes(cuda, G):
+    """One image seen by 65537 batch entries (stride 0), too large for the one-launch form."""
+    g = _gen(G)
+    B, P, C = 65537, 1030, 128
+    one, d = _randn(g, 1, P, C).to(torch.bfloat16), _randn(g, 1, P, C).to(torch.bfloat16)
+    w, b = (1 + 0.2 * _randn(g, C)).requires_grad_(), (0.2 * _randn(g, C)).requires_grad_()
+    x = one.expand(B, P, C).detach().requires_grad_()
+    y = group_norm_act(x, G, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), d.expand(B, P, C))
+    y = y.detach()
+    ref = ref_group_norm(one, G, w.detach(), b.detach(), 1e-6, "silu", d)
+    check(y[:1], *ref[0])
+    check(dx[:1], *ref[1])
+    for part in (y, dx):
+        assert all(bool((t == part[:1]).all()) for t in part.split(4096))
+    # B equal terms for each of one entry's, joined in fp64
+    check(dw, ref[2][0] * B, ref[2][1] * B)
+    check(db, ref[3][0] * B, ref[3][1] * B)
