@@ -22,7 +22,10 @@
 //
 // Sums.  A thread subtracts a value of its own group first (the mean of its first pixel's channels),
 // adds the differences and their squares in fp32 over 16 pixels at most and joins them in fp64, so a mean that
-// is large against the spread costs no precision.  All sums have a fixed order (no atomics).
+// is large against the spread costs no precision.  A thread adds the backward sums A and E in fp32 over
+// kGradRun pixels at most (more CTAs where there are more pixels) and joins them in fp64; a CTA's sum and
+// the sum of a cluster's eight are rounded to fp32 on their way to the next fp64 sum.  All sums have a fixed
+// order (no atomics).
 //
 // Arithmetic is on packed pairs (f32x2): at 12 elements per clock and SM, the rate of HBM, single
 // operations left the SMs short of issue slots (79 us instead of 58 for the statistics of
@@ -38,6 +41,9 @@ constexpr int kCluster = 8;
 constexpr int kMaxChannels = 8192;  // one pixel's partial sums fit shared memory
 constexpr int kDirectGroups = 64;   // groups whose partial sums every CTA of the second pass adds itself
 constexpr int kMaxSmem = 232448;
+// Pixels whose gradient terms a thread adds in fp32: terms of one sign err by 2^-15 of their sum at worst.
+// fp64 sums beside them, every 64 pixels, spilled registers: [2, 16384, 512] backward 58 -> 66 us.
+constexpr int kGradRun = 512;
 
 struct Params {
   const void* x;
@@ -745,6 +751,11 @@ static int64_t most_clusters(int64_t B, int64_t P) {
   return c < 1 ? 1 : c;
 }
 
+// the same of the backward pass, whose threads' runs are bounded (a thread row to a CTA at least)
+static int64_t most_grad_clusters(int64_t B, int64_t P) {
+  return most_clusters(B, P) + (P > kCluster * kGradRun ? ceil_div(P, kCluster * kGradRun) : 0);
+}
+
 // One cluster per batch entry is enough up to this many bytes of x: 8 CTAs read 32 KB each in about
 // the time of the second launch that they save.
 constexpr int64_t kFusedBytes = 256 * 1024;
@@ -785,8 +796,9 @@ static int resident_clusters(void (*kernel)(Params), unsigned threads, size_t sm
   return known[dev];
 }
 
-// `resident`: clusters of the first pass that run at once, so that it runs in one wave
-static Plan plan(Params& p, int vec, int size, int resident) {
+// `resident`: clusters of the first pass that run at once, so that it runs in one wave, or where `run`
+// bounds a thread's pixels in whole ones
+static Plan plan(Params& p, int vec, int size, int resident, int run = 0) {
   p.V = p.C / vec;
   p.vlanes = p.V < kThreads ? p.V : kThreads;
   p.rows = kThreads / p.vlanes;
@@ -796,6 +808,13 @@ static Plan plan(Params& p, int vec, int size, int resident) {
   // at least 16 pixels per thread row, so that runs fill
   const int64_t most = ceil_div(p.P, (int64_t)kCluster * p.rows * 16);
   if (clusters > most) clusters = most;
+  const int64_t need = run ? ceil_div(p.P, (int64_t)kCluster * p.rows * run) : 0;
+  if (need > clusters) {
+    clusters = ceil_div(need * p.B, resident) * resident / p.B;
+    if (clusters < need) clusters = need;
+    const int64_t room = most_grad_clusters(p.B, p.P);
+    if (clusters > room) clusters = room;
+  }
   p.clusters = (int)clusters;
   p.chunks = kCluster * p.clusters;
   p.chunk = ceil_div(p.P, p.chunks);
@@ -875,7 +894,7 @@ static int backward_v(Params& p, cudaStream_t st) {
   const char* what = "zib_group_norm_backward";
   static int known[64];
   const Plan pl = plan(p, VEC, 2 * sizeof(T),  // x and dy
-                       resident_clusters(grad_stats_kernel<T, VEC, false>, kThreads, 24 * 1024, known));
+                       resident_clusters(grad_stats_kernel<T, VEC, false>, kThreads, 24 * 1024, known), kGradRun);
   size_t smem = ((size_t)p.C + (size_t)p.rows * p.vlanes * VEC) * sizeof(float2);
   const size_t sums = ((size_t)2 * p.C + p.G) * sizeof(float2);
   if (smem < sums) smem = sums;
@@ -944,7 +963,7 @@ using namespace zib;
 
 extern "C" int64_t zib_group_norm_workspace(int64_t B, int64_t P, int64_t C, int64_t G, int backward) {
   if (B < 0 || P < 0 || C < 1 || G < 1) return 0;
-  const int64_t n = B * gn::most_clusters(B, P);
+  const int64_t n = B * (backward ? gn::most_grad_clusters(B, P) : gn::most_clusters(B, P));
   const int64_t groups = n * G * (int64_t)sizeof(double2);
   return backward ? groups + (n * C + B * G) * (int64_t)sizeof(float2) : groups;
 }
@@ -993,7 +1012,7 @@ extern "C" int zib_group_norm_backward(const void* x, int64_t xsb, int64_t xsp, 
                  (long long)zib_group_norm_workspace(B, P, C, G, 1));
   if (!dx && !dw && !db) return ZIB_OK;
   p.C = (int)C; p.G = (int)G; p.cpg = (int)(C / G);
-  const int64_t n = B * gn::most_clusters(B, P);
+  const int64_t n = B * gn::most_grad_clusters(B, P);
   p.gpart = (double2*)workspace;
   p.cpart = (float2*)(p.gpart + n * G);
   p.coef = p.cpart + n * C;

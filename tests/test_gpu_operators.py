@@ -1112,3 +1112,25 @@ def test_group_norm_of_many_batch_entries_in_two_passes(cuda, G):
     # B equal terms for each of one entry's, joined in fp64
     check(dw, ref[2][0] * B, ref[2][1] * B)
     check(db, ref[3][0] * B, ref[3][1] * B)
+
+
+def test_group_norm_parameter_gradients_of_long_sums(cuda):
+    """Many pixels to a cluster, all terms of one sign: each addition in 32 bits errs the same way."""
+    g = _gen(101)
+    B, P, C, G = 30, 1 << 17, 1024, 32
+    one = _randn(g, 1, P, C)
+    d = (1 / 3 + torch.arange(C, device="cuda") / 7).expand(1, P, C)
+    w, b = torch.ones(C, device="cuda", requires_grad=True), torch.zeros(C, device="cuda", requires_grad=True)
+    y = group_norm_act(one.expand(B, P, C), G, w, b, activation="none")
+    dw, db = torch.autograd.grad(y, (w, b), d.expand(B, P, C))
+    # 511 additions of a thread's run of 512 at most, one rounding of the CTA's sum, seven additions of the cluster's
+    n = 511 + 1 + 7
+    check(db, B * P * d[0, 0].double(), n * U32 * B * P * d[0, 0].double())
+    xd = one.double().view(P, G, C // G)
+    mean = xd.mean((0, 2), keepdim=True)
+    r = 1 / torch.sqrt(((xd - mean) ** 2).mean((0, 2), keepdim=True) + 1e-6)
+    h = ((xd - mean) * r).view(P, C)
+    # h as in ref_group_norm (the subtraction, the statistics' own error), one more step for the multiply-add
+    dh = U32 * (2 * (one[0].double().abs() + mean.abs().max()) * r.max() + 31 * r.max() + 23 * h.abs())
+    gh = d[0].double() * h
+    check(dw, B * gh.sum(0), B * (d[0].double() * dh + (n + 1) * U32 * gh.abs()).sum(0))
