@@ -28,7 +28,10 @@ def rotary_table(positions: torch.Tensor | int, dim: int, theta: float = 10000.0
     theta f^(dim/(dim-2))) or {"type": "yarn", "factor": f, "original_length": n} with optional
     "beta_fast" (32), "beta_slow" (1) and "attention_factor" (0.1 ln f + 1): frequencies that turn
     less than beta_slow times over the original length are divided by f, those that turn more than
-    beta_fast times are kept, a linear ramp between (Peng et al., arXiv 2309.00071).
+    beta_fast times are kept, a linear ramp between (Peng et al., arXiv 2309.00071).  The ramp runs over
+    the number of turns, as in the paper's text; a ramp over the frequency's index gives other tables for
+    the same parameters.  "original_length" may be given with any type; entries that a type does not
+    have are refused.
     """
     if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or dim % 2:
         raise ValueError(f"dim must be a positive even number, got {dim!r}")
@@ -42,6 +45,10 @@ def rotary_table(positions: torch.Tensor | int, dim: int, theta: float = 10000.0
         if kind != "none" and not 1.0 <= factor < 1e9:
             raise ValueError(f"scaling factor must be at least 1, got {factor}")
         original = float(sc.pop("original_length", 0.0))
+        if kind == "none" and factor != 1.0:
+            raise ValueError(f"scaling type 'none' has no factor, got {factor}")
+        if kind != "yarn" and sc:
+            raise ValueError(f"scaling type {kind!r} has no entries {sorted(sc)}")
         fast, slow = float(sc.pop("beta_fast", 32.0)), float(sc.pop("beta_slow", 1.0))
         attn = sc.pop("attention_factor", None)
         if sc:

@@ -241,3 +241,22 @@ def test_fp8_block_linear_keeps_its_rows_aligned(K, N):
         for t, k in ((m.w_q, "w_q"), (m.w_q_t, "w_q_t")):
             assert torch.equal(t.contiguous().view(torch.uint8), dense[k].view(torch.uint8))
     check(copy.deepcopy(made[0]).to("meta"))
+
+
+@pytest.mark.parametrize("scaling", [
+    {"type": "linear", "factor": 2.0, "attention_factor": 1.2}, {"type": "ntk", "factor": 2.0, "beta_fast": 16.0},
+    {"type": "ntk", "factor": 2.0, "beta_slow": 2.0}, {"type": "none", "factor": 2.0},
+    {"type": "none", "attention_factor": 1.0}])
+def test_rotary_table_refuses_entries_of_another_type(scaling):
+    """They were taken and ignored."""
+    with pytest.raises(ValueError, match="has no"):
+        rotary_table(torch.arange(4), 8, scaling=scaling)
+
+
+@pytest.mark.parametrize("scaling", [
+    {"type": "linear", "factor": 2.0, "original_length": 100}, {"type": "ntk", "factor": 2.0, "original_length": 100},
+    {"type": "none"}, {"type": "none", "factor": 1.0, "original_length": 100}, {},
+    {"type": "yarn", "factor": 2.0, "original_length": 100, "beta_fast": 16.0, "beta_slow": 2.0, "attention_factor": 1.0}])
+def test_rotary_table_takes_its_type_s_entries(scaling):
+    with pytest.raises(ValueError, match="CUDA"):  # as far as a tensor on the host goes
+        rotary_table(torch.arange(4), 8, scaling=scaling)
