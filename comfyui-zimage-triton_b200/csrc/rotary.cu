@@ -210,13 +210,24 @@ struct TableParams {
   float* sin;
 };
 
-// cos and sin of an angle in fixed point, 2^-32 turns: its nearest multiple of a quarter turn decides
-// which of them is which and their signs, exactly, in integers; the rest, within an eighth of a turn
-// and rounded once to fp32, goes through the Taylor series of sine (to x^9) and cosine (to x^10), whose
-// next terms are below 2e-9 and 2e-10 there.
-__device__ __forceinline__ void sincos_turns(uint32_t a, float& s, float& c) {
-  const uint32_t quarter = (a + 0x20000000u) >> 30;
-  const float x = (float)(int32_t)(a - (quarter << 30)) * 1.4629180792671596e-09f;  // 2 pi / 2^32
+// An angle in fixed point, 2^-64 turns: its nearest multiple of a quarter turn, and the rest, within an
+// eighth of a turn, in units of 2^-32 turns as fp32.  The lower word keeps the rest's relative accuracy
+// (two roundings) down to 2^-56 turns: the sine of a slow frequency at an early position is as small as
+// its angle.
+__device__ __forceinline__ uint32_t quarter_of(uint64_t a) { return ((uint32_t)(a >> 32) + 0x20000000u) >> 30; }
+__device__ __forceinline__ float high_rest(uint64_t a, uint32_t quarter) {
+  return (float)(int32_t)((uint32_t)(a >> 32) - (quarter << 30));
+}
+__device__ __forceinline__ float low_rest(uint64_t a) { return (float)(uint32_t)a; }
+constexpr float kLow = 2.3283064365386963e-10f;     // 2^-32
+constexpr float kRadians = 1.4629180792671596e-09f;  // 2 pi / 2^32
+
+// cos and sin of such an angle: the quarter decides which of them is which and their signs, exactly, in
+// integers; the rest goes through the Taylor series of sine (to x^9) and cosine (to x^10), whose next
+// terms are below 2e-9 and 2e-10 there.
+__device__ __forceinline__ void sincos_turns(uint64_t a, float& s, float& c) {
+  const uint32_t quarter = quarter_of(a);
+  const float x = fmaf(low_rest(a), kLow, high_rest(a, quarter)) * kRadians;
   const float x2 = x * x;
   float ps = 2.7557319e-6f;  // 1 / 9!
   ps = fmaf(ps, x2, -1.9841270e-4f);
@@ -235,11 +246,11 @@ __device__ __forceinline__ void sincos_turns(uint32_t a, float& s, float& c) {
 }
 
 // the same of two angles, on packed pairs
-__device__ __forceinline__ void sincos_turns2(uint32_t a0, uint32_t a1, float m, float (&s)[2], float (&c)[2]) {
-  const uint32_t q[2] = {(a0 + 0x20000000u) >> 30, (a1 + 0x20000000u) >> 30};
+__device__ __forceinline__ void sincos_turns2(uint64_t a0, uint64_t a1, float m, float (&s)[2], float (&c)[2]) {
+  const uint32_t q[2] = {quarter_of(a0), quarter_of(a1)};
   auto all = [](float v) { return px::mk(v, v); };
-  const px::f2 x = px::mul(px::mk((float)(int32_t)(a0 - (q[0] << 30)), (float)(int32_t)(a1 - (q[1] << 30))),
-                           all(1.4629180792671596e-09f));
+  const px::f2 x = px::mul(px::fma(px::mk(low_rest(a0), low_rest(a1)), all(kLow),
+                                   px::mk(high_rest(a0, q[0]), high_rest(a1, q[1]))), all(kRadians));
   const px::f2 x2 = px::mul(x, x);
   px::f2 ps = all(2.7557319e-6f);
   ps = px::fma(ps, x2, all(-1.9841270e-4f));
@@ -298,8 +309,7 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const TableParams p) 
       pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[t * p.ps]
                     : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[t * p.ps];
     Pack<float, J> c, s;
-    // the nearest 2^-32 turns of the 64-bit product
-    auto angle = [&](int i) { return (uint32_t)(((uint64_t)pos * turns[i] + 0x80000000ull) >> 32); };
+    auto angle = [&](int i) { return (uint64_t)pos * turns[i]; };
     if constexpr (J == 2) {
       sincos_turns2(angle(0), angle(1), p.mscale, s.v, c.v);
     } else {

@@ -31,7 +31,8 @@ def rotary_table(positions: torch.Tensor | int, dim: int, theta: float = 10000.0
     beta_fast times are kept, a linear ramp between (Peng et al., arXiv 2309.00071).  The ramp runs over
     the number of turns, as in the paper's text; a ramp over the frequency's index gives other tables for
     the same parameters.  "original_length" may be given with any type; entries that a type does not
-    have are refused.
+    have are refused.  Values are within a few steps of fp32 (2^-24 of each) of the exact ones, beside an
+    error of the angle of 2^-55 turns for each unit of the position.
     """
     if isinstance(dim, bool) or not isinstance(dim, int) or dim < 2 or dim % 2:
         raise ValueError(f"dim must be a positive even number, got {dim!r}")

@@ -391,8 +391,9 @@ ZIB_API int zib_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, 
  *   yarn    frequencies with fewer than beta_slow turns over `original`
  *           positions divided by factor, those with more than beta_fast kept, a
  *           linear ramp between; cos and sin times attention_factor.
- * Angles are formed in 64-bit fixed point, off by 2^-32 turns and 2^-55 turns for
- * each unit of the position (its fp64 frequency) at most. */
+ * Angles are formed in 64-bit fixed point, off by 2^-55 turns for each unit of the
+ * position at most (its fp64 frequency), and keep fp32's relative accuracy where they are
+ * small. */
 ZIB_API int zib_rotary_table(const void* positions, int pos64, int64_t ps, int64_t start, int64_t T,
                      int64_t dim, double theta, int scaling, double factor, double original,
                      double beta_fast, double beta_slow, double attention_factor, float* cos,

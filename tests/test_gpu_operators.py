@@ -1134,3 +1134,24 @@ def test_group_norm_parameter_gradients_of_long_sums(cuda):
     dh = U32 * (2 * (one[0].double().abs() + mean.abs().max()) * r.max() + 31 * r.max() + 23 * h.abs())
     gh = d[0].double() * h
     check(dw, B * gh.sum(0), B * (d[0].double() * dh + (n + 1) * U32 * gh.abs()).sum(0))
+
+
+@pytest.mark.parametrize("dim,theta", [(128, 10000.0), (128, 500000.0), (62, 256.0), (64, 1e6)])
+def test_rotary_table_keeps_small_angles(cuda, dim, theta):
+    """Relative to each value: slow frequencies at early positions have small sines."""
+    pos = torch.cat([torch.arange(-40, 300), torch.tensor([1000, 4095, 131071, (1 << 31) - 1])]).cuda()
+    f = torch.tensor([theta ** (-2.0 * j / dim) for j in range(dim // 2)], dtype=torch.float64, device="cuda")
+    p = pos.double()[:, None]
+    ang = p * f
+    cos, sin = rotary_table(pos, dim, theta=theta)
+    for got, ref in ((cos, ang.cos()), (sin, ang.sin())):
+        # the rest of the angle: two conversions joined in one multiply-add, the constant and the product, four
+        # roundings; the series' last step, its terms before (a tenth of it, four roundings) and what it leaves out
+        # (2e-9 of an eighth of a turn, a thirtieth of a step), the factor: seven steps of the value.  The angle's
+        # own error: 2^-55 turns a position for its fp64 frequency, 2^-64 for its fixed point, and the
+        # reference's, three steps of 2^-53
+        check(got, ref, 7 * U32 * ref.abs() + p.abs() * 2 * math.pi * (2.0 ** -55 + 2.0 ** -64) + ang.abs() * 2.0 ** -51)
+    s = sin[pos == 1][0]
+    small = f < 1e-3
+    if bool(small.any()):
+        assert bool(((s.double() - f.sin()).abs() <= 8 * U32 * f)[small].all())
