@@ -795,14 +795,14 @@ static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, 
   int smem;
   if constexpr (MX) kernel = gemm_mx_kernel<T>, smem = Mx::SMEM;
   else kernel = gemm_pair_kernel<T, BN>, smem = Cfg<BN>::SMEM;
-  static bool set[64] = {false};
+  static std::atomic<bool> set[64];
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !set[dev]) {
+  if (dev >= 0 && dev < 64 && !set[dev].load(std::memory_order_relaxed)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     ZIB_HOST_CHECK(e == cudaSuccess, ZIB_ERR_LAUNCH, "%s: cudaFuncSetAttribute failed: %s", what,
                    cudaGetErrorString(e));
-    set[dev] = true;
+    set[dev].store(true, std::memory_order_relaxed);
   }
   p.num_mb = (int)ceil_div(p.M, 256);
   p.num_nb = (int)ceil_div(p.N, BN);

@@ -759,10 +759,12 @@ struct Plan {
 };
 
 // clusters of `kernel` that run at once on the current device (asked for once per device)
-static int resident_clusters(void (*kernel)(Params), unsigned threads, size_t smem, int (&known)[64]) {
+static int resident_clusters(void (*kernel)(Params), unsigned threads, size_t smem,
+                             std::atomic<int> (&known)[64]) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count() * 2 / kCluster;
-  if (known[dev] == 0) {
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kCluster * 64);
     cfg.blockDim = dim3(threads);
@@ -773,14 +775,13 @@ static int resident_clusters(void (*kernel)(Params), unsigned threads, size_t sm
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = sm_count() * 2 / kCluster;
     }
-    known[dev] = n;
+    known[dev].store(n, std::memory_order_relaxed);
   }
-  return known[dev];
+  return n;
 }
 
 // `resident`: clusters of the first pass that run at once, so that it runs in one wave, or where `run`
@@ -864,7 +865,7 @@ static int launch_batch(void (*kernel)(Params), unsigned x, unsigned threads, si
 template <typename T, int VEC, int GV>
 static int forward_g(Params& p, cudaStream_t st) {
   const char* what = "zib_group_norm";
-  static int known[64];
+  static std::atomic<int> known[64];
   const Plan pl = plan(p, VEC, sizeof(T), resident_clusters(stats_kernel<T, VEC, GV, false>, kThreads, 24 * 1024, known));
   const size_t sums = (size_t)p.rows * p.V * (VEC / GV);
   size_t smem = ((p.cpg / GV * p.rows == 1 ? 0 : (size_t)p.G) + sums) * sizeof(double2);
@@ -892,7 +893,7 @@ static int forward_v(Params& p, cudaStream_t st) {
 template <typename T, int VEC>
 static int backward_v(Params& p, cudaStream_t st) {
   const char* what = "zib_group_norm_backward";
-  static int known[64];
+  static std::atomic<int> known[64];
   const Plan pl = plan(p, VEC, 2 * sizeof(T),  // x and dy
                        resident_clusters(grad_stats_kernel<T, VEC, false>, kThreads, 24 * 1024, known), kGradRun);
   size_t smem = ((size_t)p.C + (size_t)p.rows * p.vlanes * VEC) * sizeof(float2);

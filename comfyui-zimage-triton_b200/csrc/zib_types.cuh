@@ -3,6 +3,7 @@
 
 #include "zib_common.cuh"
 
+#include <atomic>
 #include <cuda_fp16.h>
 
 namespace zib {
@@ -48,15 +49,16 @@ inline int dtype_bytes(int d) { return d == ZIB_F32 ? 4 : 2; }
 
 // multiprocessors of the current device (looked up once per device)
 inline int sm_count() {
-  static int cached[64] = {0};
+  static std::atomic<int> cached[64];  // 0: not yet; threads that look it up at once find the same
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (!cached[dev]) {
-    int n = 0;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (!n) {
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    cached[dev] = n > 0 ? n : 148;
+    if (n <= 0) n = 148;
+    cached[dev].store(n, std::memory_order_relaxed);
   }
-  return cached[dev];
+  return n;
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
