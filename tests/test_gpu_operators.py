@@ -1155,3 +1155,146 @@ def test_rotary_table_keeps_small_angles(cuda, dim, theta):
     small = f < 1e-3
     if bool(small.any()):
         assert bool(((s.double() - f.sin()).abs() <= 8 * U32 * f)[small].all())
+
+
+# --- several tiles to a pair of CTAs ------------------------------------------------------------------
+
+# 74 pairs.  By the launch rule: 360 tiles of 256 x 192 where the tensor cores apply the scales and, for other
+# scales, 270 of 256 x 256; 143 of 256 x 128
+SEVERAL_TILES = [(4608, 2048, 3840), (4500, 2000, 3701)]
+SEVERAL_SLIM_TILES = [(3328, 1024, 1408), (3300, 1000, 1399)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", SEVERAL_TILES)
+def test_linear_of_several_tiles_to_a_pair(cuda, dtype, M, K, N):
+    """Accumulators, stages, scales and the bias' copy used again by a pair's next tiles."""
+    g = _gen(M + K)
+    x = _varied(g, M, K, 3).to(dtype)
+    wq, ws = fp8_block_quantize_weight(_varied(g, N, K, 3) / 64)
+    bias = (_randn(g, N) * 30).to(dtype)
+    qx, sx = ref_rows(x)
+    ref, mag = product_terms(qx, sx, wq, ws)
+    check(fp8_block_linear(x, wq, ws, bias), ref + bias.double(), product_extra(mag, K, bias))
+    check(fp8_block_linear(x, wq, ws), ref, product_extra(mag, K))
+    other = ws.clone()
+    other[-1, -1] = 0.7  # no power of two: the second launch
+    ref, mag = product_terms(qx, sx, wq, other)
+    check(fp8_block_linear(x, wq, other, bias), ref + bias.double(), product_extra(mag, K, bias))
+    assert _lib.device_error_read_clear() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", SEVERAL_TILES + SEVERAL_SLIM_TILES)
+def test_matmul_of_several_tiles_to_a_pair(cuda, dtype, M, K, N):
+    g = _gen(M + K + 1)
+    xq, sx = fp8_block_quantize(_varied(g, M, K, 3))
+    wq, sw = fp8_block_quantize_weight(_varied(g, N, K, 3) / 64)
+    bias = (_randn(g, N) * 30).to(dtype)
+    sx = sx * (0.5 + torch.rand(sx.shape, generator=g, device="cuda"))
+    ref, mag = product_terms(xq, sx, wq, sw)
+    # the product of the two scales is rounded once more where they are no powers of two
+    y = fp8_block_matmul(xq, sx, wq, sw, bias, out_dtype=dtype)
+    check(y, ref + bias.double(), product_extra(mag, K, bias))
+    assert _lib.device_error_read_clear() == 0
+
+
+def test_linear_gradients_of_several_tiles_to_a_pair(cuda):
+    M, K, N = 4608, 3840, 2048
+    g = _gen(103)
+    x = _randn(g, M, K).to(torch.bfloat16).requires_grad_()
+    b = _randn(g, N).to(torch.bfloat16).requires_grad_()
+    wq, ws = fp8_block_quantize_weight(_varied(g, N, K, 3) / 64)
+    dy = _varied(g, M, N, 3).to(torch.bfloat16)
+    want = product_terms(*ref_rows(dy), wq.t(), ws.t())
+    for wt in (None, fp8_block_transpose(wq)):
+        dx, db = torch.autograd.grad(fp8_block_linear(x, wq, ws, b, w_q_t=wt), (x, b), dy)
+        check(dx, want[0], product_extra(want[1], N))
+        check(db, dy.double().sum(0), (M + 2) * U32 * dy.double().abs().sum(0))
+
+
+# --- what the sums hold -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("M,K,N,quantised", [(600, 4096, 3840, False), (600, 4096, 3840, True), (600, 4096, 128, True),
+                                             (8, 4096, 3840, False), (2, 4096, 256, False), (200, 4096, 128, False)])
+@pytest.mark.parametrize("at", [1, 31, 32, 64, 127, 128])
+def test_sums_hold_24_bits(cuda, M, K, N, quantised, at):
+    """2^16 and a term of 2^-7 in the same step, in another one of its block, or 31 of them in other blocks: every
+    partial sum is a multiple of 2^-7 below 2^17, so exact in 24 bits, in any order."""
+    x = torch.zeros(M, K, device="cuda")
+    x[:, 0] = 256.0
+    x[:, 2] = 448.0  # the block's scale is 1; its weights are 0
+    x[:, at::128] = 2.0 ** -6 if at < 128 else 0.0
+    if at == 128:
+        x[:, 128::128] = 2.0 ** -6
+        x[:, 130::128] = 448.0
+    w = torch.zeros(N, K, device="cuda")
+    w[:, 0] = 256.0
+    w[:, at::128] = 2.0 ** -1
+    if at < 128:
+        w[:, 128:] = 0.0
+    wq, ws = w.to(torch.float8_e4m3fn), torch.ones(-(-N // 128), K // 128, device="cuda")
+    q, s = fp8_block_quantize(x)
+    assert bool((s[:, 0] == 1).all()) and same(q, x / s.repeat_interleave(128, 1))
+    y = fp8_block_matmul(q, s, wq, ws, out_dtype=torch.float32) if quantised else fp8_block_linear(x, wq, ws)
+    assert bool((y == 65536.0 + (1 if at < 128 else 31) * 2.0 ** -7).all()), float(y.flatten()[0] - 65536.0)
+
+
+@pytest.mark.parametrize("ex,ew", [(50, 60), (60, 50), (-50, -60), (100, 10)])
+def test_linear_of_many_blocks_far_exponents_within_range(cuda, ex, ew):
+    """The sum of magnitudes times 2^(ex + ew) stays below 2^128, so no partial sum may be infinite."""
+    M, K, N = 600, 4096, 3840
+    g = _gen(15)
+    x, w = _randn(g, M, K), _randn(g, N, K)
+    wq, ws = fp8_block_quantize_weight(w)
+    ref, mag = product_terms(*ref_rows(x), wq, ws)
+    f = 2.0 ** (ex + ew)
+    assert float(mag.max()) * f < 2.0 ** 127
+    y = fp8_block_linear(x * 2.0 ** ex, wq, ws * 2.0 ** ew)
+    assert bool(torch.isfinite(y).all())
+    check(y, ref * f, product_extra(mag, K) * f)
+
+
+# --- group norm: many groups in two passes, and each parameter alone ------------------------------------
+
+MANY_GROUPS = [(2, 900, 768, 96), (1, 700, 1024, 1024), (3, 1100, 325, 65), (1, 2000, 1000, 125)]
+
+
+@pytest.mark.parametrize("act", ["silu", "none"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,P,C,G", MANY_GROUPS)
+def test_group_norm_of_many_groups(cuda, act, dtype, B, P, C, G):
+    g = _gen(P + C)
+    x = (_randn(g, B, P, C) * (0.5 + torch.rand(C, generator=g, device="cuda")) + _randn(g, C)).to(dtype)
+    x.requires_grad_()
+    w, b = (1 + 0.2 * _randn(g, C)).requires_grad_(), (0.2 * _randn(g, C)).requires_grad_()
+    dy = _randn(g, B, P, C).to(dtype)
+    y = group_norm_act(x, G, w, b, eps=1e-5, activation=act)
+    ref = ref_group_norm(x.detach(), G, w.detach(), b.detach(), 1e-5, act, dy)
+    for a, (r, e) in zip((y.detach(), *torch.autograd.grad(y, (x, w, b), dy)), ref):
+        check(a, r, e)
+
+
+@pytest.mark.parametrize("pdtype", TYPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,P,C,G", [(2, 64, 320, 32), (2, 900, 768, 96), (1, 4097, 64, 4)])
+def test_group_norm_gradients_of_each_parameter(cuda, pdtype, dtype, B, P, C, G):
+    """Weights and biases of each type, together, one of them given, one of them wanted."""
+    g = _gen(P + C + 7)
+    x = (_randn(g, B, P, C) + _randn(g, C)).to(dtype)
+    w, b = (1 + 0.2 * _randn(g, C)).to(pdtype), (0.2 * _randn(g, C)).to(pdtype)
+    dy = _randn(g, B, P, C).to(dtype)
+    for has_w, has_b in ((True, True), (True, False), (False, True)):
+        ref = ref_group_norm(x, G, w if has_w else None, b if has_b else None, 1e-5, "silu", dy)
+        for want_x, want_w, want_b in ((True, has_w, has_b), (False, has_w, False), (False, False, has_b)):
+            if not (want_x or want_w or want_b):
+                continue
+            xx = x.detach().requires_grad_(want_x)
+            ww = w.detach().requires_grad_(want_w) if has_w else None
+            bb = b.detach().requires_grad_(want_b) if has_b else None
+            y = group_norm_act(xx, G, ww, bb, eps=1e-5)
+            leaves = [(t, r) for t, wanted, r in ((xx, want_x, ref[1]), (ww, want_w, ref[2]), (bb, want_b, ref[3])) if wanted]
+            for a, (t, r) in zip(torch.autograd.grad(y, [t for t, _ in leaves], dy), leaves):
+                assert a.dtype == t.dtype
+                check(a, *r)
