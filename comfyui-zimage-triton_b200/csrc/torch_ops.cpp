@@ -55,7 +55,14 @@ int dtype_of(const Tensor& t, const char* name) {
   return d;
 }
 
+// A view whose elements read as their negatives (autograd forms some behind complex products) holds the
+// others in memory: refused as an operand, resolved as an upstream gradient.
+void materialised(const Tensor& t) {
+  TORCH_CHECK_VALUE(!t.is_neg(), "an operand is a view that is not yet negated in memory: pass it through resolve_neg()");
+}
+
 void require_device(const Tensor& t) {
+  materialised(t);
   TORCH_CHECK_VALUE(t.is_cuda(), "zimage_b200 ops run only on CUDA tensors (sm_100a); got a tensor on ", t.device(),
                     ". There is no CPU path.");
   static std::atomic<bool> checked[64];
@@ -65,6 +72,7 @@ void require_device(const Tensor& t) {
   if (dev < 64) checked[dev].store(true, std::memory_order_relaxed);
 }
 void same_device(const Tensor& t, const Tensor& o) {
+  materialised(o);
   TORCH_CHECK_VALUE(o.device() == t.device(), "an operand is on ", o.device(), ", expected ", t.device());
 }
 void same_device(const Tensor& t, const OptTensor& o) {
@@ -276,7 +284,8 @@ struct Linear : torch::autograd::Function<Linear> {
                 "fp8_block_linear is differentiable once: its gradient has no gradient of its own");
     no_tangent("the gradient of fp8_block_linear", grads[0]);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &dy = grads[0], &w = saved[0], &s = saved[1];
+    const Tensor dy = grads[0].resolve_neg();
+    const Tensor &w = saved[0], &s = saved[1];
     const int64_t N = w.size(0);
     Tensor dx, db;
     if (ctx->saved_data["bias"].toBool()) db = at::empty({N}, dy.options());
@@ -381,6 +390,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
     if (conf & 2) dk = grads[at++];
     if (!(conf & 4)) dq = Tensor();
     if (!(conf & 8)) dk = Tensor();
+    if (dq.defined()) dq = dq.resolve_neg();
+    if (dk.defined()) dk = dk.resolve_neg();
     no_tangent("the gradient of rotary_embed", dq, dk);
     Tensor gq, gk;
     if (dq.defined() || dk.defined()) {
@@ -540,7 +551,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     if (conf & 4) db = empty ? at::zeros({C}, b.options()) : at::empty({C}, b.options());
     if (!empty) {
       int64_t xsb, xsp, dsb, dsp;
-      const Tensor xs = positions_of(x, P, xsb, xsp), ds = positions_of(grads[0], P, dsb, dsp);
+      const Tensor xs = positions_of(x, P, xsb, xsp), ds = positions_of(grads[0].resolve_neg(), P, dsb, dsp);
       On on(x);
       const int64_t n = zib_group_norm_workspace(B, P, C, G, 1);
       const Tensor ws = bytes(n, x);

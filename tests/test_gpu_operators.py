@@ -1298,3 +1298,26 @@ def test_group_norm_gradients_of_each_parameter(cuda, pdtype, dtype, B, P, C, G)
             for a, (t, r) in zip(torch.autograd.grad(y, [t for t, _ in leaves], dy), leaves):
                 assert a.dtype == t.dtype
                 check(a, *r)
+
+
+def test_views_that_read_as_negatives_are_refused(cuda):
+    """Such as the imaginary part of a conjugate: memory holds the other sign."""
+    g = _gen(105)
+    x, wq, ws = _randn(g, 4, 64), *fp8_block_quantize_weight(_randn(g, 8, 64))
+    z = torch.complex(_randn(g, 1, 1), _randn(g, 1, 1)).conj()
+    neg = torch._neg_view
+    c = _randn(g, 4, 8)
+    q = _randn(g, 1, 4, 2, 16)
+    for call in (lambda: fp8_block_linear(x, wq, z.imag), lambda: fp8_block_linear(neg(x), wq, ws),
+                 lambda: fp8_block_quantize(neg(x)), lambda: fp8_block_quantize_weight(neg(x)),
+                 lambda: rotary_embed(neg(q), None, c, c), lambda: rotary_embed(q, neg(q), c, c),
+                 lambda: rotary_embed(q, None, c, neg(c)), lambda: group_norm_act(neg(x), 4),
+                 lambda: group_norm_act(x, 4, neg(torch.ones(64, device="cuda")))):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    # upstream gradients are resolved
+    xs = x.detach().requires_grad_()
+    for y in (fp8_block_linear(xs, wq, ws), group_norm_act(xs, 4), rotary_embed(xs.view(1, 4, 4, 16), None, c, c)[0]):
+        d = _randn(g, *y.shape)
+        a, b = (torch.autograd.grad(y, (xs,), t, retain_graph=True)[0] for t in (neg(d), -d))
+        assert torch.equal(a, b)
