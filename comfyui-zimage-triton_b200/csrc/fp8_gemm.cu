@@ -843,10 +843,16 @@ static int gemm(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t
   const int64_t pairs = sm_count() / 2, mb = ceil_div(p.M, 256), kb = ceil_div(K, kBlock);
   const int64_t wide = ceil_div(mb * ceil_div(p.N, 256), pairs) * 2, slim = ceil_div(mb * ceil_div(p.N, 128), pairs);
   if (exponents) {
-    // the tensor cores apply the scales where that and the second launch, which then ends at once, are
-    // sooner: 0.34 us a wave and K-block and 3 us for the launch, against 0.50 or 0.29 (wide, slim)
+    // The tensor cores apply the scales where that and the second launch, which then ends at once, are sooner.
+    // A call there takes 5 us more than here, and each wave 0.27 us a K-block and 0.6 us; here each wave 0.54 us a
+    // K-block and 0.6 us (wide) or 0.34 us a K-block (slim).  Fitted to 400 calls of 256 to 9216 rows, both sides
+    // timed in turns: by this rule a call takes 0.2% more than on its faster side on average.  With bias, the
+    // tensor cores' scales / sums in registers: 4608 x 2560 -> 3840 56 / 69 us, 4608 x 3840 -> 2560 60 / 76, 768 x
+    // 2560 -> 3840 26 / 26, 512 x 3840 -> 7680 38 / 31, 2304 x 512 -> 11520 47 / 41, and the wrong way 256 x 3840 ->
+    // 11520 34 / 30 (few rows: bound by the weight's way from memory).
     const int64_t mx = ceil_div(mb * ceil_div(p.N, Mx::BN), pairs);
-    if (300 + 34 * mx * kb < (slim < wide ? 29 * slim : 25 * wide) * kb) {
+    const int64_t sums = slim < wide ? 34 * kb * slim : (27 * kb + 30) * wide;
+    if (500 + (27 * kb + 60) * mx < sums) {
       const int rc = launch_pair<T, Mx::BN, true>(p, q, ldq, w, ldw, K, dependent, st, what);
       if (rc) return rc;
       p.where = 1;
