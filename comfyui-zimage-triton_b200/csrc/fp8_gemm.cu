@@ -4,7 +4,14 @@
 //   y[m, n] = sum_b sx[m, b] sw[n / 128, b] sum_{k in block b} q[m, k] w[n, k]  (+ bias[n])
 //
 // The tensor cores sum one block of 128 products per accumulator; the scales differ from block to
-// block, so the sum over blocks is formed outside of them, in fp32 registers.
+// block, so the sum over blocks is formed outside of them, in fp32 registers, from s = sx sw in fp32 (scales whose
+// product leaves fp32's range are not for this kernel).
+//
+// The accumulators hold fp32's 24 bits, here, with the tensor cores' scales and in mma.sync alike (measured: 2^-23
+// beside 1 survives in the same step of 32 products, in another one of its block and in other blocks).  A step
+// counts terms down to 2^-25 of its largest and cuts its sum to 24 bits instead of rounding it, so it errs by at
+// most 33 2^-25 + 2^-23 of that, less than 32 additions in fp32 may.  One accumulator for all of K is therefore
+// fp32 arithmetic too; sums of one sign come out low rather than to either side.
 //
 // Design (persistent, warp-specialised, clusters of two CTAs, tiles of 256 rows x BN columns):
 //   warp 0     TMA producer: 128-byte swizzled K-major boxes, one K-block of 128 per stage (each CTA
@@ -836,9 +843,8 @@ static int launch_pair(GemmParams p, const void* q, int64_t ldq, const void* w, 
 }
 
 template <typename T>
-static int gemm(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K, bool dependent,
-                cudaStream_t st, const char* what) {
-  const bool exponents = dependent;  // the scales of q come from the quantiser: powers of two
+static int gemm(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t ldw, int64_t K, bool exponents,
+                bool dependent, cudaStream_t st, const char* what) {
   // whole waves of 256 x 256 tiles, or twice as many 256 x 128 ones where those end sooner
   const int64_t pairs = sm_count() / 2, mb = ceil_div(p.M, 256), kb = ceil_div(K, kBlock);
   const int64_t wide = ceil_div(mb * ceil_div(p.N, 256), pairs) * 2, slim = ceil_div(mb * ceil_div(p.N, 128), pairs);
@@ -870,15 +876,16 @@ using namespace zib;
 
 int zib::fp8_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k, const void* w, int64_t ldw,
                   const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, int dtype,
-                  int64_t M, int64_t N, int64_t K, bool dependent, cudaStream_t st, const char* what) {
+                  int64_t M, int64_t N, int64_t K, bool exponents, bool dependent, cudaStream_t st,
+                  const char* what) {
   fp8::GemmParams p{};
   p.M = (int)M; p.N = (int)N;
   p.sx = sx; p.sx_m = sx_m; p.sx_k = sx_k;
   p.sw = sw; p.sw_n = sw_n; p.sw_k = sw_k;
   p.bias = bias; p.y = y; p.ldy = ldy;
-  if (dtype == ZIB_BF16) return fp8::gemm<__nv_bfloat16>(p, q, ldq, w, ldw, K, dependent, st, what);
-  if (dtype == ZIB_F16) return fp8::gemm<__half>(p, q, ldq, w, ldw, K, dependent, st, what);
-  return fp8::gemm<float>(p, q, ldq, w, ldw, K, dependent, st, what);
+  if (dtype == ZIB_BF16) return fp8::gemm<__nv_bfloat16>(p, q, ldq, w, ldw, K, exponents, dependent, st, what);
+  if (dtype == ZIB_F16) return fp8::gemm<__half>(p, q, ldq, w, ldw, K, exponents, dependent, st, what);
+  return fp8::gemm<float>(p, q, ldq, w, ldw, K, exponents, dependent, st, what);
 }
 
 extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
@@ -895,6 +902,6 @@ extern "C" int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, i
                  ZIB_ERR_ALIGNMENT, "%s: q and w need 16-byte aligned rows", what);
   if (M == 0) return ZIB_OK;
   ZIB_HOST_CHECK(q && sx && w && sw && y, ZIB_ERR_INVALID_ARG, "%s: null operand", what);
-  return fp8_gemm(q, ldq, sx, sx_m, sx_k, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, false,
+  return fp8_gemm(q, ldq, sx, sx_m, sx_k, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, false, false,
                   (cudaStream_t)stream, what);
 }

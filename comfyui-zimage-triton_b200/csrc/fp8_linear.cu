@@ -291,7 +291,8 @@ extern "C" int zib_fp8_block_linear(const void* x, int64_t ldx, int dtype, const
     if (sum) fp8_sum_finish(part, sum, dtype, M, K, st);
   }
   if (!fp8::is_small(M, N, kb))
-    return fp8_gemm(scratch, ldq, s, 1, M, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, true, st, what);
+    return fp8_gemm(scratch, ldq, s, 1, M, w, ldw, sw, sw_n, sw_k, bias, y, ldy, dtype, M, N, K, true, true, st,
+                    what);
   const bool fused = sc.bytes == 0;
   const int size = dtype_bytes(dtype);
   fp8::SmallParams p{};

@@ -87,9 +87,10 @@ int fp8_quant_rows(const void* x, int64_t ldx, int dtype, void* q, int64_t ldq, 
                    float* part, int64_t M, int64_t K, cudaStream_t st, const char* what);
 int64_t fp8_sum_rows(int64_t M);
 void fp8_sum_finish(const float* part, void* sum, int dtype, int64_t M, int64_t K, cudaStream_t st);
-// the product on tensor cores (fp8_gemm.cu); dependent: q and sx come from the launch before
+// the product on tensor cores (fp8_gemm.cu); exponents: sx are powers of two (no subnormals) or NaN, as the
+// quantiser makes them; dependent: q and sx come from the launch before
 int fp8_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k, const void* w, int64_t ldw,
              const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, int dtype, int64_t M,
-             int64_t N, int64_t K, bool dependent, cudaStream_t st, const char* what);
+             int64_t N, int64_t K, bool exponents, bool dependent, cudaStream_t st, const char* what);
 
 }  // namespace zib
