@@ -23,7 +23,8 @@ def fp8_block_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
     A block of 128 values with largest magnitude a has the scale 2^e, e >= -120 the least with
     a <= 448 * 2^e, so x / scale is exact and rounded once (to nearest, ties to even).  A block with an
-    infinity or a NaN comes back NaN.  Rows of the values start on 16-byte boundaries.
+    infinity or a NaN comes back NaN.  Rows of the values start on 16-byte boundaries.  Rounding has no
+    gradient: the results are constants to autograd.
     """
     return _lib.ops().fp8_block_quantize(x)
 
@@ -42,8 +43,8 @@ def fp8_block_transpose(w_q: torch.Tensor) -> torch.Tensor:
 def fp8_block_matmul(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
                      bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The product of quantised operands: x_q e4m3 [..., K], x_scale fp32 [..., ceil(K/128)], w_q e4m3
-    [N, K], w_scale fp32 [ceil(N/128), ceil(K/128)] (any scales, not only powers of two), bias of
-    ``out_dtype`` [N] or None.  Sums in fp32, rounded once to ``out_dtype`` (bf16, fp16, fp32).  Not
+    [N, K], w_scale fp32 [ceil(N/128), ceil(K/128)] (any scales whose products stay within fp32's range,
+    not only powers of two), bias of ``out_dtype`` [N] or None.  Sums in fp32, rounded once to ``out_dtype`` (bf16, fp16, fp32).  Not
     differentiable (its operands are not); ``fp8_block_linear`` is."""
     return _lib.ops().fp8_block_matmul(x_q, x_scale, w_q, w_scale, bias, out_dtype)
 

@@ -335,7 +335,7 @@ ZIB_API int zib_fp8_quant_blocks(const void* w, int64_t ldw, int dtype, void* q,
 /* y[m,n] = sum_b sx[m,b] * sw[n/128,b] * sum_{k in block b} q[m,k] w[n,k] (+ bias[n]),
  * fp32 sums, rounded once to `dtype` (of y and bias).  q: e4m3 [M,K] row stride
  * ldq; w: e4m3 [N,K] row stride ldw; both with 16-byte aligned rows.  sx, sw: any
- * fp32 scales, strided as above. */
+ * fp32 scales whose products stay within fp32's range, strided as above. */
 ZIB_API int zib_fp8_block_gemm(const void* q, int64_t ldq, const float* sx, int64_t sx_m, int64_t sx_k,
                        const void* w, int64_t ldw, const float* sw, int64_t sw_n, int64_t sw_k,
                        const void* bias, void* y, int64_t ldy, int dtype, int64_t M, int64_t N,
@@ -377,7 +377,8 @@ ZIB_API int zib_col_sum(const void* x, int64_t ldx, int dtype, void* y, float* w
  * (int64 if pos64, else int32; strides ps_b, ps_s), or s where positions is
  * NULL.  inverse turns the other way (the gradient).  A position outside
  * [0, L) reads no table row: its turned features are NaN and the device error
- * word becomes ZIB_ERR_INVALID_ARG. */
+ * word becomes ZIB_ERR_INVALID_ARG.  The interleaved layout moves pairs: even
+ * strides and operands aligned to two elements (else ZIB_ERR_ALIGNMENT). */
 ZIB_API int zib_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, void* q_out, int64_t Hq,
                const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh, void* k_out, int64_t Hk,
                int dtype, const float* cos, const float* sin, int64_t cs_b, int64_t cs_l, int64_t L,
