@@ -224,7 +224,9 @@ constexpr float kRadians = 1.4629180792671596e-09f;  // 2 pi / 2^32
 
 // cos and sin of such an angle: the quarter decides which of them is which and their signs, exactly, in
 // integers; the rest goes through the Taylor series of sine (to x^9) and cosine (to x^10), whose next
-// terms are below 2e-9 and 2e-10 there.
+// terms are below 2e-9 and 2e-10 there.  One fp32 for the rest leaves values 2.9e-8 off in the mean (1e-7 at
+// most), where the rounding to fp32 alone leaves 2.1e-8; carrying its rounding error too gave 2.2e-8 (6.6e-8) and
+// took 35 us instead of 27 for 131072 x 64.
 __device__ __forceinline__ void sincos_turns(uint64_t a, float& s, float& c) {
   const uint32_t quarter = quarter_of(a);
   const float x = fmaf(low_rest(a), kLow, high_rest(a, quarter)) * kRadians;
