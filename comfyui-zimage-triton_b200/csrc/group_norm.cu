@@ -107,8 +107,8 @@ using px::f2;
 // --- activation ------------------------------------------------------------------
 
 // 1 / (1 + e^-z): the accurate functions where x, and so the outputs, have 32 bits; where they have 16, the fast
-// power of two and reciprocal, off by at most 2^-22 + 2^-23 + |z| 2^-24 of the value (two functions, the rounded
-// exponent) and 0 below 2^-126.  That is 2^-13 of a 16-bit step, and what the gradients of 32-bit parameters, sums
+// power of two and reciprocal, off by about 2^-22 + 2^-23 + |z| 2^-24 of the value (two functions, the rounded
+// exponent) at worst and 0 below 2^-126.  That is 2^-13 of a 16-bit step, and what the gradients of 32-bit parameters, sums
 // over such terms, then carry.
 template <typename T>
 __device__ __forceinline__ f2 sigmoid(f2 z) {

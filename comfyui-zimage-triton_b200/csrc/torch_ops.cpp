@@ -272,12 +272,13 @@ Tensor linear(const Tensor& x, const Tensor& w, const Tensor& s, int64_t sn, int
 }
 
 struct Linear : torch::autograd::Function<Linear> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& bias, const Tensor& w,
+  // w_q is kept as it came (an aligned copy of it lives for the call alone), and only where it is needed again
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& bias, const Tensor& w_q,
                         const Tensor& s, const OptTensor& wt) {
-    ctx->save_for_backward({w, s, wt ? *wt : Tensor()});
+    ctx->save_for_backward({wt ? Tensor() : w_q, s, wt ? *wt : Tensor()});
     ctx->saved_data["x"] = wants_grad(x);
     ctx->saved_data["bias"] = wants_grad(bias);
-    return linear(x, w, s, s.stride(0), s.stride(1), bias, Tensor());
+    return linear(x, aligned(w_q), s, s.stride(0), s.stride(1), bias, Tensor());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(),
@@ -286,7 +287,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const auto saved = ctx->get_saved_variables();
     const Tensor dy = grads[0].resolve_neg();
     const Tensor &w = saved[0], &s = saved[1];
-    const int64_t N = w.size(0);
+    const int64_t N = dy.size(-1);
     Tensor dx, db;
     if (ctx->saved_data["bias"].toBool()) db = at::empty({N}, dy.options());
     if (ctx->saved_data["x"].toBool()) {  // the pass that quantises dy adds up its columns too
@@ -324,9 +325,8 @@ Tensor fp8_block_linear(const Tensor& x, const Tensor& w_q, const Tensor& w_scal
   TORCH_CHECK_VALUE(!grad || !(w_q.requires_grad() || w_scale.requires_grad()),
                     "the quantised weight of fp8_block_linear is a constant and must not require gradients");
   const OptTensor bias = bias_ && !bias_->is_contiguous() ? OptTensor(bias_->contiguous()) : bias_;
-  const Tensor w = aligned(w_q);
-  if (grad && (wants_grad(x) || wants_grad(bias))) return Linear::apply(x, bias, w, w_scale, w_q_t);
-  return linear(x, w, w_scale, w_scale.stride(0), w_scale.stride(1), bias, Tensor());
+  if (grad && (wants_grad(x) || wants_grad(bias))) return Linear::apply(x, bias, w_q, w_scale, w_q_t);
+  return linear(x, aligned(w_q), w_scale, w_scale.stride(0), w_scale.stride(1), bias, Tensor());
 }
 
 // --- rotary positions ------------------------------------------------------------------

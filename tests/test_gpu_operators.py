@@ -1321,3 +1321,24 @@ def test_views_that_read_as_negatives_are_refused(cuda):
         d = _randn(g, *y.shape)
         a, b = (torch.autograd.grad(y, (xs,), t, retain_graph=True)[0] for t in (neg(d), -d))
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("laid_out", [False, True])
+def test_linear_keeps_no_copy_of_the_weight(cuda, laid_out):
+    """A weight whose rows are copied to aligned ones: the copy ends with the call, not with the backward pass."""
+    g = _gen(107)
+    M, K, N = 4, 2001, 1000
+    wq, ws = fp8_block_quantize_weight(_randn(g, N, K))
+    w = wq.contiguous()
+    wt = fp8_block_transpose(wq) if laid_out else None
+    x = _randn(g, M, K).to(torch.bfloat16).requires_grad_()
+    y = fp8_block_linear(x, w, ws, w_q_t=wt)
+    del y
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = fp8_block_linear(x, w, ws, w_q_t=wt)
+    assert torch.cuda.memory_allocated() - before < 1 << 20 < w.numel()
+    d = _randn(g, M, N).to(torch.bfloat16)
+    (dx,) = torch.autograd.grad(y, (x,), d)
+    ref, mag = product_terms(*ref_rows(d), wq.t(), ws.t())
+    check(dx, ref, product_extra(mag, N))
