@@ -851,14 +851,17 @@ static int gemm(GemmParams p, const void* q, int64_t ldq, const void* w, int64_t
   if (exponents) {
     // The tensor cores apply the scales where that and the second launch, which then ends at once, are sooner.
     // A call there takes 5 us more than here, and each wave 0.27 us a K-block and 0.6 us; here each wave 0.54 us a
-    // K-block and 0.6 us (wide) or 0.34 us a K-block (slim).  Fitted to 400 calls of 256 to 9216 rows, both sides
-    // timed in turns: by this rule a call takes 0.2% more than on its faster side on average.  With bias, the
-    // tensor cores' scales / sums in registers: 4608 x 2560 -> 3840 56 / 69 us, 4608 x 3840 -> 2560 60 / 76, 768 x
-    // 2560 -> 3840 26 / 26, 512 x 3840 -> 7680 38 / 31, 2304 x 512 -> 11520 47 / 41, and the wrong way 256 x 3840 ->
-    // 11520 34 / 30 (few rows: bound by the weight's way from memory).
+    // K-block and 0.6 us (wide) or 0.34 us a K-block (slim).  16-bit rows of y that start on any element leave by
+    // elements, there through four warps instead of eight: 1 us more a wave.  Fitted to 1600 calls of 256 to 18226
+    // rows, aligned or not, in 16 and 32 bits, both sides timed in turns: by this rule a call takes 0.1 to 0.6% more
+    // than on its faster side on average.  bf16 with bias, the tensor cores' scales / sums in registers: 4608 x
+    // 2560 -> 3840 56 / 69 us, 4608 x 3840 -> 2560 60 / 76, 768 x 2560 -> 3840 26 / 26, 512 x 3840 -> 7680 38 / 31, 2304 x
+    // 512 -> 11520 47 / 41, 18226 x 512 -> 4071 173 / 143, and the wrong way 256 x 3840 -> 11520 34 / 30 (few rows: bound
+    // by the weight's way from memory).
     const int64_t mx = ceil_div(mb * ceil_div(p.N, Mx::BN), pairs);
     const int64_t sums = slim < wide ? 34 * kb * slim : (27 * kb + 30) * wide;
-    if (500 + (27 * kb + 60) * mx < sums) {
+    const bool elements = sizeof(T) == 2 && ((uintptr_t)p.y % 16 != 0 || p.ldy * sizeof(T) % 16 != 0);
+    if (500 + (27 * kb + (elements ? 160 : 60)) * mx < sums) {
       const int rc = launch_pair<T, Mx::BN, true>(p, q, ldq, w, ldw, K, dependent, st, what);
       if (rc) return rc;
       p.where = 1;
