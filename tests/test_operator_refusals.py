@@ -1,5 +1,4 @@
-"""The operators' host side: what the block-scaled 8-bit products, rotary positions and group normalisation refuse
-before any launch, and how the linear layer keeps its weight."""
+"""What the block-scaled 8-bit products, rotary positions and group normalisation refuse, before any launch."""
 
 import math
 
